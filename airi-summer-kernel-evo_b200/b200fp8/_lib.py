@@ -213,6 +213,94 @@ class HeadPrepArgs(ctypes.Structure):
     ]
 
 
+class RotaryArgs(ctypes.Structure):
+    """Mirror of ``b2f_rotary_args`` (include/b200fp8.h)."""
+
+    _fields_ = [
+        ("rows", ctypes.c_int), ("q_heads", ctypes.c_int), ("k_heads", ctypes.c_int),
+        ("head_dim", ctypes.c_int), ("rotary_dim", ctypes.c_int),
+        ("interleaved", ctypes.c_int), ("inverse", ctypes.c_int),
+        ("q", ctypes.c_void_p), ("q_ld", ctypes.c_longlong), ("q_head_stride", ctypes.c_longlong),
+        ("k", ctypes.c_void_p), ("k_ld", ctypes.c_longlong), ("k_head_stride", ctypes.c_longlong),
+        ("in_dtype", ctypes.c_int), ("in_scale", ctypes.c_float),
+        ("q_weight", ctypes.c_void_p), ("k_weight", ctypes.c_void_p),
+        ("weight_offset", ctypes.c_float), ("eps", ctypes.c_float),
+        ("positions", ctypes.c_void_p), ("position_bits", ctypes.c_int),
+        ("freqs", ctypes.c_void_p), ("magnitude", ctypes.c_float),
+        ("q_out", ctypes.c_void_p), ("q_out_ld", ctypes.c_longlong),
+        ("k_out", ctypes.c_void_p), ("k_out_ld", ctypes.c_longlong),
+        ("out_dtype", ctypes.c_int), ("out_scale", ctypes.c_float),
+    ]
+
+
+class Kv4Cache(ctypes.Structure):
+    """Mirror of ``b2f_kv4_cache``."""
+
+    _fields_ = [
+        ("storage", ctypes.c_void_p), ("page_stride", ctypes.c_longlong),
+        ("pages", ctypes.c_int), ("kv_heads", ctypes.c_int), ("head_dim", ctypes.c_int),
+        ("page_size", ctypes.c_int), ("k_scale", ctypes.c_float), ("v_scale", ctypes.c_float),
+        ("table", ctypes.c_void_p), ("table_rows", ctypes.c_int), ("table_cols", ctypes.c_int),
+        ("table_ld", ctypes.c_longlong), ("lens", ctypes.c_void_p),
+    ]
+
+
+class Kv4Batch(ctypes.Structure):
+    """Mirror of ``b2f_kv4_batch``."""
+
+    _fields_ = [("seqs", ctypes.c_int), ("tokens", ctypes.c_int), ("rows", ctypes.c_void_p),
+                ("starts", ctypes.c_void_p)]
+
+
+class Kv4WriteArgs(ctypes.Structure):
+    """Mirror of ``b2f_kv4_write_args``."""
+
+    _fields_ = [
+        ("cache", Kv4Cache), ("batch", Kv4Batch),
+        ("k", ctypes.c_void_p), ("k_ld", ctypes.c_longlong), ("k_in_scale", ctypes.c_float),
+        ("v", ctypes.c_void_p), ("v_ld", ctypes.c_longlong), ("v_in_scale", ctypes.c_float),
+        ("dtype", ctypes.c_int),
+    ]
+
+
+class Kv4ReadArgs(ctypes.Structure):
+    """Mirror of ``b2f_kv4_read_args``."""
+
+    _fields_ = [
+        ("cache", Kv4Cache), ("batch", Kv4Batch),
+        ("k", ctypes.c_void_p), ("k_ld", ctypes.c_longlong),
+        ("v", ctypes.c_void_p), ("v_ld", ctypes.c_longlong), ("dtype", ctypes.c_int),
+    ]
+
+
+class Kv4AttnArgs(ctypes.Structure):
+    """Mirror of ``b2f_kv4_attn_args``."""
+
+    _fields_ = [
+        ("cache", Kv4Cache), ("batch", Kv4Batch), ("heads", ctypes.c_int),
+        ("causal", ctypes.c_int),
+        ("q", ctypes.c_void_p), ("q_dtype", ctypes.c_int), ("q_ld", ctypes.c_longlong),
+        ("q_scale", ctypes.c_float), ("sm_scale", ctypes.c_float),
+        ("gate", ctypes.c_void_p), ("gate_dtype", ctypes.c_int), ("gate_ld", ctypes.c_longlong),
+        ("gate_head_stride", ctypes.c_longlong), ("gate_scale", ctypes.c_float),
+        ("out", ctypes.c_void_p), ("out_dtype", ctypes.c_int), ("out_ld", ctypes.c_longlong),
+        ("ctx_scale", ctypes.c_float), ("lse", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_longlong),
+    ]
+
+
+class Kv4Pool(ctypes.Structure):
+    """Mirror of ``b2f_kv4_pool``."""
+
+    _fields_ = [
+        ("storage", ctypes.c_void_p), ("layer_stride", ctypes.c_longlong),
+        ("page_stride", ctypes.c_longlong), ("layers", ctypes.c_int), ("pages", ctypes.c_int),
+        ("page_size", ctypes.c_int), ("page_bytes", ctypes.c_int),
+        ("table", ctypes.c_void_p), ("table_rows", ctypes.c_int), ("table_cols", ctypes.c_int),
+        ("table_ld", ctypes.c_longlong), ("lens", ctypes.c_void_p), ("refs", ctypes.c_void_p),
+    ]
+
+
 class Op(ctypes.Structure):
     """Mirror of ``b2f_op``."""
 
@@ -235,6 +323,11 @@ EXPORTED_SYMBOLS = (
     "b2f_lnrows_args_init", "b2f_layer_norm_rows_workspace_bytes", "b2f_layer_norm_rows",
     "b2f_gpt2_block_args_init", "b2f_gpt2_block_workspace_bytes", "b2f_gpt2_block",
     "b2f_qwen_block_args_init", "b2f_qwen_block_workspace_bytes", "b2f_qwen_block",
+    "b2f_rotary_args_init", "b2f_rotary",
+    "b2f_kv4_write_args_init", "b2f_kv4_write", "b2f_kv4_read_args_init", "b2f_kv4_read",
+    "b2f_kv4_attn_args_init", "b2f_kv4_attention_workspace_bytes", "b2f_kv4_attention",
+    "b2f_kv4_extend", "b2f_kv4_fork_workspace_bytes", "b2f_kv4_fork", "b2f_kv4_free",
+    "b2f_kv4_compact_workspace_bytes", "b2f_kv4_compact", "b2f_kv4_copy_pages",
     "b2f_registry_lookup", "b2f_registry_size", "b2f_registry_at",
 )
 
@@ -303,6 +396,28 @@ def _declare(lib: ctypes.CDLL) -> None:
                                    ctypes.c_longlong, ctypes.c_int, ctypes.c_int, ctypes.c_float,
                                    ctypes.c_float, vp]
     lib.b2f_swiglu_fp8.restype = ctypes.c_int
+    for nm, st in (("rotary", RotaryArgs), ("kv4_write", Kv4WriteArgs), ("kv4_read", Kv4ReadArgs)):
+        getattr(lib, f"b2f_{nm}_args_init").argtypes = [ctypes.POINTER(st)]
+        getattr(lib, f"b2f_{nm}_args_init").restype = None
+        getattr(lib, f"b2f_{nm}").argtypes = [ctypes.POINTER(st), vp]
+        getattr(lib, f"b2f_{nm}").restype = ctypes.c_int
+    lib.b2f_kv4_attn_args_init.argtypes = [ctypes.POINTER(Kv4AttnArgs)]
+    lib.b2f_kv4_attn_args_init.restype = None
+    lib.b2f_kv4_attention_workspace_bytes.argtypes = [ctypes.c_int]
+    lib.b2f_kv4_attention_workspace_bytes.restype = ctypes.c_longlong
+    lib.b2f_kv4_attention.argtypes = [ctypes.POINTER(Kv4AttnArgs), vp]
+    lib.b2f_kv4_attention.restype = ctypes.c_int
+    pool = ctypes.POINTER(Kv4Pool)
+    lib.b2f_kv4_extend.argtypes = [pool, vp, vp, ctypes.c_int, vp]
+    lib.b2f_kv4_fork.argtypes = [pool, vp, vp, ctypes.c_int, vp, ctypes.c_longlong, vp]
+    lib.b2f_kv4_free.argtypes = [pool, vp, ctypes.c_int, vp]
+    lib.b2f_kv4_compact.argtypes = [pool, vp, ctypes.c_longlong, vp]
+    lib.b2f_kv4_copy_pages.argtypes = [pool, vp, vp, ctypes.c_int, vp]
+    for nm in ("extend", "fork", "free", "compact", "copy_pages"):
+        getattr(lib, f"b2f_kv4_{nm}").restype = ctypes.c_int
+    for nm in ("fork", "compact"):
+        getattr(lib, f"b2f_kv4_{nm}_workspace_bytes").argtypes = [ctypes.c_int]
+        getattr(lib, f"b2f_kv4_{nm}_workspace_bytes").restype = ctypes.c_longlong
     lib.b2f_registry_lookup.argtypes = [ctypes.c_char_p]
     lib.b2f_registry_lookup.restype = ctypes.POINTER(Op)
     lib.b2f_registry_size.restype = ctypes.c_int

@@ -1,0 +1,313 @@
+"""Paged key / value cache at 4.5 bits an element, and the attention that reads it.
+
+Pages of 16, 32 or 64 tokens; e2m1 codes with one e4m3 scale for 16 consecutive elements of a
+head and an f32 scale for all keys and for all values (include/b200fp8.h has the layout).
+Every list that changes while a model runs (table, lengths, use counts) lives on the device,
+no call waits for the GPU, and all calls can be captured in CUDA graphs (copy_pages with the
+pages that it was given then).
+
+A step of a serving loop:
+
+    cache.extend(rows, counts)                  # pages for the new tokens
+    q, k = ops.rotary(q, k, positions, plan, ...)
+    cache.write(k, v, layer=l, rows=rows)
+    ctx = cache.attention(q, heads=h, layer=l, rows=rows)
+
+What a call on the device finds wrong (a row out of range, too few pages) it leaves undone and
+records in the device status word (:func:`b200fp8.device_status`: 5 bad lists, 6 no pages).
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional, Sequence, Tuple
+
+import torch
+
+from . import _lib
+from ._lib import check
+from .ops import _DT, _stream
+
+_PAGE_SIZES = (16, 32, 64)
+_HEAD_DIMS = (64, 128, 256)
+
+
+class Fp4Cache:
+    """``layers`` x ``pages`` pages of ``page_size`` tokens of ``kv_heads`` heads, and a table of
+    ``max_seqs`` sequences of at most ``max_pages`` pages each."""
+
+    def __init__(self, *, layers: int, pages: int, page_size: int, kv_heads: int, head_dim: int,
+                 max_seqs: int, max_pages: int, k_scale: float = 1.0, v_scale: float = 1.0,
+                 device="cuda"):
+        if page_size not in _PAGE_SIZES or head_dim not in _HEAD_DIMS:
+            raise ValueError("page_size must be 16, 32 or 64 and head_dim 64, 128 or 256")
+        block = page_size * head_dim * 9 // 8
+        i32 = dict(dtype=torch.int32, device=device)
+        self._init(torch.zeros((layers, pages, kv_heads, block), dtype=torch.uint8, device=device),
+                   torch.full((max_seqs, max_pages), -1, **i32), torch.zeros(max_seqs, **i32),
+                   torch.zeros(pages, **i32), page_size, head_dim, k_scale, v_scale)
+
+    @classmethod
+    def from_buffers(cls, storage: torch.Tensor, table: torch.Tensor, lens: torch.Tensor,
+                     refs: torch.Tensor, *, page_size: int, head_dim: int, k_scale: float = 1.0,
+                     v_scale: float = 1.0) -> "Fp4Cache":
+        """A cache over the caller's buffers: ``storage`` uint8 [layers, pages, kv_heads,
+        page_size * head_dim * 9 / 8], ``table`` int32 [seqs, pages of a sequence], ``lens``
+        int32 [seqs], ``refs`` int32 [pages] (the number of table rows that use a page)."""
+        self = cls.__new__(cls)
+        self._init(storage, table, lens, refs, page_size, head_dim, k_scale, v_scale)
+        return self
+
+    def _init(self, storage, table, lens, refs, page_size, head_dim, k_scale, v_scale):
+        if page_size not in _PAGE_SIZES or head_dim not in _HEAD_DIMS:
+            raise ValueError("page_size must be 16, 32 or 64 and head_dim 64, 128 or 256")
+        block = page_size * head_dim * 9 // 8
+        if (storage.dtype != torch.uint8 or storage.dim() != 4 or storage.shape[3] != block
+                or storage.stride(3) != 1 or storage.stride(2) != block):
+            raise ValueError(f"storage must be uint8 [layers, pages, kv_heads, {block}], its pages "
+                             "in one piece")
+        for t, dim in ((table, 2), (lens, 1), (refs, 1)):
+            if t.dtype != torch.int32 or t.dim() != dim or t.stride(-1) != 1:
+                raise TypeError("table, lens and refs must be int32 of 2, 1 and 1 dimensions, "
+                                "rows in one piece")
+        if lens.shape[0] != table.shape[0] or refs.shape[0] != storage.shape[1]:
+            raise ValueError("lens goes by the table's rows, refs by the storage's pages")
+        if not storage.is_cuda or any(t.device != storage.device for t in (table, lens, refs)):
+            raise ValueError("b200fp8 ops take CUDA tensors only (no CPU fallback), of one device")
+        self.storage, self.table, self.lens, self.refs = storage, table, lens, refs
+        self.layers, self.pages, self.kv_heads = storage.shape[:3]
+        self.page_size, self.head_dim = page_size, head_dim
+        self.k_scale, self.v_scale = float(k_scale), float(v_scale)
+        self.device = storage.device
+        c = _lib.Kv4Cache()
+        c.page_stride, c.pages, c.kv_heads = storage.stride(1), self.pages, self.kv_heads
+        c.head_dim, c.page_size = head_dim, page_size
+        c.k_scale, c.v_scale = self.k_scale, self.v_scale
+        c.table, c.table_rows, c.table_cols = table.data_ptr(), *table.shape
+        c.table_ld, c.lens = table.stride(0), lens.data_ptr()
+        self._cache = c
+        p = _lib.Kv4Pool()
+        p.storage, p.layer_stride, p.page_stride = (storage.data_ptr(), storage.stride(0),
+                                                    storage.stride(1))
+        p.layers, p.pages, p.page_size = self.layers, self.pages, page_size
+        p.page_bytes = self.kv_heads * block
+        p.table, p.table_rows, p.table_cols = table.data_ptr(), *table.shape
+        p.table_ld, p.lens, p.refs = table.stride(0), lens.data_ptr(), refs.data_ptr()
+        self._pool = p
+        self._work_bytes = None
+
+    # ------------------------------------------------------------------ helpers
+
+    def _run(self, fn, *args) -> None:
+        """Calls ``fn(*args, stream)`` with this cache's device current, on its current stream."""
+        if torch.cuda.current_device() == self.device.index:
+            check(fn(*args, _stream()))
+        else:
+            with torch.cuda.device(self.device):
+                check(fn(*args, _stream()))
+
+    def _here(self, *tensors: Optional[torch.Tensor]) -> None:
+        for t in tensors:
+            if t is not None and t.device != self.device:
+                if not t.is_cuda:
+                    raise ValueError("b200fp8 ops take CUDA tensors only (no CPU fallback)")
+                raise ValueError(f"tensor on {t.device}, the cache is on {self.device}")
+
+    def _list(self, t: Optional[torch.Tensor], name: str) -> None:
+        if t is not None and (t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous()):
+            raise TypeError(f"{name} must be a contiguous int32 vector")
+
+    def _fill(self, a, layer: int, tokens: int, rows, starts) -> None:
+        """Cache and batch of an argument block."""
+        if not 0 <= layer < self.layers:
+            raise ValueError(f"layer {layer} of {self.layers}")
+        self._here(rows, starts)
+        self._list(rows, "rows")
+        self._list(starts, "starts")
+        seqs = rows.shape[0] if rows is not None else (
+            starts.shape[0] - 1 if starts is not None else self.table.shape[0])
+        if starts is not None and starts.shape[0] != seqs + 1:
+            raise ValueError("starts must have one entry more than there are sequences")
+        if starts is None and (seqs == 0 or tokens % seqs):
+            raise ValueError("without starts, every sequence has the same number of new tokens")
+        a.cache = self._cache
+        a.cache.storage = self.storage.data_ptr() + layer * self.storage.stride(0)
+        b = a.batch
+        b.seqs, b.tokens = seqs, tokens
+        b.rows = None if rows is None else rows.data_ptr()
+        b.starts = None if starts is None else starts.data_ptr()
+
+    def _matrix(self, t: torch.Tensor, name: str, heads: int, dtypes) -> None:
+        if t.dim() != 2 or t.stride(1) != 1 or t.shape[1] != heads * self.head_dim:
+            raise ValueError(f"{name} must be a row-major [tokens, {heads * self.head_dim}] tensor")
+        if t.dtype not in dtypes:
+            raise TypeError(f"{name} must be one of {[str(d) for d in dtypes]}")
+
+    # ------------------------------------------------------------------ tokens
+
+    def write(self, k: torch.Tensor, v: torch.Tensor, *, layer: int = 0,
+              rows: Optional[torch.Tensor] = None, starts: Optional[torch.Tensor] = None,
+              k_in_scale: float = 1.0, v_in_scale: float = 1.0) -> None:
+        """Quantises the new tokens' keys and values ([tokens, kv_heads * head_dim], both f32,
+        bf16, f16 or e4m3; value = stored * in_scale) into their places: token i of the n of a
+        sequence at position length - n + i.  ``starts`` int32 [seqs + 1] cuts the packed
+        tokens into sequences (None: equal parts), ``rows`` int32 [seqs] names their table
+        rows (None: in order; distinct)."""
+        self._here(k, v)
+        kinds = (torch.float32, torch.bfloat16, torch.float16, torch.float8_e4m3fn, torch.uint8)
+        self._matrix(k, "k", self.kv_heads, kinds)
+        self._matrix(v, "v", self.kv_heads, kinds)
+        if k.shape != v.shape or k.dtype != v.dtype:
+            raise ValueError("k and v must have one shape and type")
+        if k.shape[0] == 0:
+            return
+        a = _lib.Kv4WriteArgs()
+        self._fill(a, layer, k.shape[0], rows, starts)
+        a.k, a.k_ld, a.k_in_scale = k.data_ptr(), k.stride(0), k_in_scale
+        a.v, a.v_ld, a.v_in_scale = v.data_ptr(), v.stride(0), v_in_scale
+        a.dtype = _DT[k.dtype]
+        self._run(_lib.lib().b2f_kv4_write, ctypes.byref(a))
+
+    def read(self, tokens: int, *, layer: int = 0, rows: Optional[torch.Tensor] = None,
+             starts: Optional[torch.Tensor] = None, dtype: torch.dtype = torch.bfloat16,
+             k: Optional[torch.Tensor] = None, v: Optional[torch.Tensor] = None
+             ) -> Tuple[torch.Tensor, torch.Tensor]:
+        """The values that the cache holds for the last tokens of the sequences, placed as in
+        :meth:`write`: (k, v), [tokens, kv_heads * head_dim] each, f32, bf16 or f16.  Rows of
+        given ``k`` / ``v`` that belong to no sequence are left as they are."""
+        cols = self.kv_heads * self.head_dim
+        if k is None:
+            k = torch.empty((tokens, cols), dtype=dtype, device=self.device)
+        if v is None:
+            v = torch.empty((tokens, cols), dtype=k.dtype, device=self.device)
+        self._here(k, v)
+        kinds = (torch.float32, torch.bfloat16, torch.float16)
+        self._matrix(k, "k", self.kv_heads, kinds)
+        self._matrix(v, "v", self.kv_heads, kinds)
+        if k.shape != v.shape or k.dtype != v.dtype or k.shape[0] != tokens:
+            raise ValueError("k and v must have one type and [tokens, kv_heads * head_dim] elements")
+        if tokens == 0:
+            return k, v
+        a = _lib.Kv4ReadArgs()
+        self._fill(a, layer, tokens, rows, starts)
+        a.k, a.k_ld, a.v, a.v_ld = k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0)
+        a.dtype = _DT[k.dtype]
+        self._run(_lib.lib().b2f_kv4_read, ctypes.byref(a))
+        return k, v
+
+    def attention(self, q: torch.Tensor, *, heads: int, layer: int = 0,
+                  rows: Optional[torch.Tensor] = None, starts: Optional[torch.Tensor] = None,
+                  causal: bool = True, q_scale: float = 1.0, sm_scale: float = 0.0,
+                  gate: Optional[torch.Tensor] = None, gate_scale: float = 1.0,
+                  gate_head_stride: Optional[int] = None, out: Optional[torch.Tensor] = None,
+                  out_dtype: torch.dtype = torch.bfloat16, ctx_scale: float = 1.0,
+                  return_lse: bool = False, lse: Optional[torch.Tensor] = None):
+        """Attention of the new tokens ([tokens, heads * head_dim]; bf16, f16, or e4m3 with
+        value = stored * q_scale) over the cached keys of their sequences, the new ones among
+        them (see b2f_kv4_attention).  ``out`` bf16, f16 or e4m3 (stored = value / ctx_scale).
+        With ``return_lse`` returns (out, lse f32 [tokens, heads])."""
+        self._here(q, gate, out, lse)
+        kinds = (torch.bfloat16, torch.float16, torch.float8_e4m3fn, torch.uint8)
+        self._matrix(q, "q", heads, kinds)
+        tokens = q.shape[0]
+        if out is None:
+            out = torch.empty((tokens, heads * self.head_dim), dtype=out_dtype, device=self.device)
+        self._matrix(out, "out", heads, kinds)
+        if out.shape[0] != tokens:
+            raise ValueError("out must have a row for every token")
+        if return_lse and lse is None:
+            lse = torch.empty((tokens, heads), dtype=torch.float32, device=self.device)
+        if lse is not None and (lse.dtype != torch.float32 or lse.shape != (tokens, heads)
+                                or not lse.is_contiguous()):
+            raise ValueError("lse must be contiguous float32 [tokens, heads]")
+        if gate is not None and (gate.dim() != 2 or gate.stride(1) != 1 or gate.shape[0] != tokens
+                                 or gate.dtype not in (torch.float8_e4m3fn, torch.uint8,
+                                                       torch.bfloat16)):
+            raise ValueError("gate must be row-major e4m3 or bf16 with a row for every token")
+        if tokens == 0:
+            return (out, lse) if return_lse else out
+        a = _lib.Kv4AttnArgs()
+        self._fill(a, layer, tokens, rows, starts)
+        a.heads, a.causal = heads, 1 if causal else 0
+        a.q, a.q_dtype, a.q_ld, a.q_scale = q.data_ptr(), _DT[q.dtype], q.stride(0), q_scale
+        a.sm_scale = sm_scale
+        if gate is not None:
+            a.gate, a.gate_dtype, a.gate_ld = gate.data_ptr(), _DT[gate.dtype], gate.stride(0)
+            a.gate_head_stride = self.head_dim if gate_head_stride is None else gate_head_stride
+            if gate.shape[1] < (heads - 1) * a.gate_head_stride + self.head_dim:
+                raise ValueError("gate has too few columns")
+        a.gate_scale = gate_scale
+        a.out, a.out_dtype, a.out_ld, a.ctx_scale = (out.data_ptr(), _DT[out.dtype], out.stride(0),
+                                                     ctx_scale)
+        a.lse = None if lse is None else lse.data_ptr()
+        # A workspace of this call's own, from the caching allocator of the current stream: calls
+        # on other streams, and in graphs, never share it.
+        if self._work_bytes is None:
+            with torch.cuda.device(self.device):
+                self._work_bytes = int(_lib.lib().b2f_kv4_attention_workspace_bytes(self.head_dim))
+        work = torch.empty(self._work_bytes, dtype=torch.uint8, device=self.device)
+        a.workspace, a.workspace_bytes = work.data_ptr(), self._work_bytes
+        self._run(_lib.lib().b2f_kv4_attention, ctypes.byref(a))
+        return (out, lse) if return_lse else out
+
+    # ------------------------------------------------------------------ pages
+
+    def extend(self, counts: torch.Tensor, rows: Optional[torch.Tensor] = None) -> None:
+        """Lengthens rows (None: rows 0 .. n - 1) by ``counts`` tokens (int32 [n], n <= 1024) and
+        gives them the pages for it, or does nothing when the pages do not suffice."""
+        self._here(counts, rows)
+        self._list(counts, "counts")
+        self._list(rows, "rows")
+        if rows is not None and rows.shape != counts.shape:
+            raise ValueError("rows and counts must have one length")
+        if counts.shape[0]:
+            self._run(_lib.lib().b2f_kv4_extend, ctypes.byref(self._pool),
+                      None if rows is None else rows.data_ptr(), counts.data_ptr(),
+                      counts.shape[0])
+
+    def fork(self, src: torch.Tensor, dst: torch.Tensor) -> None:
+        """Makes the empty rows ``dst`` copies of rows ``src`` (int32 [n]; src may repeat): full
+        pages are shared, a last page that is not full is copied."""
+        self._here(src, dst)
+        self._list(src, "src")
+        self._list(dst, "dst")
+        n = src.shape[0]
+        if dst.shape[0] != n:
+            raise ValueError("src and dst must have one length")
+        if n:
+            work = torch.empty(n + 1, dtype=torch.int32, device=self.device)
+            self._run(_lib.lib().b2f_kv4_fork, ctypes.byref(self._pool), src.data_ptr(),
+                      dst.data_ptr(), n, work.data_ptr(), 4 * (n + 1))
+
+    def free(self, rows: Optional[torch.Tensor] = None) -> None:
+        """Empties ``rows`` (int32 [n]; None: all); pages that no other row uses become free."""
+        self._here(rows)
+        self._list(rows, "rows")
+        if rows is not None and rows.shape[0]:
+            self._run(_lib.lib().b2f_kv4_free, ctypes.byref(self._pool), rows.data_ptr(),
+                      rows.shape[0])
+        elif rows is None:
+            every = torch.arange(self.table.shape[0], dtype=torch.int32, device=self.device)
+            for part in every.split(1024):
+                self._run(_lib.lib().b2f_kv4_free, ctypes.byref(self._pool), part.data_ptr(),
+                          part.shape[0])
+
+    def compact(self) -> None:
+        """Moves the pages in use to the front of the pool; the table follows."""
+        n = int(_lib.lib().b2f_kv4_compact_workspace_bytes(self.pages))
+        work = torch.empty(n, dtype=torch.uint8, device=self.device)
+        self._run(_lib.lib().b2f_kv4_compact, ctypes.byref(self._pool), work.data_ptr(), n)
+
+    def copy_pages(self, src: Sequence[int], dst: Sequence[int]) -> None:
+        """Copies pages ``src[i]`` to ``dst[i]`` in all layers (host lists); table and counts
+        stay as they are."""
+        n = len(src)
+        if len(dst) != n:
+            raise ValueError("src and dst must have one length")
+        if n:
+            ints = ctypes.c_int * n
+            self._run(_lib.lib().b2f_kv4_copy_pages, ctypes.byref(self._pool), ints(*src),
+                      ints(*dst), n)
+
+    def free_pages(self) -> int:
+        """Pages that no row uses (waits for the device)."""
+        return int((self.refs == 0).sum().item())

@@ -467,6 +467,82 @@ def attn_prep(q_src: torch.Tensor, k_src: torch.Tensor, v_src: Optional[torch.Te
     return True
 
 
+def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, plan, *,
+           heads: int, kv_heads: int = 0, q_head_stride: Optional[int] = None,
+           k_head_stride: Optional[int] = None, in_scale: float = 1.0,
+           q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None,
+           weight_offset: float = 1.0, eps: float = 1e-6, inverse: bool = False,
+           q_out: Optional[torch.Tensor] = None, k_out: Optional[torch.Tensor] = None,
+           out_dtype: Optional[torch.dtype] = None, out_scale: float = 1.0):
+    """Rotary positions of q and k at explicit ``positions`` (int32 or int64 [rows]) in one launch
+    (see b2f_rotary); ``plan`` is a :class:`b200fp8.rotary.RotaryPlan`.
+
+    q, k: f32, bf16, f16 or e4m3 (value = stored * in_scale) 2-D views, head h at column
+    h * head_stride (None: head_dim); k may be None.  f32 [head_dim] weights select the RMSNorm
+    (w + weight_offset) of every head before it is turned.  ``inverse`` turns back (the
+    transposed map).  Outputs, [rows, heads * head_dim], have the inputs' type unless
+    ``out_dtype`` says otherwise (e4m3: stored = value / out_scale); ``q_out`` / ``k_out`` may be
+    the inputs themselves.  Returns (q_out, k_out)."""
+    _check_cuda(q, k, positions, q_weight, k_weight, q_out, k_out, plan.freqs)
+    d = plan.head_dim
+    rows = q.shape[0]
+    if (k is None) != (kv_heads == 0):
+        raise ValueError("k and kv_heads go together")
+    if k is not None and (k.dtype != q.dtype or k.shape[0] != rows):
+        raise ValueError("q and k must have one type and number of rows")
+    if (positions.dtype not in (torch.int32, torch.int64) or positions.dim() != 1
+            or positions.shape[0] != rows or not positions.is_contiguous()):
+        raise TypeError("positions must be contiguous int32 or int64 [rows]")
+    for w in (q_weight, k_weight):
+        if w is not None and (w.dtype != torch.float32 or not w.is_contiguous() or w.numel() != d):
+            raise TypeError("weights must be contiguous float32 [head_dim]")
+    if k is not None and (q_weight is None) != (k_weight is None):
+        raise ValueError("q_weight and k_weight go together")
+    dtype = out_dtype if out_dtype is not None else (
+        q_out.dtype if q_out is not None else k_out.dtype if k_out is not None else q.dtype)
+    if q_out is None:
+        q_out = torch.empty((rows, heads * d), dtype=dtype, device=q.device)
+    if k is not None and k_out is None:
+        k_out = torch.empty((rows, kv_heads * d), dtype=dtype, device=q.device)
+    a = _lib.RotaryArgs()
+    _lib.lib().b2f_rotary_args_init(ctypes.byref(a))
+    a.rows, a.q_heads, a.k_heads = rows, heads, kv_heads
+    a.head_dim, a.rotary_dim = d, plan.rotary_dim
+    a.interleaved, a.inverse = int(plan.interleaved), int(inverse)
+    a.q_head_stride = d if q_head_stride is None else q_head_stride
+    a.k_head_stride = d if k_head_stride is None else k_head_stride
+    for x, y, n, hs, nm in ((q, q_out, heads, a.q_head_stride, "q"),
+                            (k, k_out, kv_heads, a.k_head_stride, "k")):
+        if x is None:
+            continue
+        if x.dim() != 2 or x.stride(1) != 1 or x.dtype not in _DT:
+            raise ValueError(f"{nm} must be a row-major 2-D tensor of f32, bf16, f16 or e4m3")
+        if n <= 0 or x.shape[1] < (n - 1) * hs + d:
+            raise ValueError(f"{nm} has too few columns for {n} heads")
+        if (y.dim() != 2 or y.stride(1) != 1 or y.dtype != dtype or y.dtype not in _DT
+                or y.shape != (rows, n * d)):
+            raise ValueError(f"{nm}_out must be a row-major [{rows}, {n * d}] tensor of {dtype}")
+        if x.device != positions.device or y.device != positions.device:
+            raise ValueError("all tensors must be on one device")
+    if plan.freqs.device != positions.device:
+        raise ValueError(f"the plan is on {plan.freqs.device}, the tensors are on "
+                         f"{positions.device}")
+    if rows == 0:
+        return q_out, k_out
+    a.q, a.q_ld, a.q_out, a.q_out_ld = q.data_ptr(), q.stride(0), q_out.data_ptr(), q_out.stride(0)
+    if k is not None:
+        a.k, a.k_ld, a.k_out, a.k_out_ld = (k.data_ptr(), k.stride(0), k_out.data_ptr(),
+                                            k_out.stride(0))
+    a.in_dtype, a.in_scale, a.out_dtype, a.out_scale = _DT[q.dtype], in_scale, _DT[dtype], out_scale
+    a.q_weight, a.k_weight = _ptr(q_weight), _ptr(k_weight)
+    a.weight_offset, a.eps = weight_offset, eps
+    a.positions, a.position_bits = positions.data_ptr(), 8 * positions.element_size()
+    a.freqs, a.magnitude = plan.freqs.data_ptr(), plan.magnitude
+    with torch.cuda.device(q.device):
+        check(_lib.lib().b2f_rotary(ctypes.byref(a), _stream()))
+    return q_out, k_out
+
+
 def quantize_fp8(x: torch.Tensor, *, scale: Optional[float] = None,
                  out: Optional[torch.Tensor] = None, amax: Optional[torch.Tensor] = None,
                  scale_out: Optional[torch.Tensor] = None,

@@ -151,6 +151,15 @@ const b2f_op g_ops[] = {
     {"qwen_block", B2F_ABI_VERSION, (void*)&b2f_qwen_block, "b2f_qwen_block_args"},
     {"quantize_fp8", B2F_ABI_VERSION, (void*)&b2f_quantize_fp8, "b2f_quant_args"},
     {"layer_norm_rows", B2F_ABI_VERSION, (void*)&b2f_layer_norm_rows, "b2f_lnrows_args"},
+    {"rotary", B2F_ABI_VERSION, (void*)&b2f_rotary, "b2f_rotary_args"},
+    {"kv4_write", B2F_ABI_VERSION, (void*)&b2f_kv4_write, "b2f_kv4_write_args"},
+    {"kv4_read", B2F_ABI_VERSION, (void*)&b2f_kv4_read, "b2f_kv4_read_args"},
+    {"kv4_attention", B2F_ABI_VERSION, (void*)&b2f_kv4_attention, "b2f_kv4_attn_args"},
+    {"kv4_extend", B2F_ABI_VERSION, (void*)&b2f_kv4_extend, "(b2f_kv4_pool, rows, counts, n)"},
+    {"kv4_fork", B2F_ABI_VERSION, (void*)&b2f_kv4_fork, "(b2f_kv4_pool, src, dst, n, workspace, workspace_bytes)"},
+    {"kv4_free", B2F_ABI_VERSION, (void*)&b2f_kv4_free, "(b2f_kv4_pool, rows, n)"},
+    {"kv4_compact", B2F_ABI_VERSION, (void*)&b2f_kv4_compact, "(b2f_kv4_pool, workspace, workspace_bytes)"},
+    {"kv4_copy_pages", B2F_ABI_VERSION, (void*)&b2f_kv4_copy_pages, "(b2f_kv4_pool, src, dst, n)"},
 };
 }
 

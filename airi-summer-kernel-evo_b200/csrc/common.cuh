@@ -30,6 +30,7 @@ enum DevCode : unsigned int {
   kDevTimeoutEpilogue = 3,
   kDevTimeoutDrain = 4,
   kDevBadArgs = 5,
+  kDevNoPages = 6,
 };
 
 // Element types of tensors passed through the C ABI (B2F_DTYPE_*).

@@ -1,0 +1,52 @@
+// Loads and stores of four neighbouring elements of any element type of the C ABI, as f32.
+// Plain (coherent) accesses: operators that may run in place use them.
+#pragma once
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+namespace b2f {
+
+template <int DT>
+__device__ __forceinline__ void load4(const char* base, long long off, float* x) {
+  if (DT == kF32) {
+    const float4 v = *reinterpret_cast<const float4*>(base + off * 4);
+    x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+  } else if (DT == kE4M3) {
+    const uint32_t v = *reinterpret_cast<const uint32_t*>(base + off);
+    const float2 a = e4m3x2_to_f32x2(uint16_t(v)), b = e4m3x2_to_f32x2(uint16_t(v >> 16));
+    x[0] = a.x; x[1] = a.y; x[2] = b.x; x[3] = b.y;
+  } else {
+    const uint2 v = *reinterpret_cast<const uint2*>(base + off * 2);
+    const float2 a = DT == kBF16 ? unpack_bf16x2(v.x) : unpack_f16x2(v.x);
+    const float2 b = DT == kBF16 ? unpack_bf16x2(v.y) : unpack_f16x2(v.y);
+    x[0] = a.x; x[1] = a.y; x[2] = b.x; x[3] = b.y;
+  }
+}
+
+// Round-to-nearest-even; e4m3 saturates.
+template <int DT>
+__device__ __forceinline__ void store4(char* base, long long off, const float* x) {
+  if (DT == kF32) {
+    *reinterpret_cast<float4*>(base + off * 4) = make_float4(x[0], x[1], x[2], x[3]);
+  } else if (DT == kE4M3) {
+    *reinterpret_cast<uint32_t*>(base + off) =
+        uint32_t(f32x2_to_e4m3x2(x[0], x[1])) | (uint32_t(f32x2_to_e4m3x2(x[2], x[3])) << 16);
+  } else {
+    uint2 v;
+    v.x = DT == kBF16 ? pack_bf16x2(x[0], x[1]) : pack_f16x2(x[0], x[1]);
+    v.y = DT == kBF16 ? pack_bf16x2(x[2], x[3]) : pack_f16x2(x[2], x[3]);
+    *reinterpret_cast<uint2*>(base + off * 2) = v;
+  }
+}
+
+// Eight e2m1 codes (a byte holds two, the first in its low nibble) as four f16 pairs: exact.
+__device__ __forceinline__ void e2m1x8_to_f16x2(uint32_t w, uint32_t (&f)[4]) {
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\tmov.b32 {b0, b1, b2, b3}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, b0;\n\tcvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, b2;\n\tcvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
+      : "=r"(f[0]), "=r"(f[1]), "=r"(f[2]), "=r"(f[3])
+      : "r"(w));
+}
+
+}  // namespace b2f

@@ -1,0 +1,897 @@
+// Attention of new tokens over the 4-bit paged cache (C ABI: b2f_kv4_attention; the layout of
+// the cache stands in kv4.cuh).
+//
+//   out[t, h] = sum_j softmax_j(q_h . k_j * sm_scale) v_j [* sigmoid(gate)] / ctx_scale
+// over the keys j <= position of t (causal) or all cached keys of its sequence.
+//
+// Bound: a step of one token per sequence reads 9/8 D bytes per key and kv head and does
+// 4 D * (heads / kv_heads) operations on them: HBM, if the codes become matrix operands cheaply
+// enough.  At the copy rate an SM receives one key (D = 128, 144 B) in 6.2 clocks; in
+// these it converts 256 codes (3.5 clocks: cvt.rn.f16x2.e2m1x2, measured 3.5 clocks a
+// warp instruction on a scheduler), scales them (2 clocks) and feeds 2 clocks of matrix
+// instructions, on three different pipes.
+//
+// How the work is laid out
+//  - Keys on the rows of the matrix instruction (m16n8k16, f16 in, f32 out): S^T = K Q^T and
+//    O^T = V^T P^T, up to 8 query rows (query heads of the kv head x new tokens) a column
+//    tile, so that the 16-row operand that has to be made from codes is never padding.
+//  - The sums over d and over keys may run in any order, which lets every thread use codes
+//    where they lie: thread (r, c) = (lane / 4, lane % 4) reads 16 consecutive bytes of the K
+//    row of its key, whose byte pairs are the k slots (2c, 2c+1), (2c+8, 2c+9) of eight
+//    steps; q is read in the same order.  For V it reads the D / 8 elements r D / 8 .. of the
+//    keys c, c + 4, c + 8, c + 12 of 16, merges the codes of two keys nibble by nibble, and
+//    has the pairs along the keys that the instruction wants.  Slot s of 16 is key
+//    (s & 7) / 2 + (s & 1) * 4 + (s & 8): the K rows are taken in that order.
+//  - e2m1 x e4m3 is exact in f16.  A query row is brought to [2^14, 2^15) by a power of two:
+//    bf16 and f16 queries lose nothing that is above 2^-39 of the row's largest.  P is held
+//    in f16, at most 2^15 and scaled so that the row's largest is at least 2^7: a rounding of
+//    2^-11, and of 2^-31 of the largest for the smallest.  Sums, maxima and O are f32.
+//  - Each warp walks over 32 keys at a time with a maximum, a sum and an O of its own (the
+//    maximum moves only when a score passes it by 2^8, so most steps need no exchange), and
+//    has its own ring of pages in shared memory, filled by bulk copies that it starts itself.
+//    No two warps wait for each other until a piece of work ends.
+//  - The keys of all (sequence, kv head, row tile) items are cut into units of 128 keys, and
+//    every CTA takes an equal run of consecutive units, whatever the lengths: at most its
+//    first and its last item are shared with other CTAs.  Their partial (O, max, sum) go to a
+//    workspace and a second kernel joins them in order of the keys: same bits in every run.
+#include <algorithm>
+#include <cmath>
+#include <string>
+
+#include "common.cuh"
+#include "host_common.h"
+#include "convert.cuh"
+#include "kv4.cuh"
+
+namespace b2f {
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kThreads = 32 * kWarps;
+constexpr int kChunk = 32;                // keys of a warp's step
+constexpr int kUnit = kChunk * kWarps;    // keys of a unit of work
+constexpr float kLift = 7.0f;             // P is scaled by 2^7 ...
+constexpr float kSlack = 8.0f;            // ... and the maximum may lag behind by 2^8
+
+struct Kv4AttnParams {
+  Kv4Cache c;
+  Kv4Batch b;
+  int heads, group, causal;
+  const char* q;
+  int q_dtype;
+  long long q_ld;
+  float scale_log2;  // sm_scale * q_scale * k_scale * log2(e)
+  float out_mul;     // v_scale
+  const char* gate;
+  int gate_dtype;
+  long long gate_ld, gate_hstride;
+  float gate_scale;
+  char* out;
+  int out_dtype;
+  long long out_ld;
+  float ctx_scale;
+  float* lse;
+  float* partial;  // [2 * CTAs][R][D] O, then [2 * CTAs][R][2] (max, sum)
+  int ctas;
+};
+
+// One (sequence, kv head, row tile): its keys and rows.
+struct Item {
+  Kv4Seq s;
+  int b, h, rt, rts;  // row tiles of the sequence
+  int keys;           // keys that some row of the tile may see
+  int units;
+};
+
+template <int R>
+__device__ __forceinline__ int tile_keys(const Kv4Seq& s, int rt, int group, int causal) {
+  if (!causal) return s.len;
+  const int last = (min((rt + 1) * R, s.n * group) - 1) / group;  // last token of the tile
+  return max(s.len - s.n + last + 1, 0);
+}
+
+__device__ __forceinline__ int units_of(int keys) { return (keys + kUnit - 1) / kUnit; }
+
+// Units of one kv head of a sequence.
+template <int R>
+__device__ __forceinline__ long long seq_units(const Kv4Seq& s, int group, int causal) {
+  const int rts = (s.n * group + R - 1) / R;
+  if (!causal || rts <= 1) return rts == 0 ? 0 : (long long)rts * units_of(tile_keys<R>(s, 0, group, causal));
+  long long u = 0;
+  for (int rt = 0; rt < rts; ++rt) u += units_of(tile_keys<R>(s, rt, group, causal));
+  return u;
+}
+
+struct Scan {
+  long long warp_sum[kWarps];
+  long long at;  // units before the sequence that was looked for
+  int b;
+};
+
+// Units of all sequences; with find >= 0 also the sequence of unit `find` (in sc.b, sc.at).
+template <int R>
+__device__ long long scan_units(const Kv4AttnParams& p, long long find, Scan& sc) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  long long before = 0;
+  for (int base = 0; base < p.b.seqs; base += kThreads) {
+    const int b = base + (int)threadIdx.x;
+    long long mine = 0;
+    if (b < p.b.seqs)
+      mine = seq_units<R>(kv4_seq(p.c, p.b, b), p.group, p.causal) * p.c.kv_heads;
+    long long x = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    __syncthreads();
+    if (lane == 31) sc.warp_sum[warp] = x;
+    __syncthreads();
+    long long lead = before;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) lead += sc.warp_sum[w];
+      before += sc.warp_sum[w];
+    }
+    const long long start = lead + x - mine;
+    if (find >= start && find < start + mine) {
+      sc.b = b;
+      sc.at = start;
+    }
+  }
+  __syncthreads();
+  return before;
+}
+
+template <int R>
+__device__ __forceinline__ void open_item(const Kv4AttnParams& p, Item& it) {
+  it.keys = tile_keys<R>(it.s, it.rt, p.group, p.causal);
+  it.units = units_of(it.keys);
+}
+
+// The item of unit `unit` of sequence b, and the unit's place in it.
+template <int R>
+__device__ int find_item(const Kv4AttnParams& p, int b, long long unit, Item& it) {
+  it.b = b;
+  it.s = kv4_seq(p.c, p.b, b);
+  it.rts = (it.s.n * p.group + R - 1) / R;
+  const long long per = seq_units<R>(it.s, p.group, p.causal);
+  it.h = (int)(unit / per);
+  long long rest = unit - it.h * per;
+  for (it.rt = 0;; ++it.rt) {
+    open_item<R>(p, it);
+    if (rest < it.units || it.rt + 1 >= it.rts) break;
+    rest -= it.units;
+  }
+  return (int)rest;
+}
+
+// The next item that has units.  There is one: the caller still has units to do.
+template <int R>
+__device__ void next_item(const Kv4AttnParams& p, Item& it) {
+  do {
+    if (++it.rt >= it.rts) {
+      it.rt = 0;
+      if (++it.h >= p.c.kv_heads) {
+        it.h = 0;
+        do {
+          if (++it.b >= p.b.seqs) {
+            it.units = 0;
+            it.keys = 0;
+            return;
+          }
+          it.s = kv4_seq(p.c, p.b, it.b);
+          it.rts = (it.s.n * p.group + R - 1) / R;
+        } while (it.rts == 0);
+      }
+    }
+    open_item<R>(p, it);
+  } while (it.units == 0);
+}
+
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                         uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
+  return r;
+}
+
+// Two e4m3 bytes as an f16 pair (exact).
+__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t v) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((unsigned short)v));
+  return r;
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+__device__ __forceinline__ bool e4m3_is_nan(uint32_t v) { return (v & 0x7f) == 0x7f; }
+
+__device__ __forceinline__ float load1(const char* base, int dt, long long off) {
+  switch (dt) {
+    case kF32: return reinterpret_cast<const float*>(base)[off];
+    case kBF16: return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(base)[off]);
+    case kF16: return __half2float(reinterpret_cast<const __half*>(base)[off]);
+    default: return e4m3_to_f32(reinterpret_cast<const uint8_t*>(base)[off]);
+  }
+}
+
+__device__ __forceinline__ void store1(char* base, int dt, long long off, float x) {
+  switch (dt) {
+    case kF32: reinterpret_cast<float*>(base)[off] = x; break;
+    case kBF16: reinterpret_cast<__nv_bfloat16*>(base)[off] = __float2bfloat16_rn(x); break;
+    case kF16: reinterpret_cast<__half*>(base)[off] = __float2half_rn(x); break;
+    default: reinterpret_cast<uint8_t*>(base)[off] = uint8_t(f32x2_to_e4m3x2(x, 0.f)); break;
+  }
+}
+
+// Where row r of an item's tile goes: token t and query head, or t = -1.
+__device__ __forceinline__ int row_token(const Kv4AttnParams& p, const Item& it, int row, int& head) {
+  const int i = row / p.group;
+  head = it.h * p.group + (row - i * p.group);
+  return i < it.s.n ? it.s.start + i : -1;
+}
+
+// Normalises, gates and stores `n` neighbouring elements (o, unnormalised) of one row.
+template <int N>
+__device__ __forceinline__ void finish_row(const Kv4AttnParams& p, int t, int head, int d0, const float* o,
+                                           float sum) {
+  const float inv = sum > 0.f || sum != sum ? 1.0f / sum : 0.f;
+  const long long at = (long long)t * p.out_ld + (long long)head * p.c.head_dim + d0;
+  float x[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    x[i] = o[i] * inv * p.out_mul;
+    if (p.gate != nullptr) {
+      const float g = load1(p.gate, p.gate_dtype, (long long)t * p.gate_ld + head * p.gate_hstride + d0 + i) * p.gate_scale;
+      x[i] = x[i] / (1.0f + __expf(-g));
+    }
+    if (p.out_dtype == kE4M3) x[i] = __fdiv_rn(x[i], p.ctx_scale);
+  }
+  if (N % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      switch (p.out_dtype) {
+        case kBF16: store4<kBF16>(p.out, at + i, x + i); break;
+        case kF16: store4<kF16>(p.out, at + i, x + i); break;
+        default: store4<kE4M3>(p.out, at + i, x + i); break;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) store1(p.out, p.out_dtype, at + i, x[i]);
+  }
+}
+
+// log sum exp of a row: P was 2^(score * log2 e - ref), sum over the keys.
+__device__ __forceinline__ void finish_lse(const Kv4AttnParams& p, int t, int head, float ref, float sum) {
+  if (p.lse == nullptr) return;
+  const float l2 = log2f(sum) + ref;
+  p.lse[(long long)t * p.heads + head] = sum > 0.f ? l2 * 0.69314718055994531f
+                                         : sum != sum ? sum : -INFINITY;
+}
+
+template <int D, int NT, int STAGES>
+struct Layout {
+  static constexpr int R = 8 * NT;
+  static constexpr int kCodes = kChunk * D / 2, kScales = kChunk * D / 16;
+  static constexpr int kStage = 2 * (kCodes + kScales);  // K codes, K scales, V codes, V scales
+  static constexpr int kPad = 4;                         // floats between rows of the join
+  static constexpr int kRing = kWarps * STAGES * kStage;
+  static constexpr int kJoin = kWarps * R * (D + kPad) * 4;
+  static constexpr int kBytes = kRing + kJoin;
+};
+
+template <int D, int NT, int STAGES>
+__global__ void __launch_bounds__(kThreads) kv4_attention_kernel(const Kv4AttnParams p) {
+  using L = Layout<D, NT, STAGES>;
+  constexpr int R = L::R;
+  constexpr int kSteps = D / 16;         // k16 steps of Q.K; m16 tiles of O^T
+  constexpr int kWordsK = D / 32;        // 32-bit words of K codes of a thread and key
+  constexpr int kWordsV = D / 64;        // words of V codes of a thread and key
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ Scan sc;
+  __shared__ __align__(8) uint64_t bars[kWarps][STAGES];
+  __shared__ int stage_ok[kWarps][STAGES];
+  __shared__ float join_ms[kWarps][R][2];
+
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int r = lane >> 2, c = lane & 3;
+  uint8_t* ring = smem + warp * STAGES * L::kStage;
+  float* join = reinterpret_cast<float*>(smem + L::kRing);
+
+  if (lane == 0) {
+    for (int s = 0; s < STAGES; ++s) mbar_init(&bars[warp][s], 1);
+    fence_mbarrier_init();
+  }
+  pdl_wait();
+  pdl_trigger();
+
+  // rows that see no key at all: zeros
+  for (int b = blockIdx.x; b < p.b.seqs; b += gridDim.x) {
+    Item it;
+    it.s = kv4_seq(p.c, p.b, b);
+    it.b = b;
+    it.rts = (it.s.n * p.group + R - 1) / R;
+    for (it.rt = 0; it.rt < it.rts; ++it.rt) {
+      if (tile_keys<R>(it.s, it.rt, p.group, p.causal) > 0) break;  // later tiles see more
+      for (int x = threadIdx.x; x < p.c.kv_heads * R * (D / 4); x += kThreads) {
+        it.h = x / (R * (D / 4));
+        const int y = x - it.h * (R * (D / 4));
+        int head;
+        const int t = row_token(p, it, it.rt * R + y / (D / 4), head);
+        const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+        if (t >= 0) {
+          finish_row<4>(p, t, head, (y % (D / 4)) * 4, zero, 0.f);
+          if (y % (D / 4) == 0) finish_lse(p, t, head, 0.f, 0.f);
+        }
+      }
+    }
+  }
+
+  const long long total = scan_units<R>(p, -1, sc);
+  const long long u0 = total * blockIdx.x / gridDim.x, u1 = total * (blockIdx.x + 1) / gridDim.x;
+  if (u0 >= u1) return;
+  scan_units<R>(p, u0, sc);
+  Item it;       // of the keys that are worked on
+  int u = find_item<R>(p, sc.b, u0 - sc.at, it);
+  Item ahead = it;  // of the keys that are fetched
+  int ahead_u = u;
+  long long fetched = u0;  // unit that is fetched next
+  int issued = 0;          // chunks whose copies this warp has started
+  bool alive = true;       // false once a copy did not arrive in time: no more work, no more copies
+
+  // The page of a lane's copies: lane = 4 * (page of the chunk) + part of the block.
+  const int log2p = p.c.page_log2;
+  const int pages_per_chunk = log2p == 4 ? 2 : 1;
+  const int keys_per_page = log2p == 4 ? 16 : 32;  // of the chunk
+  const bool copies = lane < 4 * pages_per_chunk;
+  const int part = lane & 3, sub = lane >> 2;
+  const uint64_t policy = policy_evict_normal();
+  auto page_of = [&](const Item& x, int key) -> int {
+    if (!copies || key + sub * 16 >= x.keys) return -2;
+    return p.c.table[(long long)x.s.row * p.c.table_ld + ((key + sub * 16) >> log2p)];
+  };
+  // skips over units in which this warp has no key, then the page of the next copy
+  auto seek = [&]() {
+    while (fetched < u1 && ahead_u * kUnit + warp * kChunk >= ahead.keys) {
+      if (++fetched < u1 && ++ahead_u == ahead.units) {
+        next_item<R>(p, ahead);
+        ahead_u = 0;
+      }
+    }
+  };
+  seek();
+  int next_page = fetched < u1 ? page_of(ahead, ahead_u * kUnit + warp * kChunk) : -2;
+  auto fetch = [&]() {
+    if (fetched >= u1 || !alive) return;
+    const int key = ahead_u * kUnit + warp * kChunk;
+    const int st = issued % STAGES;
+    const bool ok = next_page >= 0 && next_page < p.c.pages;
+    if (copies && next_page != -2 && !ok) record_error(kDevBadArgs);
+    const unsigned good = __ballot_sync(0xffffffffu, copies && ok);
+    const uint32_t bytes = part & 1 ? keys_per_page * (D / 16) : keys_per_page * (D / 2);
+    if (lane == 0) {
+      stage_ok[warp][st] = (good & 1) | ((good >> 4) & 1) << 1;
+      mbar_arrive_expect_tx(&bars[warp][st], (L::kStage / pages_per_chunk) * __popc(good & 0x11));
+    }
+    __syncwarp();
+    if (copies && ok) {
+      const uint8_t* from = p.c.storage + (long long)next_page * p.c.page_stride +
+                            (long long)ahead.h * p.c.block_bytes +
+                            (part >> 1) * (p.c.codes_bytes + p.c.scales_bytes) +
+                            (part & 1 ? p.c.codes_bytes : 0) +
+                            (key & (p.c.page_size - 1)) * (part & 1 ? D / 16 : D / 2);
+      uint8_t* to = ring + st * L::kStage + (part >> 1) * (L::kCodes + L::kScales) +
+                    (part & 1 ? L::kCodes : 0) + sub * 16 * (part & 1 ? D / 16 : D / 2);
+      bulk_load(to, from, bytes, &bars[warp][st], policy);
+    }
+    ++issued;
+    if (++fetched < u1 && ++ahead_u == ahead.units) {
+      next_item<R>(p, ahead);
+      ahead_u = 0;
+    }
+    seek();
+    next_page = fetched < u1 ? page_of(ahead, ahead_u * kUnit + warp * kChunk) : -2;
+  };
+  for (int s = 0; s < STAGES; ++s) fetch();
+
+  int done = 0;  // chunks worked on
+  long long unit = u0;
+  while (unit < u1) {
+    const int piece_begin = u;  // units [piece_begin, piece_end) of the item
+    const int piece_end = (int)min((long long)it.units, u + (u1 - unit));
+    // ---- the queries of the tile, and what a score is multiplied by
+    uint32_t qf[NT][kSteps][2];
+    float mul[NT][2];
+    int limit[NT][2];  // keys that the column sees
+    int lowest = 0x7fffffff;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      int head;
+      const int t = row_token(p, it, it.rt * R + nt * 8 + r, head);
+      float top = 0.f;
+      float x[2 * kWordsK][4];
+      const long long at = (long long)t * p.q_ld + (long long)head * D;
+#pragma unroll
+      for (int half = 0; half < (D == 256 ? 2 : 1); ++half) {
+        constexpr int kPer = D == 256 ? 8 : 2 * kWordsK;  // fours of a run
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+          float* y = x[half * kPer + i];
+          const long long e = at + half * 128 + c * (kPer * 4) + i * 4;
+          if (t < 0) {
+            y[0] = y[1] = y[2] = y[3] = 0.f;
+          } else if (p.q_dtype == kBF16) {
+            load4<kBF16>(p.q, e, y);
+          } else if (p.q_dtype == kF16) {
+            load4<kF16>(p.q, e, y);
+          } else {
+            load4<kE4M3>(p.q, e, y);
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) top = fmaxf(top, fabsf(y[j]));
+        }
+      }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      // 2^(14 - exponent of top), and its inverse; 1 for a row of zeros or with an infinity
+      const int ex = (__float_as_int(top) >> 23) & 0xff;
+      const int up = ex == 0 || ex == 255 ? 0 : min(max(127 + 14 - ex, -120), 120);
+      const float lift = __int_as_float((127 + up) << 23), drop = __int_as_float((127 - up) << 23);
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        qf[nt][s][0] = pack_f16x2(x[s][0] * lift, x[s][1] * lift);
+        qf[nt][s][1] = pack_f16x2(x[s][2] * lift, x[s][3] * lift);
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        mul[nt][j] = __shfl_sync(0xffffffffu, drop, (2 * c + j) * 4) * p.scale_log2;
+        const int row = it.rt * R + nt * 8 + 2 * c + j;
+        limit[nt][j] = p.causal ? min(it.s.len - it.s.n + row / p.group + 1, it.keys) : it.keys;
+        if (row < it.s.n * p.group) lowest = min(lowest, limit[nt][j]);
+      }
+    }
+    lowest = __reduce_min_sync(0xffffffffu, lowest);
+
+    float ref[NT][2], sum[NT][2], o[kSteps][NT][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        ref[nt][j] = -INFINITY;
+        sum[nt][j] = 0.f;
+      }
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[s][nt][j] = 0.f;
+    }
+
+    for (; u < piece_end; ++u, ++unit) {
+      const int key0 = u * kUnit + warp * kChunk;
+      if (key0 >= it.keys) continue;
+      const int st = done % STAGES;
+      if (done < issued &&
+          !__all_sync(0xffffffffu, mbar_wait(&bars[warp][st], (done / STAGES) & 1, kDevTimeoutMma, nullptr)))
+        alive = false;
+      ++done;
+      const uint8_t* kc = ring + st * L::kStage;
+      const uint8_t* ks = kc + L::kCodes;
+      const uint8_t* vc = ks + L::kScales;
+      const uint8_t* vs = vc + L::kCodes;
+      const int okay = stage_ok[warp][st];
+      const bool edge = key0 + kChunk > lowest || okay != (1 << pages_per_chunk) - 1;
+      if (alive) {
+#pragma unroll
+        for (int g = 0; g < kChunk / 16; ++g) {
+          // ---- S^T: 16 keys x R rows
+          float s[NT][4];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+          const int kr = g * 16 + (r >> 1) + (r & 1) * 4;  // key of slot r; slot r + 8: kr + 8
+          uint32_t w0[kWordsK], w1[kWordsK], sc0, sc1;     // codes, scales of both keys
+          if (D == 64) {
+            const uint2 a = *reinterpret_cast<const uint2*>(kc + kr * 32 + c * 8);
+            const uint2 b = *reinterpret_cast<const uint2*>(kc + (kr + 8) * 32 + c * 8);
+            w0[0] = a.x; w0[1] = a.y; w1[0] = b.x; w1[1] = b.y;
+            sc0 = ks[kr * 4 + c];
+            sc1 = ks[(kr + 8) * 4 + c];
+          } else {
+#pragma unroll
+            for (int half = 0; half < kWordsK / 4; ++half) {
+              const uint4 a = *reinterpret_cast<const uint4*>(kc + kr * (D / 2) + half * 64 + c * 16);
+              const uint4 b = *reinterpret_cast<const uint4*>(kc + (kr + 8) * (D / 2) + half * 64 + c * 16);
+              w0[4 * half] = a.x; w0[4 * half + 1] = a.y; w0[4 * half + 2] = a.z; w0[4 * half + 3] = a.w;
+              w1[4 * half] = b.x; w1[4 * half + 1] = b.y; w1[4 * half + 2] = b.z; w1[4 * half + 3] = b.w;
+            }
+            sc0 = *reinterpret_cast<const uint16_t*>(ks + kr * (D / 16) + 2 * c);
+            sc1 = *reinterpret_cast<const uint16_t*>(ks + (kr + 8) * (D / 16) + 2 * c);
+            if (D == 256) {
+              sc0 |= uint32_t(*reinterpret_cast<const uint16_t*>(ks + kr * 16 + 8 + 2 * c)) << 16;
+              sc1 |= uint32_t(*reinterpret_cast<const uint16_t*>(ks + (kr + 8) * 16 + 8 + 2 * c)) << 16;
+            }
+          }
+#pragma unroll
+          for (int w = 0; w < kWordsK; ++w) {  // a word is two steps; two words share a scale
+            const uint32_t one0 = (sc0 >> (8 * (w / 2))) & 0xff, one1 = (sc1 >> (8 * (w / 2))) & 0xff;
+            const uint32_t m0 = e4m3x2_to_f16x2(one0 * 0x101), m1 = e4m3x2_to_f16x2(one1 * 0x101);
+            uint32_t f0[4], f1[4];
+            e2m1x8_to_f16x2(w0[w], f0);
+            e2m1x8_to_f16x2(w1[w], f1);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              f0[i] = hmul2(f0[i], m0);
+              f1[i] = hmul2(f1[i], m1);
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              mma16816(s[nt], f0[0], f1[0], f0[1], f1[1], qf[nt][2 * w][0], qf[nt][2 * w][1]);
+              mma16816(s[nt], f0[2], f1[2], f0[3], f1[3], qf[nt][2 * w + 1][0], qf[nt][2 * w + 1][1]);
+            }
+          }
+          // ---- scores to P
+          bool seen[NT][4];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              s[nt][j] *= mul[nt][j & 1];
+              seen[nt][j] = true;
+              if (edge) {
+                const int key = kr + (j >> 1) * 8;
+                seen[nt][j] = key0 + key < limit[nt][j & 1] &&
+                              (okay >> (pages_per_chunk == 2 ? g : 0) & 1);
+                if (!seen[nt][j]) s[nt][j] = -INFINITY;
+              }
+            }
+          bool jump = false;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) jump |= fmaxf(s[nt][j], s[nt][j + 2]) > ref[nt][j] + kSlack;
+          if (__any_sync(0xffffffffu, jump)) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                float m = fmaxf(s[nt][j], s[nt][j + 2]);
+                m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+                m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+                m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+                m = fmaxf(m, ref[nt][j]);
+                const float f = m == ref[nt][j] ? 1.f : ex2(ref[nt][j] - m);
+                ref[nt][j] = m;
+                sum[nt][j] *= f;
+#pragma unroll
+                for (int t = 0; t < kSteps; ++t) {
+                  o[t][nt][j] *= f;
+                  o[t][nt][j + 2] *= f;
+                }
+              }
+          }
+          uint32_t pf[NT][2];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float base = ref[nt][j & 1] == -INFINITY ? 0.f : ref[nt][j & 1] - kLift;
+              s[nt][j] = ex2(s[nt][j] - base);
+              sum[nt][j & 1] += s[nt][j];
+            }
+          }
+          // ---- V: codes of keys c, c + 4, c + 8, c + 12 of the 16
+          const uint8_t* vk = vc + (g * 16 + c) * (D / 2) + r * (D / 16);
+          uint32_t v[4][kWordsV == 0 ? 1 : kWordsV], vm[4];
+          const uint8_t* vsk = vs + (g * 16 + c) * (D / 16) + (r * (D / 8)) / 16;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (D == 64) {
+              v[i][0] = *reinterpret_cast<const uint32_t*>(vk + i * 4 * (D / 2));
+              vm[i] = vsk[i * 4 * (D / 16)];
+            } else if (D == 128) {
+              const uint2 a = *reinterpret_cast<const uint2*>(vk + i * 4 * (D / 2));
+              v[i][0] = a.x;
+              v[i][kWordsV - 1] = a.y;
+              vm[i] = vsk[i * 4 * (D / 16)];
+            } else {
+              const uint4 a = *reinterpret_cast<const uint4*>(vk + i * 4 * (D / 2));
+              v[i][0] = a.x;
+              v[i][kWordsV / 4] = a.y;
+              v[i][kWordsV / 2] = a.z;
+              v[i][kWordsV - 1] = a.w;
+              vm[i] = *reinterpret_cast<const uint16_t*>(vsk + i * 4 * (D / 16));
+            }
+          }
+          if (edge) {
+            // What a row may not see must not reach it: 0 * NaN would.  NaN scales (of keys
+            // behind the last, or of tokens that only later rows see) count as 0 here, and a row
+            // that does see a NaN gets it through P.
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const int key = kr + j * 8;
+              bool nan = false;
+#pragma unroll
+              for (int i = 0; i < D / 16; ++i) nan |= e4m3_is_nan(vs[key * (D / 16) + i]);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                if (nan && seen[nt][2 * j]) s[nt][2 * j] = NAN;
+                if (nan && seen[nt][2 * j + 1]) s[nt][2 * j + 1] = NAN;
+              }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              if (e4m3_is_nan(vm[i])) vm[i] &= 0xff00;
+              if (D == 256 && e4m3_is_nan(vm[i] >> 8)) vm[i] &= 0xff;
+            }
+          }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            pf[nt][0] = transpose8x8(pack_f16x2(s[nt][0], s[nt][1]));
+            pf[nt][1] = transpose8x8(pack_f16x2(s[nt][2], s[nt][3]));
+          }
+#pragma unroll
+          for (int w = 0; w < kWordsV; ++w) {  // a word: four tiles
+            const int sh = D == 256 ? 8 * (w / 2) : 0;
+            const uint32_t m01 = e4m3x2_to_f16x2(((vm[0] >> sh) & 0xff) | ((vm[1] >> sh) & 0xff) << 8);
+            const uint32_t m23 = e4m3x2_to_f16x2(((vm[2] >> sh) & 0xff) | ((vm[3] >> sh) & 0xff) << 8);
+            uint32_t lo01[4], hi01[4], lo23[4], hi23[4];
+            e2m1x8_to_f16x2((v[0][w] & 0x0f0f0f0fu) | ((v[1][w] << 4) & 0xf0f0f0f0u), lo01);
+            e2m1x8_to_f16x2(((v[0][w] >> 4) & 0x0f0f0f0fu) | (v[1][w] & 0xf0f0f0f0u), hi01);
+            e2m1x8_to_f16x2((v[2][w] & 0x0f0f0f0fu) | ((v[3][w] << 4) & 0xf0f0f0f0u), lo23);
+            e2m1x8_to_f16x2(((v[2][w] >> 4) & 0x0f0f0f0fu) | (v[3][w] & 0xf0f0f0f0u), hi23);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t a0 = hmul2(lo01[i], m01), a1 = hmul2(hi01[i], m01);
+              const uint32_t a2 = hmul2(lo23[i], m23), a3 = hmul2(hi23[i], m23);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) mma16816(o[4 * w + i][nt], a0, a1, a2, a3, pf[nt][0], pf[nt][1]);
+            }
+          }
+        }
+      }
+      __syncwarp();  // the stage has been read by all lanes
+      fetch();
+    }
+
+    // ---- the piece is done: join the warps
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float l = sum[nt][j];
+        l += __shfl_xor_sync(0xffffffffu, l, 4);
+        l += __shfl_xor_sync(0xffffffffu, l, 8);
+        l += __shfl_xor_sync(0xffffffffu, l, 16);
+        const int row = nt * 8 + 2 * c + j;
+        if (r == 0) {
+          join_ms[warp][row][0] = ref[nt][j] == -INFINITY ? -INFINITY : ref[nt][j] - kLift;
+          join_ms[warp][row][1] = l;
+        }
+        float* to = join + (warp * R + row) * (D + L::kPad) + r * (D / 8);
+#pragma unroll
+        for (int t = 0; t < kSteps; t += 2)
+          *reinterpret_cast<float4*>(to + 2 * t) =
+              make_float4(o[t][nt][j], o[t][nt][j + 2], o[t + 1][nt][j], o[t + 1][nt][j + 2]);
+      }
+    __syncthreads();
+    const bool from_start = piece_begin == 0;
+    const bool to_end = piece_end == it.units;
+    const int slot = 2 * blockIdx.x + (from_start ? 1 : 0);
+    float* part_o = p.partial + (long long)slot * R * D;
+    float* part_ms = p.partial + 2ll * p.ctas * R * D + (long long)slot * R * 2;
+    for (int x = threadIdx.x; x < R * (D / 4); x += kThreads) {
+      const int row = x / (D / 4), d0 = (x % (D / 4)) * 4;
+      float m = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) m = fmaxf(m, join_ms[w][row][0]);
+      float l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float mw = join_ms[w][row][0];
+        const float f = mw == -INFINITY ? (join_ms[w][row][1] != join_ms[w][row][1] ? 1.f : 0.f) : ex2(mw - m);
+        const float4 y = *reinterpret_cast<const float4*>(join + (w * R + row) * (D + L::kPad) + d0);
+        l += join_ms[w][row][1] * f;
+        acc[0] += y.x * f; acc[1] += y.y * f; acc[2] += y.z * f; acc[3] += y.w * f;
+      }
+      if (from_start && to_end) {
+        int head;
+        const int t = row_token(p, it, it.rt * R + row, head);
+        if (t >= 0) {
+          finish_row<4>(p, t, head, d0, acc, l);
+          if (d0 == 0) finish_lse(p, t, head, m, l);
+        }
+      } else {
+        *reinterpret_cast<float4*>(part_o + row * D + d0) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+        if (d0 == 0) {
+          part_ms[2 * row] = m;
+          part_ms[2 * row + 1] = l;
+        }
+      }
+    }
+    __syncthreads();
+    if (unit < u1) {
+      next_item<R>(p, it);
+      u = 0;
+    }
+  }
+}
+
+// Joins the pieces of the item that begins among the units of CTA blockIdx.x and goes on in
+// the next ones.  One row of the item a CTA; each warp takes every fourth piece.
+template <int D, int NT>
+__global__ void __launch_bounds__(kThreads) kv4_attention_join_kernel(const Kv4AttnParams p) {
+  constexpr int R = 8 * NT;
+  constexpr int kPer = D / 32;  // elements of a lane
+  __shared__ Scan sc;
+  __shared__ float acc_s[kWarps][D], ms[kWarps][2];
+  pdl_wait();
+  pdl_trigger();
+  const long long total = scan_units<R>(p, -1, sc);
+  const int n = p.ctas, me = blockIdx.x, row = blockIdx.y;
+  const long long u0 = total * me / n, u1 = total * (me + 1) / n;
+  if (u0 >= u1 || u1 >= total) return;
+  scan_units<R>(p, u1 - 1, sc);
+  Item it;
+  const int at = find_item<R>(p, sc.b, u1 - 1 - sc.at, it);
+  const long long begin = u1 - 1 - at, end = begin + it.units;
+  if (begin < u0 || end <= u1) return;
+  int head;
+  const int t = row_token(p, it, it.rt * R + row, head);
+  if (t < 0) return;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const float* all_ms = p.partial + 2ll * n * R * D;
+
+  float m = -INFINITY, l = 0.f, acc[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) acc[i] = 0.f;
+  for (int x = me + warp; x < n && total * x / n < end; x += kWarps) {
+    if (total * x / n == total * (x + 1) / n) continue;  // a CTA without units
+    const long long slot = 2ll * x + (x == me ? 1 : 0);
+    const float mx = all_ms[(slot * R + row) * 2], lx = all_ms[(slot * R + row) * 2 + 1];
+    const float* o = p.partial + (slot * R + row) * D + lane * kPer;
+    const float top = fmaxf(m, mx);
+    const float f = m == top ? 1.f : ex2(m - top), g = mx == top ? 1.f : ex2(mx - top);
+    m = top;
+    l = l * f + lx * g;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) acc[i] = acc[i] * f + o[i] * g;
+  }
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) acc_s[warp][lane * kPer + i] = acc[i];
+  if (lane == 0) {
+    ms[warp][0] = m;
+    ms[warp][1] = l;
+  }
+  __syncthreads();
+  float top = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) top = fmaxf(top, ms[w][0]);
+  float f[kWarps];
+  l = 0.f;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    f[w] = ms[w][0] == top ? 1.f : ex2(ms[w][0] - top);
+    l += ms[w][1] * f[w];
+  }
+  for (int d = threadIdx.x; d < D; d += kThreads) {
+    float x[1] = {0.f};
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) x[0] += acc_s[w][d] * f[w];
+    finish_row<1>(p, t, head, d, x, l);
+  }
+  if (threadIdx.x == 0) finish_lse(p, t, head, top, l);
+}
+
+constexpr int kMaxPerSm = 3;
+
+int tile_rows(int head_dim, long long rows) { return head_dim == 256 || rows <= 8 ? 8 : 16; }
+
+template <int D, int NT, int STAGES>
+int launch_attention(Kv4AttnParams& p, cudaStream_t s) {
+  using L = Layout<D, NT, STAGES>;
+  const int per_sm = std::min(kMaxPerSm, std::max(1, 225 * 1024 / (L::kBytes + 4096)));
+  p.ctas = sm_count() * per_sm;
+  B2F_CUDA_TRY(cudaFuncSetAttribute(kv4_attention_kernel<D, NT, STAGES>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    L::kBytes));
+  B2F_CUDA_TRY(launch_pdl(kv4_attention_kernel<D, NT, STAGES>, dim3((unsigned)p.ctas), dim3(kThreads), L::kBytes, s, p));
+  B2F_CUDA_TRY(launch_pdl(kv4_attention_join_kernel<D, NT>, dim3((unsigned)p.ctas, 8 * NT), dim3(kThreads), 0, s, p));
+  return B2F_OK;
+}
+
+}  // namespace
+}  // namespace b2f
+
+extern "C" {
+
+void b2f_kv4_attn_args_init(b2f_kv4_attn_args* a) {
+  if (a == nullptr) return;
+  *a = b2f_kv4_attn_args{};
+  a->causal = 1;
+  a->q_dtype = a->out_dtype = B2F_DTYPE_BF16;
+  a->gate_dtype = B2F_DTYPE_E4M3;
+  a->q_scale = a->gate_scale = a->ctx_scale = 1.0f;
+  a->cache.k_scale = a->cache.v_scale = 1.0f;
+}
+
+long long b2f_kv4_attention_workspace_bytes(int head_dim) {
+  const int sms = b2f::sm_count();
+  if (sms <= 0) return -1;
+  const int rows = head_dim == 256 ? 8 : 16;
+  return 2ll * sms * b2f::kMaxPerSm * rows * (head_dim + 2) * 4;
+}
+
+int b2f_kv4_attention(const b2f_kv4_attn_args* a, b2f_stream_t stream) {
+  using namespace b2f;
+  if (a == nullptr) return fail(B2F_ERR_ARG, "kv4_attention: null args");
+  Kv4AttnParams p = {};
+  const char* e = kv4_check_cache(a->cache, &p.c);
+  if (e == nullptr) e = kv4_check_batch(a->cache, a->batch, &p.b);
+  if (e != nullptr) return fail(B2F_ERR_ARG, std::string("kv4_attention: ") + e);
+  const int d = a->cache.head_dim, hk = a->cache.kv_heads;
+  if (a->heads <= 0 || a->heads % hk) return fail(B2F_ERR_ARG, "kv4_attention: heads must be a multiple of kv_heads");
+  if (a->heads / hk > 1024) return fail(B2F_ERR_ARG, "kv4_attention: more than 1024 query heads a kv head");
+  if ((long long)a->batch.tokens * a->heads > 0x3fffffffll) return fail(B2F_ERR_ARG, "kv4_attention: too many rows");
+  if (a->q == nullptr || a->out == nullptr) return fail(B2F_ERR_ARG, "kv4_attention: null tensor");
+  for (int dt : {a->q_dtype, a->out_dtype})
+    if (dt != B2F_DTYPE_BF16 && dt != B2F_DTYPE_F16 && dt != B2F_DTYPE_E4M3)
+      return fail(B2F_ERR_ARG, "kv4_attention: q and out must be bf16, f16 or e4m3");
+  const int qs = a->q_dtype == B2F_DTYPE_E4M3 ? 1 : 2, os = a->out_dtype == B2F_DTYPE_E4M3 ? 1 : 2;
+  const long long cols = (long long)a->heads * d;
+  if (a->q_ld < cols || a->out_ld < cols || (a->q_ld * qs) % 16 || (a->out_ld * os) % 16 ||
+      ((reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->out)) & 15))
+    return fail(B2F_ERR_ARG, "kv4_attention: q and out need 16-byte aligned rows of heads * head_dim elements");
+  if (a->gate != nullptr) {
+    if (a->gate_dtype != B2F_DTYPE_E4M3 && a->gate_dtype != B2F_DTYPE_BF16)
+      return fail(B2F_ERR_ARG, "kv4_attention: gate must be e4m3 or bf16");
+    if (a->gate_head_stride < d || a->gate_ld < (long long)(a->heads - 1) * a->gate_head_stride + d)
+      return fail(B2F_ERR_ARG, "kv4_attention: gate row pitch or head stride too small");
+    if (a->gate_dtype == B2F_DTYPE_BF16 && (reinterpret_cast<uintptr_t>(a->gate) & 1))
+      return fail(B2F_ERR_ARG, "kv4_attention: misaligned gate");
+  }
+  if (!(a->ctx_scale > 0.f) || !std::isfinite(a->ctx_scale)) return fail(B2F_ERR_ARG, "kv4_attention: ctx_scale must be > 0");
+  if (a->out_dtype != B2F_DTYPE_E4M3 && a->ctx_scale != 1.0f)
+    return fail(B2F_ERR_ARG, "kv4_attention: ctx_scale belongs to an e4m3 output");
+  if (reinterpret_cast<uintptr_t>(a->lse) & 3) return fail(B2F_ERR_ARG, "kv4_attention: misaligned lse");
+  const long long need = b2f_kv4_attention_workspace_bytes(d);
+  if (need < 0) return fail(B2F_ERR_CUDA, "kv4_attention: no device");
+  if (a->workspace == nullptr || a->workspace_bytes < need || (reinterpret_cast<uintptr_t>(a->workspace) & 15))
+    return fail(B2F_ERR_ARG, "kv4_attention: workspace too small or misaligned");
+  p.heads = a->heads; p.group = a->heads / hk; p.causal = a->causal != 0;
+  p.q = reinterpret_cast<const char*>(a->q); p.q_dtype = a->q_dtype; p.q_ld = a->q_ld;
+  const float sm = a->sm_scale > 0.f ? a->sm_scale : 1.0f / std::sqrt((float)d);
+  p.scale_log2 = sm * a->q_scale * a->cache.k_scale * 1.4426950408889634f;
+  p.out_mul = a->cache.v_scale;
+  p.gate = reinterpret_cast<const char*>(a->gate); p.gate_dtype = a->gate_dtype;
+  p.gate_ld = a->gate_ld; p.gate_hstride = a->gate_head_stride; p.gate_scale = a->gate_scale;
+  p.out = reinterpret_cast<char*>(a->out); p.out_dtype = a->out_dtype; p.out_ld = a->out_ld;
+  p.ctx_scale = a->ctx_scale; p.lse = a->lse;
+  p.partial = reinterpret_cast<float*>(a->workspace);
+  cudaStream_t s = (cudaStream_t)stream;
+  // 16 rows a tile read every key half as often as 8 do, once there are more than 8.
+  const long long most = a->batch.starts != nullptr ? a->batch.tokens : a->batch.tokens / a->batch.seqs;
+  const int rows = tile_rows(d, most * p.group);
+  if (d == 64) return rows == 8 ? launch_attention<64, 1, 4>(p, s) : launch_attention<64, 2, 4>(p, s);
+  if (d == 128) return rows == 8 ? launch_attention<128, 1, 3>(p, s) : launch_attention<128, 2, 3>(p, s);
+  return launch_attention<256, 1, 2>(p, s);
+}
+
+}  // extern "C"

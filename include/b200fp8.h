@@ -57,7 +57,8 @@ enum b2f_dev_status {
   B2F_DEV_TIMEOUT_MMA = 2,
   B2F_DEV_TIMEOUT_EPILOGUE = 3,
   B2F_DEV_TIMEOUT_DRAIN = 4,
-  B2F_DEV_BAD_ARGS = 5
+  B2F_DEV_BAD_ARGS = 5, /* a device-side list holds a row, page or position out of range */
+  B2F_DEV_NO_PAGES = 6  /* too few free pages (b2f_kv4_extend, b2f_kv4_fork) */
 };
 
 /* Library ABI version (B2F_ABI_VERSION of the build). */
@@ -444,6 +445,196 @@ int b2f_quantize_fp8(const b2f_quant_args* args, b2f_stream_t stream);
 int b2f_swiglu_fp8(const void* gate, long long gate_ld, const void* up, long long up_ld,
                    void* out, long long out_ld, int rows, int cols, float in_scale,
                    float out_scale, b2f_stream_t stream);
+
+/* ------------------------------------------------------------------ rotary positions
+ * Pair i of a head at position s turns by the angle s * w_i (optional head norm first):
+ *   x = in * in_scale;  x = x * rsqrt(mean(x^2) + eps) * (weight + weight_offset)  (weights)
+ *   (x, y) -> magnitude * (x cos - y sin, y cos + x sin);  out = x, e4m3: e4m3(x / out_scale)
+ *   pairs: (i, i + rotary_dim / 2), or with `interleaved` (2 i, 2 i + 1); elements from
+ *   rotary_dim on pass through.  `inverse` turns by -angle: the transposed map.
+ *   q, k: f32, bf16, f16 or e4m3 [rows, ld], head h at column h * head_stride (one dtype for
+ *   both); outputs of any of these types, head h at column h * head_dim; in place where type,
+ *   pitch and head places agree.  q_heads or k_heads may be 0.
+ *   positions: int32 or int64 [rows], any value.  freqs: [rotary_dim / 2] turns per position in
+ *   64-bit fixed point, round(w_i / (2 pi) * 2^64): angles of far positions stay exact.
+ * Next to b2f_head_norm_rope, which takes cos / sin tables at position row % seq and e4m3.
+ * Requirements: head_dim, rotary_dim and head strides multiples of 8, head_dim <= 256; tensors and
+ * rows aligned to four elements.
+ */
+typedef struct b2f_rotary_args {
+  int rows, q_heads, k_heads, head_dim, rotary_dim;
+  int interleaved, inverse;
+  const void* q;
+  long long q_ld, q_head_stride;
+  const void* k;
+  long long k_ld, k_head_stride;
+  int in_dtype;
+  float in_scale;
+  const float* q_weight; /* optional f32 [head_dim]; both or none */
+  const float* k_weight;
+  float weight_offset, eps;
+  const void* positions;
+  int position_bits; /* 32 or 64 */
+  const unsigned long long* freqs;
+  float magnitude;
+  void* q_out;
+  long long q_out_ld;
+  void* k_out;
+  long long k_out_ld;
+  int out_dtype;
+  float out_scale;
+} b2f_rotary_args;
+
+void b2f_rotary_args_init(b2f_rotary_args* args);
+int b2f_rotary(const b2f_rotary_args* args, b2f_stream_t stream);
+
+/* ------------------------------------------------------------------ 4-bit paged cache
+ * Keys and values at 4.5 bits an element, in pages of 16, 32 or 64 tokens.  A page of a layer
+ * holds, for each kv head, the block
+ *   [K codes: page_size x head_dim / 2 | K scales: page_size x head_dim / 16 | V codes | V scales]
+ * of page_size * head_dim * 9 / 8 bytes: e2m1 codes, two to a byte, the even element in the low
+ * nibble; one e4m3 scale for 16 consecutive elements; value = code * scale * k_scale (v_scale).
+ * Page p of a layer starts at storage + p * page_stride.  Row i of `table` lists the pages of a
+ * sequence in order, lens[i] its tokens.  head_dim 64, 128 or 256.
+ *
+ * A batch is `tokens` packed new tokens of `seqs` sequences: those of sequence b are
+ * starts[b] .. starts[b + 1] - 1 (starts: [seqs + 1], ascending; null: tokens / seqs each), and
+ * sequence b is table row rows[b] (null: row b).  Token i of its n sits at position
+ * lens[row] - n + i: the lengths already count the new tokens (b2f_kv4_extend).  Packed tokens
+ * outside of starts[0] .. starts[seqs] - 1 are left alone, in the outputs too.  The sequences of
+ * one call are distinct rows.  No list on the device can lead a kernel out of bounds: an entry
+ * out of range records B2F_DEV_BAD_ARGS and its token (in attention: its keys) is left out.
+ */
+typedef struct b2f_kv4_cache {
+  void* storage;
+  long long page_stride;
+  int pages, kv_heads, head_dim, page_size;
+  float k_scale, v_scale;
+  const int* table;
+  int table_rows, table_cols;
+  long long table_ld;
+  const int* lens;
+} b2f_kv4_cache;
+
+typedef struct b2f_kv4_batch {
+  int seqs, tokens;
+  const int* rows;
+  const int* starts;
+} b2f_kv4_batch;
+
+/* k, v (f32, bf16, f16 or e4m3 [tokens, ld], kv head h at column h * head_dim, value = stored *
+ * in_scale) into their places in the cache:
+ *   scale = e4m3(amax of 16 / (6 * k_scale)); code = e2m1(value / (scale * k_scale)), ties to
+ *   even.  A NaN makes its group NaN; infinities saturate.
+ * Next to b2f_quantize_fp8; replaces no reference interface (the reference keeps no cache). */
+typedef struct b2f_kv4_write_args {
+  b2f_kv4_cache cache;
+  b2f_kv4_batch batch;
+  const void* k;
+  long long k_ld;
+  float k_in_scale;
+  const void* v;
+  long long v_ld;
+  float v_in_scale;
+  int dtype;
+} b2f_kv4_write_args;
+
+void b2f_kv4_write_args_init(b2f_kv4_write_args* args);
+int b2f_kv4_write(const b2f_kv4_write_args* args, b2f_stream_t stream);
+
+/* The values that the cache holds for the tokens of a batch, to k, v (f32, bf16 or f16).  Zeros
+ * for a token whose row, page or position is out of range. */
+typedef struct b2f_kv4_read_args {
+  b2f_kv4_cache cache;
+  b2f_kv4_batch batch;
+  void* k;
+  long long k_ld;
+  void* v;
+  long long v_ld;
+  int dtype;
+} b2f_kv4_read_args;
+
+void b2f_kv4_read_args_init(b2f_kv4_read_args* args);
+int b2f_kv4_read(const b2f_kv4_read_args* args, b2f_stream_t stream);
+
+/* Attention of the batch's new tokens over the cache:
+ *   out[t, h] = softmax_j(q_h . k_j * sm_scale) v_j [* sigmoid(gate)], e4m3: / ctx_scale
+ *   over keys j <= position of t (causal), or all lens[row] keys; kv head h / (heads / kv_heads).
+ *   q: bf16, f16 or e4m3 [tokens, q_ld], head h at column h * head_dim, value = stored * q_scale;
+ *   gate optional, as in b2f_attention_fp8; out: bf16, f16 or e4m3.  lse: optional f32
+ *   [tokens, heads], the natural log of the sum of exp(score).  A token that sees no key gets
+ *   zeros and -infinity.  A NaN or infinity in a key or value reaches no token that may not
+ *   see it.  sm_scale <= 0 selects 1/sqrt(head_dim).
+ *   workspace: b2f_kv4_attention_workspace_bytes(head_dim) bytes, 16-byte aligned, no zeroing;
+ *   calls that may run at the same time need one each.  Bitwise reproducible.
+ * Next to b2f_attention_fp8, whose keys and values are the batch's own. */
+typedef struct b2f_kv4_attn_args {
+  b2f_kv4_cache cache;
+  b2f_kv4_batch batch;
+  int heads, causal;
+  const void* q;
+  int q_dtype;
+  long long q_ld;
+  float q_scale;
+  float sm_scale;
+  const void* gate;
+  int gate_dtype;
+  long long gate_ld, gate_head_stride;
+  float gate_scale;
+  void* out;
+  int out_dtype;
+  long long out_ld;
+  float ctx_scale;
+  float* lse;
+  void* workspace;
+  long long workspace_bytes;
+} b2f_kv4_attn_args;
+
+void b2f_kv4_attn_args_init(b2f_kv4_attn_args* args);
+long long b2f_kv4_attention_workspace_bytes(int head_dim);
+int b2f_kv4_attention(const b2f_kv4_attn_args* args, b2f_stream_t stream);
+
+/* The pages of all layers of a cache, and who uses them.  refs[p] counts the table rows that
+ * list page p; a page is free when it is 0, and the lowest free page is taken first.  Page p of
+ * layer l starts at storage + l * layer_stride + p * page_stride and has page_bytes bytes.  A
+ * call that cannot be carried out as a whole changes nothing and records B2F_DEV_BAD_ARGS (a
+ * row out of range or listed twice, a full table row, a fork onto a row in use) or
+ * B2F_DEV_NO_PAGES.  Rows of a call: at most 1024, int32 on the device. */
+typedef struct b2f_kv4_pool {
+  void* storage;
+  long long layer_stride, page_stride;
+  int layers, pages, page_size, page_bytes;
+  int* table;
+  int table_rows, table_cols;
+  long long table_ld;
+  int* lens;
+  int* refs;
+} b2f_kv4_pool;
+
+/* lens[rows[i]] += counts[i], with free pages for the new tokens (rows null: row i). */
+int b2f_kv4_extend(const b2f_kv4_pool* pool, const int* rows, const int* counts, int n,
+                   b2f_stream_t stream);
+
+/* Empty rows dst[i] become copies of rows src[i] (which may repeat): full pages are shared, a
+ * last page that is not full is copied, so that both may grow.  No row is in both lists. */
+long long b2f_kv4_fork_workspace_bytes(int n);
+int b2f_kv4_fork(const b2f_kv4_pool* pool, const int* src, const int* dst, int n,
+                 void* workspace, long long workspace_bytes, b2f_stream_t stream);
+
+/* Empties rows (null: rows 0 .. n - 1); pages that no other row uses become free.  A row that is
+ * out of range is skipped (B2F_DEV_BAD_ARGS), one that is listed twice is emptied once. */
+int b2f_kv4_free(const b2f_kv4_pool* pool, const int* rows, int n, b2f_stream_t stream);
+
+/* Moves the used pages to the front: with L of them, the i-th at or behind L goes to the i-th
+ * free page before L.  Table and counts follow. */
+long long b2f_kv4_compact_workspace_bytes(int pages);
+int b2f_kv4_compact(const b2f_kv4_pool* pool, void* workspace, long long workspace_bytes,
+                    b2f_stream_t stream);
+
+/* Copies pages src[i] to dst[i] in all layers (HOST arrays, read before the call returns; no
+ * page written twice, or both read and written).  Table and counts stay as they are. */
+int b2f_kv4_copy_pages(const b2f_kv4_pool* pool, const int* src, const int* dst, int n,
+                       b2f_stream_t stream);
 
 /* ------------------------------------------------------------------ op registry */
 typedef struct b2f_op {

@@ -1,0 +1,533 @@
+"""The 4-bit paged cache: writing, reading, attention and page bookkeeping against the 64-bit
+oracle.
+
+Codes and scales have to be the oracle's, bit for bit: a quotient of 16-bit values is never so
+near a border that f32 takes it to the other side.
+
+Attention, element by element: P is rounded to f16 (2^-11 of itself, and 2^-25 * 2^-7 of the
+row's largest for the smallest ones), so the sum of p |v| / sum of p, the mass, bounds that part
+at 2^-11; scores are f32 sums of exact products, off by 2^-21 of the largest sum of |q k|, which
+moves every p by as much; the output is rounded by half a step."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from helpers import gen, randn
+from oracle import serving
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16, F16, E4M3 = torch.float32, torch.bfloat16, torch.float16, torch.float8_e4m3fn
+
+
+def _cache(**kw):
+    from b200fp8.kvcache import Fp4Cache
+    return Fp4Cache(**kw)
+
+
+def _ints(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def _filled(lens, news, *, kv, d, page, g, ks=0.25, vs=0.25, dtype=BF16, layers=1, garbage=False):
+    """A cache whose sequences hold random tokens, written in two parts (the last `news` apart)."""
+    width = max(1, max(-(-n // page) for n in lens))
+    pages = sum(-(-n // page) for n in lens) + 3
+    c = _cache(layers=layers, pages=pages, page_size=page, kv_heads=kv, head_dim=d,
+               max_seqs=len(lens), max_pages=width, k_scale=ks, v_scale=vs)
+    if garbage:  # unused places hold NaN scales
+        c.storage.fill_(0xff)
+    # pages strewn over the pool
+    order = torch.randperm(pages, generator=g).int()
+    at = 0
+    for b, n in enumerate(lens):
+        m = -(-n // page)
+        c.table[b, :m] = order[at:at + m].cuda()
+        c.refs[order[at:at + m].long().cuda()] = 1
+        at += m
+    c.lens.copy_(_ints(lens))
+    total = sum(lens)
+    starts = [0]
+    for n in lens:
+        starts.append(starts[-1] + n)
+    k, v = randn((total, kv * d), g).to(dtype), randn((total, kv * d), g).to(dtype)
+    if total:
+        c.write(k.cuda(), v.cuda(), starts=_ints(starts), layer=layers - 1)
+    return c, k, v, starts
+
+
+def _oracle_kv(c, b, length, layer=0):
+    return serving.cached(c.storage[layer].cpu(), c.table[b].cpu(), length, c.page_size,
+                          c.head_dim, c.k_scale, c.v_scale)
+
+
+def _check_attention(c, q, out, lens, starts, heads, *, layer=0, causal=True, q_scale=1.0,
+                     sm_scale=None, gate=None, out_scale=1.0, lse=None, rows=None):
+    d = c.head_dim
+    half = torch.finfo(out.dtype).eps / 2
+    tiny = {BF16: 0.0, F16: 2.0 ** -25, E4M3: 2.0 ** -10}[out.dtype]
+    for b in range(len(starts) - 1):
+        row = b if rows is None else rows[b]
+        lo, hi = starts[b], starts[b + 1]
+        if lo == hi:
+            continue
+        k, v = _oracle_kv(c, row, lens[row], layer)
+        if lens[row] == 0:
+            k = v = torch.zeros((0, c.kv_heads, d), dtype=torch.float64)
+        want, l, mass, size = serving.attention(
+            q[lo:hi].double().unflatten(-1, (heads, d)) * q_scale, k, v, causal=causal,
+            sm_scale=sm_scale, gate=None if gate is None else gate[lo:hi].unflatten(-1, (heads, d)))
+        got = out[lo:hi].cpu().double().unflatten(-1, (heads, d)) * out_scale
+        if out.dtype == E4M3:  # saturates: at 448 / 256 = 1.75 here, which some values pass
+            want = want.clamp(-448 * out_scale, 448 * out_scale)
+        bound = mass * (2.0 ** -11 + 2.0 ** -16 + size * 2.0 ** -20) + want.abs() * half + \
+            tiny * out_scale
+        bad = (got - want).abs() > bound
+        assert not bool(bad.any()), (b, float((got - want).abs().max()), float(bound.max()))
+        if lse is not None:
+            have = lse[lo:hi].cpu().double()
+            assert torch.equal(torch.isinf(have), torch.isinf(l))
+            fine = ~torch.isinf(l)
+            assert bool(((have - l)[fine].abs() <= 2.0 ** -20 * (1 + size + l[fine].abs())).all())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32, E4M3])
+@pytest.mark.parametrize("d,page,kv", [(64, 16, 1), (128, 32, 3), (256, 64, 2)])
+def test_written_codes_and_read_values_are_the_oracles(dtype, d, page, kv):
+    g = gen(d + page)
+    lens = [1, page, page + 1, 3 * page - 1]
+    scale = 0.25 if dtype != F32 else 0.3
+    ins = 1 / 64 if dtype == E4M3 else 1.0
+    width = 3
+    c = _cache(layers=2, pages=12, page_size=page, kv_heads=kv, head_dim=d, max_seqs=4,
+               max_pages=width, k_scale=scale, v_scale=2 * scale)
+    c.extend(_ints(lens))
+    starts = [0]
+    for n in lens:
+        starts.append(starts[-1] + n)
+    k = randn((starts[-1], kv * d), g)
+    k[0, :16] = 0.0
+    k[1, :16] *= 1e-6   # its scale rounds to 0
+    k[2, :16] *= 1e6    # saturates
+    k[3, 16:32] = torch.arange(16) * 0.25  # values on the borders between codes
+    v = randn((starts[-1], kv * d), g) * 3
+    k, v = (k / ins).to(dtype), (v / ins).to(dtype)
+    if dtype == E4M3:
+        k, v = k.float().nan_to_num(448).to(dtype), v.float().nan_to_num(448).to(dtype)
+    other = c.storage[0].clone()
+    c.write(k.cuda(), v.cuda(), starts=_ints(starts), layer=1, k_in_scale=ins, v_in_scale=ins)
+    rk, rv = c.read(starts[-1], starts=_ints(starts), layer=1, dtype=F32)
+    torch.cuda.synchronize()
+    assert torch.equal(c.storage[0], other)
+    f32 = lambda s: float(torch.tensor(s, dtype=F32))  # noqa: E731
+    for x, read, s in ((k, rk, f32(scale)), (v, rv, f32(2 * scale))):
+        x = (x.float() * ins).unflatten(-1, (kv, d))
+        code, s8, value = serving.pack(x, s)
+        # scale * k_scale is rounded to f32 once before the code multiplies it
+        assert torch.allclose(read.cpu().unflatten(-1, (kv, d)).double(), value, atol=0,
+                              rtol=0 if dtype != F32 else 2.0 ** -23)
+    for b in range(4):
+        kk, _ = _oracle_kv(c, b, lens[b], 1)
+        assert torch.allclose(kk.flatten(1), rk[starts[b]:starts[b + 1]].cpu().double(), rtol=2e-7)
+    for half in (BF16, F16):
+        hk, hv = c.read(starts[-1], starts=_ints(starts), layer=1, dtype=half)
+        assert torch.equal(hk, rk.to(half)) and torch.equal(hv, rv.to(half))
+
+
+def test_nan_and_infinity_on_writing():
+    c = _cache(layers=1, pages=1, page_size=16, kv_heads=1, head_dim=64, max_seqs=1, max_pages=1)
+    c.extend(_ints([1]))
+    k = torch.ones((1, 64))
+    k[0, 5], k[0, 20], k[0, 40] = float("nan"), float("inf"), -float("inf")
+    c.write(k.cuda(), k.cuda())
+    rk, _ = c.read(1, dtype=F32)
+    rk = rk.cpu()[0]
+    assert bool(torch.isnan(rk[:16]).all()) and bool(torch.isfinite(rk[16:]).all())
+    assert float(rk[20]) == 448 * 6 and float(rk[40]) == -448 * 6
+
+
+def test_rows_behind_the_last_sequence_and_partial_batches():
+    """Packed rows outside of the sequences stay as they are; rows names table rows out of order."""
+    g = gen(4)
+    lens = [20, 7, 40]
+    c, _, _, _ = _filled(lens, None, kv=2, d=64, page=16, g=g)
+    starts, rows = _ints([2, 5, 6]), [2, 0]
+    k, v = randn((9, 128), g).to(BF16), randn((9, 128), g).to(BF16)
+    c.write(k.cuda(), v.cuda(), rows=_ints(rows), starts=starts)
+    rk = torch.full((9, 128), 7.0, dtype=BF16, device="cuda")
+    rv = rk.clone()
+    c.read(9, rows=_ints(rows), starts=starts, k=rk, v=rv)
+    q = randn((9, 256), g).to(BF16)
+    out = torch.full((9, 256), 5.0, dtype=BF16, device="cuda")
+    lse = torch.full((9, 4), 3.0, device="cuda")
+    c.attention(q.cuda(), heads=4, rows=_ints(rows), starts=starts, out=out, lse=lse)
+    torch.cuda.synchronize()
+    for i in (0, 1, 6, 7, 8):
+        assert bool((rk[i] == 7).all()) and bool((out[i] == 5).all()) and bool((lse[i] == 3).all())
+    _, _, want = serving.pack(k[2:6].unflatten(-1, (2, 64)), 0.25)
+    assert torch.equal(rk[2:6].cpu().double().unflatten(-1, (2, 64)), want)
+    _check_attention(c, q, out, lens, [2, 5, 6], 4, lse=lse, rows=rows)
+    from b200fp8 import device_status
+    assert device_status() == 0
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("page", [16, 32, 64])
+@pytest.mark.parametrize("heads,kv", [(1, 1), (8, 2), (16, 1), (5, 1), (40, 2)])
+def test_one_token_steps(d, page, heads, kv):
+    g = gen(d * page + heads)
+    lens = [1, 15, 16, 17, 31, 33, 64, 127, 128, 129, 300, 0]
+    c, _, _, _ = _filled(lens, None, kv=kv, d=d, page=page, g=g, garbage=True)
+    q = randn((len(lens), heads * d), g).to(BF16)
+    out, lse = c.attention(q.cuda(), heads=heads, return_lse=True)
+    torch.cuda.synchronize()
+    assert bool((out[-1] == 0).all())
+    _check_attention(c, q, out, lens, list(range(len(lens) + 1)), heads, lse=lse)
+
+
+@pytest.mark.parametrize("q_dtype,out_dtype", [(BF16, F16), (F16, BF16), (E4M3, E4M3)])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("causal", [True, False])
+def test_several_new_tokens(q_dtype, out_dtype, d, causal):
+    """Chunks of new tokens of different lengths, more of them than are cached among them (the
+    first ones see nothing), with gate and every type."""
+    g = gen(d + causal)
+    lens, news = [70, 3, 200, 33, 0, 129], [5, 3, 37, 1, 0, 129]
+    c, _, _, _ = _filled(lens, None, kv=2, d=d, page=16, g=g, garbage=True)
+    heads = 6
+    starts = [0]
+    for n in news:
+        starts.append(starts[-1] + n)
+    qs = 1 / 64 if q_dtype == E4M3 else 1.0
+    q = (randn((starts[-1], heads * d), g) / qs).clamp(-440, 440).to(q_dtype)
+    gate = (randn((starts[-1], heads * d), g) * 64).clamp(-440, 440).to(E4M3)
+    outs = 1 / 256 if out_dtype == E4M3 else 1.0
+    out, lse = c.attention(q.cuda(), heads=heads, starts=_ints(starts), causal=causal, q_scale=qs,
+                           gate=gate.cuda(), gate_scale=1 / 64, out_dtype=out_dtype,
+                           ctx_scale=outs, return_lse=True)
+    torch.cuda.synchronize()
+    _check_attention(c, q, out, lens, starts, heads, causal=causal, q_scale=qs,
+                     gate=gate.float() / 64, out_scale=outs, lse=lse)
+
+
+def test_more_new_tokens_than_cached():
+    """A sequence with fewer cached than new tokens: its first tokens see no key."""
+    g = gen(77)
+    lens = [4, 50]
+    c, _, _, _ = _filled(lens, None, kv=1, d=128, page=16, g=g)
+    starts = [0, 30, 40]
+    q = randn((40, 2 * 128), g).to(BF16)
+    out, lse = c.attention(q.cuda(), heads=2, starts=_ints(starts), return_lse=True)
+    torch.cuda.synchronize()
+    assert bool((out[:26] == 0).all()) and bool(torch.isinf(lse[:26]).all())
+    _check_attention(c, q, out, lens, starts, 2, lse=lse)
+
+
+def test_long_sequences_are_split_and_joined_the_same_every_time():
+    g = gen(12)
+    lens = [9000, 40, 3000]
+    c, _, _, _ = _filled(lens, None, kv=1, d=128, page=64, g=g)
+    q = (randn((3, 4 * 128), g) * 3).to(BF16)
+    first, l0 = c.attention(q.cuda(), heads=4, return_lse=True)
+    for _ in range(3):
+        again, l1 = c.attention(q.cuda(), heads=4, return_lse=True)
+        assert torch.equal(first, again) and torch.equal(l0, l1)
+    _check_attention(c, q, first, lens, [0, 1, 2, 3], 4, lse=l0)
+
+
+def test_a_late_large_score_moves_the_maximum():
+    """Scores that grow along the sequence by far more than the slack of the running maximum."""
+    g = gen(2)
+    n, d = 600, 64
+    c = _cache(layers=1, pages=40, page_size=16, kv_heads=1, head_dim=d, max_seqs=1, max_pages=40,
+               k_scale=1 / 16)
+    c.extend(_ints([n]))
+    k = randn((n, d), g) * 0.05 + torch.linspace(-4, 4, n)[:, None]
+    v = randn((n, d), g)
+    c.write(k.to(BF16).cuda(), v.to(BF16).cuda())
+    for sign in (1.0, -1.0):
+        q = torch.full((1, d), sign).to(BF16)
+        out, lse = c.attention(q.cuda(), heads=1, sm_scale=1.0, return_lse=True)
+        torch.cuda.synchronize()
+        _check_attention(c, q, out, [n], [0, 1], 1, sm_scale=1.0, lse=lse)
+
+
+@pytest.mark.parametrize("scale", [1e-30, 1e30])
+def test_queries_of_any_size(scale):
+    """bf16 queries outside the range of f16 lose nothing (sm_scale brings the scores back)."""
+    g = gen(6)
+    c, _, _, _ = _filled([100], None, kv=1, d=128, page=32, g=g)
+    q = (randn((1, 128), g) * scale).to(BF16)
+    out = c.attention(q.cuda(), heads=1, sm_scale=1.0 / scale)
+    torch.cuda.synchronize()
+    _check_attention(c, q, out, [100], [0, 1], 1, sm_scale=1.0 / scale)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_nan_reaches_only_those_who_see_it(d):
+    """A NaN in a late token's key or value leaves earlier tokens of the chunk alone, and one in
+    another sequence too."""
+    for which in ("k", "v"):
+        g = gen(d)
+        lens = [50, 50]
+        c, k, v, starts = _filled(lens, None, kv=1, d=d, page=16, g=g)
+        k, v = k.clone(), v.clone()
+        (k if which == "k" else v)[45, 3] = float("nan")
+        c.write(k.cuda(), v.cuda(), starts=_ints(starts))
+        q = randn((20, 2 * d), g).to(BF16)
+        out = c.attention(q.cuda(), heads=2, starts=_ints([0, 10, 20]))
+        torch.cuda.synchronize()
+        clean = torch.isfinite(out).all(1).cpu()
+        assert clean.tolist() == [True] * 5 + [False] * 5 + [True] * 10
+        assert bool(torch.isnan(out[5:10, :16]).all())
+        ok = [i for i in range(20) if clean[i]]
+        for b, lo, hi in ((0, 0, 5), (1, 10, 20)):
+            kk, vv = _oracle_kv(c, b, 50)
+            seen = 45 if b == 0 else 50
+            want, _, mass, size = serving.attention(
+                q[lo:hi].double().unflatten(-1, (2, d)), kk[:seen], vv[:seen])
+            got = out[lo:hi].cpu().double().unflatten(-1, (2, d))
+            bound = mass * (2.0 ** -11 + 2.0 ** -16 + size * 2.0 ** -20) + want.abs() * 2.0 ** -8
+            assert bool(((got - want).abs() <= bound).all())
+        assert len(ok) == 15
+
+
+def test_bad_lists_are_left_out_and_recorded():
+    """Pages and rows out of range lead nowhere: their keys are not attended, their tokens not
+    written, and the status word says so."""
+    from b200fp8 import device_status
+    g = gen(21)
+    lens = [64, 40]
+    c, _, _, _ = _filled(lens, None, kv=1, d=64, page=16, g=g)
+    good = c.table.clone()
+    assert device_status(reset=True) == 0
+    c.table[0, 1], c.table[0, 2] = c.pages + 5, -1
+    q = randn((2, 64), g).to(BF16)
+    out = c.attention(q.cuda(), heads=1)
+    torch.cuda.synchronize()
+    assert device_status(reset=True) == 5
+    k, v = serving.cached(c.storage[0].cpu(), good[0].cpu(), 64, 16, 64, 0.25, 0.25)
+    keep = [i for i in range(64) if i // 16 not in (1, 2)]
+    want, _, mass, size = serving.attention(q[:1].double().unflatten(-1, (1, 64)), k[keep], v[keep])
+    err = (out[0].cpu().double() - want.flatten()).abs()
+    bound = mass.flatten() * (2.0 ** -11 + 2.0 ** -16 + size * 2.0 ** -20) + want.flatten().abs() * 2.0 ** -8
+    assert bool((err <= bound).all())
+    before = c.storage.clone()
+    x = randn((2, 64), g).to(BF16).cuda()
+    c.write(x, x, rows=_ints([7, -3]))
+    rk, _ = c.read(2, rows=_ints([7, -3]))
+    assert torch.equal(c.storage, before) and bool((rk == 0).all())
+    out = c.attention(q.cuda(), heads=1, rows=_ints([9, 1]))
+    assert bool((out[0] == 0).all()) and bool((out[1] != 0).any())
+    assert device_status(reset=True) == 5
+    c.lens[1] = 10000  # more than the table row holds: cut off at what it holds, pages -1 left out
+    c.attention(q.cuda(), heads=1)
+    c.lens[1] = -4
+    out = c.attention(q.cuda(), heads=1)
+    assert bool((out[1] == 0).all())
+    c.lens[1] = 40
+    out = c.attention(q.cuda(), heads=1, starts=_ints([0, 5, 2]))  # not ascending, too far
+    torch.cuda.synchronize()
+    assert device_status(reset=True) == 5
+
+
+def test_two_streams_and_two_graphs_do_not_share_work():
+    """Two calls at once, and two captured graphs replayed at once, on one cache."""
+    g = gen(31)
+    lens = [2000, 1500, 7]
+    c, _, _, _ = _filled(lens, None, kv=2, d=128, page=32, g=g)
+    qs = [(randn((3, 8 * 128), g)).to(BF16).cuda() for _ in range(2)]
+    want = [c.attention(q, heads=8) for q in qs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    outs = [torch.empty_like(q) for q in qs]
+    for _ in range(5):
+        for s, q, o in zip(streams, qs, outs):
+            with torch.cuda.stream(s):
+                c.attention(q, heads=8, out=o)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(outs, want))
+    graphs = []
+    for q, o in zip(qs, outs):
+        o.zero_()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            c.attention(q, heads=8, out=o)
+        graphs.append(graph)
+    for _ in range(5):
+        for s, graph in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+def test_strided_queries_and_outputs():
+    g = gen(41)
+    lens = [77, 12]
+    c, _, _, _ = _filled(lens, None, kv=1, d=64, page=16, g=g)
+    wide = randn((2, 3 * 64 + 16), g).to(BF16)
+    gate = randn((2, 3 * 80), g).to(BF16)
+    hold = torch.full((2, 3 * 64 + 32), 9.0, dtype=F16, device="cuda")
+    c.attention(wide.cuda()[:, 16:], heads=3, gate=gate.cuda(), gate_head_stride=80,
+                out=hold[:, 16:16 + 192])
+    torch.cuda.synchronize()
+    assert bool((hold[:, :16] == 9).all()) and bool((hold[:, 208:] == 9).all())
+    gg = gate.float().unflatten(-1, (3, 80))[..., :64].flatten(1)
+    _check_attention(c, wide[:, 16:], hold[:, 16:208], lens, [0, 1, 2], 3, gate=gg)
+
+
+# ------------------------------------------------------------------------------------ pages
+
+def _same(c, o):
+    assert c.lens.tolist() == o.lens
+    assert c.refs.tolist() == o.refs
+    assert c.table.tolist() == o.table
+
+
+@pytest.mark.parametrize("seed", range(4))
+def test_page_bookkeeping_follows_the_oracle(seed):
+    """Random runs of extend, fork, free and compact, refused calls among them; the tokens of
+    every row stay what they were."""
+    from b200fp8 import device_status
+    import random
+    rng = random.Random(seed)
+    page = rng.choice([16, 32, 64])
+    rows, cols, pages = 12, 6, 30
+    c = _cache(layers=2, pages=pages, page_size=page, kv_heads=1, head_dim=64, max_seqs=rows,
+               max_pages=cols)
+    c.storage.copy_(torch.randint(0, 256, c.storage.shape, generator=gen(seed)).to(torch.uint8))
+    o = serving.Pages(pages, rows, cols, page)
+    store = c.storage.cpu().clone()
+    device_status(reset=True)
+    for step in range(40):
+        what = rng.choice(["extend", "extend", "fork", "free", "compact"])
+        bad = False
+        if what == "extend":
+            n = rng.randint(1, 4)
+            who = [rng.randrange(rows) for _ in range(n)] if rng.random() < .2 else rng.sample(range(rows), n)
+            counts = [rng.randint(0, 3 * page) for _ in who]
+            bad = not o.extend(who, counts)
+            c.extend(_ints(counts), rows=_ints(who))
+        elif what == "fork":
+            full = [r for r in range(rows) if o.lens[r]] or [0]
+            empty = [r for r in range(rows) if not o.lens[r]]
+            n = min(len(empty), rng.randint(1, 3))
+            if not n:
+                continue
+            src = [rng.choice(full) for _ in range(n)]
+            dst = rng.sample(empty, n)
+            if rng.random() < .15:
+                dst[0] = rng.randrange(-1, rows + 1)
+            bad = not o.fork(src, dst)
+            c.fork(_ints(src), _ints(dst))
+        elif what == "free":
+            who = rng.sample(range(rows), rng.randint(1, 3))
+            o.free(who)
+            c.free(_ints(who + who[:1]))
+        else:
+            o.compact()
+            c.compact()
+        for a, b in o.copies:
+            store[:, b] = store[:, a]
+        o.copies.clear()
+        torch.cuda.synchronize()
+        assert (device_status(reset=True) != 0) == bad, (what, step)
+        _same(c, o)
+        assert torch.equal(c.storage.cpu(), store)
+    assert c.free_pages() == sum(r == 0 for r in o.refs)
+
+
+def test_large_pool_and_many_rows():
+    """More pages than one round of the scan covers, 1024 rows in one call."""
+    rows, page = 1024, 16
+    c = _cache(layers=1, pages=40000, page_size=page, kv_heads=1, head_dim=64, max_seqs=rows,
+               max_pages=40)
+    o = serving.Pages(40000, rows, 40, page)
+    counts = [(i * 37) % 500 for i in range(rows)]
+    o.extend(list(range(rows)), counts)
+    c.extend(_ints(counts))
+    who = list(range(0, rows, 3))
+    o.free(who)
+    c.free(_ints(who))
+    o.compact()
+    c.compact()
+    again = [500] * len(who)
+    o.extend(who, again)
+    c.extend(_ints(again), rows=_ints(who))
+    torch.cuda.synchronize()
+    _same(c, o)
+    c.free()
+    assert c.free_pages() == 40000 and int(c.lens.sum()) == 0
+
+
+def test_too_few_pages_change_nothing():
+    from b200fp8 import device_status
+    c = _cache(layers=1, pages=5, page_size=16, kv_heads=1, head_dim=64, max_seqs=3, max_pages=9)
+    device_status(reset=True)
+    c.extend(_ints([40, 17, 0]))
+    state = [t.clone() for t in (c.table, c.lens, c.refs)]
+    c.extend(_ints([0, 0, 1]))
+    assert device_status(reset=True) == 6
+    c.fork(_ints([0]), _ints([2]))
+    assert device_status(reset=True) == 6
+    assert all(torch.equal(a, b) for a, b in zip(state, (c.table, c.lens, c.refs)))
+
+
+def test_copy_pages():
+    c = _cache(layers=3, pages=700, page_size=16, kv_heads=2, head_dim=64, max_seqs=1, max_pages=1)
+    c.storage.copy_(torch.randint(0, 256, c.storage.shape, generator=gen(1)).to(torch.uint8))
+    want = c.storage.clone()
+    src, dst = list(range(0, 600, 2)), list(range(1, 601, 2))
+    want[:, dst] = want[:, src]
+    c.copy_pages(src, dst)
+    torch.cuda.synchronize()
+    assert torch.equal(c.storage, want)
+    from b200fp8 import B2FError
+    for bad in (([1, 2], [3, 3]), ([1, 2], [2, 5]), ([1], [700]), ([-1], [0])):
+        with pytest.raises(B2FError):
+            c.copy_pages(*bad)
+
+
+def test_a_served_sequence():
+    """The operators as they are used: a prompt, forked samples that grow apart, a freed one,
+    packing, and steps of a captured graph; every step's context against the oracle."""
+    from b200fp8 import device_status, ops, rotary
+    g = gen(100)
+    kv, heads, d, page = 2, 8, 128, 16
+    c = _cache(layers=1, pages=64, page_size=page, kv_heads=kv, head_dim=d, max_seqs=6,
+               max_pages=12, k_scale=1 / 8, v_scale=1 / 8)
+    plan = rotary.RotaryPlan(d, theta=1e6, device="cuda")
+    device_status(reset=True)
+    lens = [0] * 6
+
+    def step(rows, news):
+        starts = [0]
+        for n in news:
+            starts.append(starts[-1] + n)
+        for r, n in zip(rows, news):
+            lens[r] += n
+        pos = torch.tensor([lens[r] - n + i for r, n in zip(rows, news) for i in range(n)],
+                           dtype=torch.int32)
+        q, k, v = (randn((starts[-1], h * d), g).to(BF16).cuda() for h in (heads, kv, kv))
+        c.extend(_ints(news), rows=_ints(rows))
+        q, k = ops.rotary(q, k, pos.cuda(), plan, heads=heads, kv_heads=kv)
+        c.write(k, v, rows=_ints(rows), starts=_ints(starts))
+        out, lse = c.attention(q, heads=heads, rows=_ints(rows), starts=_ints(starts),
+                               return_lse=True)
+        torch.cuda.synchronize()
+        _check_attention(c, q.cpu(), out, lens, starts, heads, lse=lse, rows=rows)
+
+    step([0, 3], [37, 20])
+    c.fork(_ints([0, 0, 3]), _ints([1, 2, 5]))
+    for r, s in ((1, 0), (2, 0), (5, 3)):
+        lens[r] = lens[s]
+    step([0, 1, 2, 3, 5], [1] * 5)
+    step([5, 2, 0], [2, 1, 17])
+    c.free(_ints([0]))
+    lens[0] = 0
+    c.compact()
+    step([1, 2, 3, 5], [1] * 4)
+    assert int((c.refs > 0).nonzero().max()) < 64 - c.free_pages() + 4
+    assert device_status() == 0
