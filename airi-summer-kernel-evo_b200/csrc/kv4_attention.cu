@@ -53,6 +53,12 @@ constexpr int kUnit = kChunk * kWarps;    // keys of a unit of work
 constexpr float kLift = 7.0f;             // P is scaled by 2^7 ...
 constexpr float kSlack = 8.0f;            // ... and the maximum may lag behind by 2^8
 
+// The item that begins in a CTA's run of units and goes on in those of the next `more` CTAs
+// (0: there is none): what the join needs of it.
+struct Shared {
+  int more, start, n, head0, row0;
+};
+
 struct Kv4AttnParams {
   Kv4Cache c;
   Kv4Batch b;
@@ -71,7 +77,8 @@ struct Kv4AttnParams {
   long long out_ld;
   float ctx_scale;
   float* lse;
-  float* partial;  // [2 * CTAs][R][D] O, then [2 * CTAs][R][2] (max, sum)
+  float* partial;  // [2 * CTAs][R][D] O, then [2 * CTAs][R][2] (base, sum)
+  Shared* shared;  // [CTAs]
   int ctas;
 };
 
@@ -102,45 +109,91 @@ __device__ __forceinline__ long long seq_units(const Kv4Seq& s, int group, int c
   return u;
 }
 
+// x / y for 0 <= x, 0 < y; the 32-bit division where it does (a tenth of the other's time).
+__device__ __forceinline__ long long divide(long long x, long long y) {
+  return ((x | y) >> 32) == 0 ? (long long)((unsigned)x / (unsigned)y) : x / y;
+}
+
+// The units of all items, cut into `ctas` runs of consecutive ones.
+struct Runs {
+  long long each, more;  // the first `more` CTAs take each + 1 units, the others `each`
+  __device__ __forceinline__ Runs(long long total, int ctas) {
+    each = divide(total, ctas);
+    more = total - each * ctas;
+  }
+  __device__ __forceinline__ long long begin(int cta) const { return each * cta + min((long long)cta, more); }
+  __device__ __forceinline__ int of(long long unit) const {  // the CTA that has it
+    const long long x = more * (each + 1);
+    return (int)(unit < x ? divide(unit, each + 1) : more + divide(unit - x, each));
+  }
+};
+
 struct Scan {
   long long warp_sum[kWarps];
   long long at;  // units before the sequence that was looked for
   int b;
 };
 
-// Units of all sequences; with find >= 0 also the sequence of unit `find` (in sc.b, sc.at).
-template <int R>
-__device__ long long scan_units(const Kv4AttnParams& p, long long find, Scan& sc) {
+// One round of kThreads sequences: units of thread's sequence base + threadIdx.x (`mine`), of
+// those before it (returned), and `before` moved on.
+__device__ __forceinline__ long long scan_round(long long mine, long long& before, Scan& sc) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  long long before = 0;
-  for (int base = 0; base < p.b.seqs; base += kThreads) {
-    const int b = base + (int)threadIdx.x;
-    long long mine = 0;
-    if (b < p.b.seqs)
-      mine = seq_units<R>(kv4_seq(p.c, p.b, b), p.group, p.causal) * p.c.kv_heads;
-    long long x = mine;
+  long long x = mine;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long y = __shfl_up_sync(0xffffffffu, x, o);
-      if (lane >= o) x += y;
-    }
-    __syncthreads();
-    if (lane == 31) sc.warp_sum[warp] = x;
-    __syncthreads();
-    long long lead = before;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      if (w < warp) lead += sc.warp_sum[w];
-      before += sc.warp_sum[w];
-    }
-    const long long start = lead + x - mine;
-    if (find >= start && find < start + mine) {
-      sc.b = b;
-      sc.at = start;
-    }
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
   }
   __syncthreads();
-  return before;
+  if (lane == 31) sc.warp_sum[warp] = x;
+  __syncthreads();
+  long long lead = before;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) lead += sc.warp_sum[w];
+    before += sc.warp_sum[w];
+  }
+  return lead + x - mine;
+}
+
+// This CTA's run of units [u0, u1), with the sequence of u0 in sc.b and the units before it in
+// sc.at.  `blank`: this CTA has to look after sequences with rows that see no key.
+template <int R>
+__device__ __forceinline__ Runs find_run(const Kv4AttnParams& p, Scan& sc, long long& u0, long long& u1, bool& blank) {
+  long long before = 0, mine = 0, start = 0;
+  bool empty = false;
+  for (int base = 0; base < p.b.seqs; base += kThreads) {
+    const int b = base + (int)threadIdx.x;
+    mine = 0;
+    if (b < p.b.seqs) {
+      const Kv4Seq s = kv4_seq(p.c, p.b, b);
+      mine = seq_units<R>(s, p.group, p.causal) * p.c.kv_heads;
+      empty |= b % gridDim.x == blockIdx.x && s.n > 0 && tile_keys<R>(s, 0, p.group, p.causal) <= 0;
+    }
+    start = scan_round(mine, before, sc);
+  }
+  const Runs runs(before, gridDim.x);
+  u0 = runs.begin(blockIdx.x);
+  u1 = runs.begin(blockIdx.x + 1);
+  if (p.b.seqs <= kThreads) {
+    if (u0 >= start && u0 < start + mine) {
+      sc.b = threadIdx.x;
+      sc.at = start;
+    }
+  } else {
+    before = 0;
+    for (int base = 0; base < p.b.seqs; base += kThreads) {
+      const int b = base + (int)threadIdx.x;
+      mine = b < p.b.seqs ? seq_units<R>(kv4_seq(p.c, p.b, b), p.group, p.causal) * p.c.kv_heads : 0;
+      start = scan_round(mine, before, sc);
+      if (u0 >= start && u0 < start + mine) {
+        sc.b = b;
+        sc.at = start;
+      }
+    }
+  }
+  blank = __syncthreads_or(empty);
+  return runs;
 }
 
 template <int R>
@@ -156,7 +209,7 @@ __device__ int find_item(const Kv4AttnParams& p, int b, long long unit, Item& it
   it.s = kv4_seq(p.c, p.b, b);
   it.rts = (it.s.n * p.group + R - 1) / R;
   const long long per = seq_units<R>(it.s, p.group, p.causal);
-  it.h = (int)(unit / per);
+  it.h = (int)divide(unit, per);
   long long rest = unit - it.h * per;
   for (it.rt = 0;; ++it.rt) {
     open_item<R>(p, it);
@@ -202,6 +255,13 @@ __device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
   uint32_t r;
   asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
+}
+
+// a times the lower (upper) half of the pair b.
+__device__ __forceinline__ uint32_t hmul2_by(uint32_t a, uint32_t b, int upper) {
+  const __half2 x = *reinterpret_cast<const __half2*>(&a), y = *reinterpret_cast<const __half2*>(&b);
+  const __half2 z = __hmul2(x, upper ? __high2half2(y) : __low2half2(y));
+  return *reinterpret_cast<const uint32_t*>(&z);
 }
 
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
@@ -300,12 +360,12 @@ struct Layout {
   static constexpr int kBytes = kRing + kJoin;
 };
 
-template <int D, int NT, int STAGES>
-__global__ void __launch_bounds__(kThreads) kv4_attention_kernel(const Kv4AttnParams p) {
+template <int D, int NT, int STAGES, int CTAS>
+__global__ void __launch_bounds__(kThreads, CTAS) kv4_attention_kernel(const Kv4AttnParams p) {
   using L = Layout<D, NT, STAGES>;
   constexpr int R = L::R;
   constexpr int kSteps = D / 16;         // k16 steps of Q.K; m16 tiles of O^T
-  constexpr int kWordsK = D / 32;        // 32-bit words of K codes of a thread and key
+  constexpr int kWordsK = D / 32;        // 32-bit words of K codes (16 queries' worth) of a thread
   constexpr int kWordsV = D / 64;        // words of V codes of a thread and key
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ Scan sc;
@@ -325,8 +385,11 @@ __global__ void __launch_bounds__(kThreads) kv4_attention_kernel(const Kv4AttnPa
   pdl_wait();
   pdl_trigger();
 
+  long long u0, u1;
+  bool blank;
+  const Runs runs = find_run<R>(p, sc, u0, u1, blank);
   // rows that see no key at all: zeros
-  for (int b = blockIdx.x; b < p.b.seqs; b += gridDim.x) {
+  for (int b = blockIdx.x; blank && b < p.b.seqs; b += gridDim.x) {
     Item it;
     it.s = kv4_seq(p.c, p.b, b);
     it.b = b;
@@ -346,79 +409,79 @@ __global__ void __launch_bounds__(kThreads) kv4_attention_kernel(const Kv4AttnPa
       }
     }
   }
-
-  const long long total = scan_units<R>(p, -1, sc);
-  const long long u0 = total * blockIdx.x / gridDim.x, u1 = total * (blockIdx.x + 1) / gridDim.x;
+  if (threadIdx.x == 0) p.shared[blockIdx.x].more = 0;
   if (u0 >= u1) return;
-  scan_units<R>(p, u0, sc);
-  Item it;       // of the keys that are worked on
-  int u = find_item<R>(p, sc.b, u0 - sc.at, it);
-  Item ahead = it;  // of the keys that are fetched
-  int ahead_u = u;
-  long long fetched = u0;  // unit that is fetched next
-  int issued = 0;          // chunks whose copies this warp has started
-  bool alive = true;       // false once a copy did not arrive in time: no more work, no more copies
+  Item it;                    // the item that is worked on, from unit `first` on
+  int first = find_item<R>(p, sc.b, u0 - sc.at, it);
+  long long left = u1 - u0;   // units from there to the end of the CTA's run
+  Item ahead = it;            // the item whose pages are fetched
+  long long ahead_left = left;
 
-  // The page of a lane's copies: lane = 4 * (page of the chunk) + part of the block.
+  // ---- the fetching side: a lane of 4 * (page of the chunk) + part of the block copies its part
   const int log2p = p.c.page_log2;
   const int pages_per_chunk = log2p == 4 ? 2 : 1;
-  const int keys_per_page = log2p == 4 ? 16 : 32;  // of the chunk
-  const bool copies = lane < 4 * pages_per_chunk;
   const int part = lane & 3, sub = lane >> 2;
+  const bool copies = lane < 4 * pages_per_chunk;
+  const int row_bytes = part & 1 ? D / 16 : D / 2;
+  const uint32_t copy_bytes = (log2p == 4 ? 16 : 32) * row_bytes;
+  const uint32_t page_bytes = (log2p == 4 ? 16 : 32) * (D / 8 * 9);  // all parts of a page's share
+  const int from_part = (part >> 1) * (p.c.codes_bytes + p.c.scales_bytes) + (part & 1 ? p.c.codes_bytes : 0);
+  uint8_t* const to_part = ring + (part >> 1) * (L::kCodes + L::kScales) + (part & 1 ? L::kCodes : 0) + sub * 16 * row_bytes;
   const uint64_t policy = policy_evict_normal();
-  auto page_of = [&](const Item& x, int key) -> int {
-    if (!copies || key + sub * 16 >= x.keys) return -2;
-    return p.c.table[(long long)x.s.row * p.c.table_ld + ((key + sub * 16) >> log2p)];
+  bool alive = true;       // false once a copy did not arrive in time: no more work, no more copies
+  int ahead_key, ahead_end;            // this warp's next chunk of the item, and where its keys end
+  const uint8_t* ahead_block;
+  const int* ahead_pages;
+  int next_page = -2;                  // page of the lane's next copy; -2: none
+  int fetch_stage = 0, in_ring = 0;    // chunks whose copies were started and not yet worked on
+  auto open_ahead = [&](int unit) {
+    const int take = (int)min((long long)(ahead.units - unit), ahead_left);
+    ahead_left -= take;
+    ahead_key = unit * kUnit + warp * kChunk;
+    ahead_end = min((unit + take) * kUnit, ahead.keys);
+    ahead_block = p.c.storage + (long long)ahead.h * p.c.block_bytes + from_part;
+    ahead_pages = p.c.table + (long long)ahead.s.row * p.c.table_ld;
   };
-  // skips over units in which this warp has no key, then the page of the next copy
-  auto seek = [&]() {
-    while (fetched < u1 && ahead_u * kUnit + warp * kChunk >= ahead.keys) {
-      if (++fetched < u1 && ++ahead_u == ahead.units) {
-        next_item<R>(p, ahead);
-        ahead_u = 0;
+  auto find_page = [&]() {  // of the next chunk; moves on to the next item with a chunk for this warp
+    while (ahead_key >= ahead_end && ahead_left > 0) {
+      next_item<R>(p, ahead);
+      open_ahead(0);
+    }
+    next_page = -2;
+    if (copies && ahead_key + sub * 16 < ahead_end) {
+      next_page = ahead_pages[(ahead_key + sub * 16) >> log2p];
+      if ((unsigned)next_page >= (unsigned)p.c.pages) {
+        record_error(kDevBadArgs);
+        next_page = -2;
       }
     }
   };
-  seek();
-  int next_page = fetched < u1 ? page_of(ahead, ahead_u * kUnit + warp * kChunk) : -2;
   auto fetch = [&]() {
-    if (fetched >= u1 || !alive) return;
-    const int key = ahead_u * kUnit + warp * kChunk;
-    const int st = issued % STAGES;
-    const bool ok = next_page >= 0 && next_page < p.c.pages;
-    if (copies && next_page != -2 && !ok) record_error(kDevBadArgs);
-    const unsigned good = __ballot_sync(0xffffffffu, copies && ok);
-    const uint32_t bytes = part & 1 ? keys_per_page * (D / 16) : keys_per_page * (D / 2);
+    if (ahead_key >= ahead_end || !alive) return;
+    const unsigned good = __ballot_sync(0xffffffffu, next_page >= 0) & 0x11;
     if (lane == 0) {
-      stage_ok[warp][st] = (good & 1) | ((good >> 4) & 1) << 1;
-      mbar_arrive_expect_tx(&bars[warp][st], (L::kStage / pages_per_chunk) * __popc(good & 0x11));
+      stage_ok[warp][fetch_stage] = (good & 1) | good >> 3;
+      mbar_arrive_expect_tx(&bars[warp][fetch_stage], page_bytes * __popc(good));
     }
     __syncwarp();
-    if (copies && ok) {
-      const uint8_t* from = p.c.storage + (long long)next_page * p.c.page_stride +
-                            (long long)ahead.h * p.c.block_bytes +
-                            (part >> 1) * (p.c.codes_bytes + p.c.scales_bytes) +
-                            (part & 1 ? p.c.codes_bytes : 0) +
-                            (key & (p.c.page_size - 1)) * (part & 1 ? D / 16 : D / 2);
-      uint8_t* to = ring + st * L::kStage + (part >> 1) * (L::kCodes + L::kScales) +
-                    (part & 1 ? L::kCodes : 0) + sub * 16 * (part & 1 ? D / 16 : D / 2);
-      bulk_load(to, from, bytes, &bars[warp][st], policy);
-    }
-    ++issued;
-    if (++fetched < u1 && ++ahead_u == ahead.units) {
-      next_item<R>(p, ahead);
-      ahead_u = 0;
-    }
-    seek();
-    next_page = fetched < u1 ? page_of(ahead, ahead_u * kUnit + warp * kChunk) : -2;
+    if (next_page >= 0)
+      bulk_load(to_part + fetch_stage * L::kStage,
+                ahead_block + next_page * p.c.page_stride + (ahead_key & (p.c.page_size - 1)) * row_bytes,
+                copy_bytes, &bars[warp][fetch_stage], policy);
+    fetch_stage = fetch_stage + 1 == STAGES ? 0 : fetch_stage + 1;
+    ++in_ring;
+    ahead_key += kUnit;
+    find_page();
   };
+  open_ahead(first);
+  find_page();
   for (int s = 0; s < STAGES; ++s) fetch();
 
-  int done = 0;  // chunks worked on
-  long long unit = u0;
-  while (unit < u1) {
-    const int piece_begin = u;  // units [piece_begin, piece_end) of the item
-    const int piece_end = (int)min((long long)it.units, u + (u1 - unit));
+  int stage = 0;
+  uint32_t phase = 0;
+  while (left > 0) {
+    const int take = (int)min((long long)(it.units - first), left);  // units [first, first + take) of the item
+    const int end = min((first + take) * kUnit, it.keys);
     // ---- the queries of the tile, and what a score is multiplied by
     uint32_t qf[NT][kSteps][2];
     float mul[NT][2];
@@ -472,12 +535,13 @@ __global__ void __launch_bounds__(kThreads) kv4_attention_kernel(const Kv4AttnPa
     }
     lowest = __reduce_min_sync(0xffffffffu, lowest);
 
-    float ref[NT][2], sum[NT][2], o[kSteps][NT][4];
+    // P = 2^(score - base); base is 7 below the largest score seen when it was last moved
+    float base[NT][2], sum[NT][2], o[kSteps][NT][4];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        ref[nt][j] = -INFINITY;
+        base[nt][j] = -INFINITY;
         sum[nt][j] = 0.f;
       }
 #pragma unroll
@@ -486,122 +550,172 @@ __global__ void __launch_bounds__(kThreads) kv4_attention_kernel(const Kv4AttnPa
         for (int j = 0; j < 4; ++j) o[s][nt][j] = 0.f;
     }
 
-    for (; u < piece_end; ++u, ++unit) {
-      const int key0 = u * kUnit + warp * kChunk;
-      if (key0 >= it.keys) continue;
-      const int st = done % STAGES;
-      if (done < issued &&
-          !__all_sync(0xffffffffu, mbar_wait(&bars[warp][st], (done / STAGES) & 1, kDevTimeoutMma, nullptr)))
+    for (int key0 = first * kUnit + warp * kChunk; key0 < end; key0 += kUnit) {
+      if (in_ring > 0 &&
+          !__all_sync(0xffffffffu, mbar_wait(&bars[warp][stage], phase, kDevTimeoutMma, nullptr)))
         alive = false;
-      ++done;
-      const uint8_t* kc = ring + st * L::kStage;
+      --in_ring;
+      const uint8_t* kc = ring + stage * L::kStage;
       const uint8_t* ks = kc + L::kCodes;
       const uint8_t* vc = ks + L::kScales;
       const uint8_t* vs = vc + L::kCodes;
-      const int okay = stage_ok[warp][st];
+      const int okay = stage_ok[warp][stage];
       const bool edge = key0 + kChunk > lowest || okay != (1 << pages_per_chunk) - 1;
+      if (++stage == STAGES) {
+        stage = 0;
+        phase ^= 1;
+      }
       if (alive) {
+        // ---- S^T: two times 16 keys x R rows, each in two chains of sums
+        float s[2][NT][4], s2[2][NT][4];
 #pragma unroll
-        for (int g = 0; g < kChunk / 16; ++g) {
-          // ---- S^T: 16 keys x R rows
-          float s[NT][4];
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
-          const int kr = g * 16 + (r >> 1) + (r & 1) * 4;  // key of slot r; slot r + 8: kr + 8
-          uint32_t w0[kWordsK], w1[kWordsK], sc0, sc1;     // codes, scales of both keys
-          if (D == 64) {
-            const uint2 a = *reinterpret_cast<const uint2*>(kc + kr * 32 + c * 8);
-            const uint2 b = *reinterpret_cast<const uint2*>(kc + (kr + 8) * 32 + c * 8);
-            w0[0] = a.x; w0[1] = a.y; w1[0] = b.x; w1[1] = b.y;
-            sc0 = ks[kr * 4 + c];
-            sc1 = ks[(kr + 8) * 4 + c];
-          } else {
-#pragma unroll
-            for (int half = 0; half < kWordsK / 4; ++half) {
-              const uint4 a = *reinterpret_cast<const uint4*>(kc + kr * (D / 2) + half * 64 + c * 16);
-              const uint4 b = *reinterpret_cast<const uint4*>(kc + (kr + 8) * (D / 2) + half * 64 + c * 16);
-              w0[4 * half] = a.x; w0[4 * half + 1] = a.y; w0[4 * half + 2] = a.z; w0[4 * half + 3] = a.w;
-              w1[4 * half] = b.x; w1[4 * half + 1] = b.y; w1[4 * half + 2] = b.z; w1[4 * half + 3] = b.w;
-            }
-            sc0 = *reinterpret_cast<const uint16_t*>(ks + kr * (D / 16) + 2 * c);
-            sc1 = *reinterpret_cast<const uint16_t*>(ks + (kr + 8) * (D / 16) + 2 * c);
-            if (D == 256) {
-              sc0 |= uint32_t(*reinterpret_cast<const uint16_t*>(ks + kr * 16 + 8 + 2 * c)) << 16;
-              sc1 |= uint32_t(*reinterpret_cast<const uint16_t*>(ks + (kr + 8) * 16 + 8 + 2 * c)) << 16;
-            }
-          }
-#pragma unroll
-          for (int w = 0; w < kWordsK; ++w) {  // a word is two steps; two words share a scale
-            const uint32_t one0 = (sc0 >> (8 * (w / 2))) & 0xff, one1 = (sc1 >> (8 * (w / 2))) & 0xff;
-            const uint32_t m0 = e4m3x2_to_f16x2(one0 * 0x101), m1 = e4m3x2_to_f16x2(one1 * 0x101);
-            uint32_t f0[4], f1[4];
-            e2m1x8_to_f16x2(w0[w], f0);
-            e2m1x8_to_f16x2(w1[w], f1);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              f0[i] = hmul2(f0[i], m0);
-              f1[i] = hmul2(f1[i], m1);
-            }
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              mma16816(s[nt], f0[0], f1[0], f0[1], f1[1], qf[nt][2 * w][0], qf[nt][2 * w][1]);
-              mma16816(s[nt], f0[2], f1[2], f0[3], f1[3], qf[nt][2 * w + 1][0], qf[nt][2 * w + 1][1]);
-            }
-          }
-          // ---- scores to P
-          bool seen[NT][4];
+        for (int g = 0; g < 2; ++g)
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              s[nt][j] *= mul[nt][j & 1];
-              seen[nt][j] = true;
-              if (edge) {
-                const int key = kr + (j >> 1) * 8;
-                seen[nt][j] = key0 + key < limit[nt][j & 1] &&
-                              (okay >> (pages_per_chunk == 2 ? g : 0) & 1);
-                if (!seen[nt][j]) s[nt][j] = -INFINITY;
+            for (int j = 0; j < 4; ++j) s[g][nt][j] = s2[g][nt][j] = 0.f;
+        const int kr = (r >> 1) + (r & 1) * 4;  // key of slot r (of the first 16); slot r + 8: kr + 8
+#pragma unroll
+        for (int half = 0; half < (D == 256 ? 2 : 1); ++half) {
+          constexpr int kW = D == 64 ? 2 : 4;  // words of a run of codes
+          uint32_t w[4][kW], m[4];             // codes of the keys kr + 8 i, scales of two groups as f16
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int key = kr + 8 * i;
+            if (D == 64) {
+              const uint2 a = *reinterpret_cast<const uint2*>(kc + key * 32 + c * 8);
+              w[i][0] = a.x; w[i][1] = a.y;
+              m[i] = e4m3x2_to_f16x2(ks[key * 4 + c]);
+            } else {
+              const uint4 a = *reinterpret_cast<const uint4*>(kc + key * (D / 2) + half * 64 + c * 16);
+              w[i][0] = a.x; w[i][1] = a.y; w[i][kW - 2] = a.z; w[i][kW - 1] = a.w;
+              m[i] = e4m3x2_to_f16x2(*reinterpret_cast<const uint16_t*>(ks + key * (D / 16) + 8 * half + 2 * c));
+            }
+          }
+#pragma unroll
+          for (int x = 0; x < kW; ++x) {  // a word is two steps; two words share a scale
+            const int st = 2 * (half * kW + x);
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+              uint32_t f0[4], f1[4];
+              e2m1x8_to_f16x2(w[2 * g][x], f0);
+              e2m1x8_to_f16x2(w[2 * g + 1][x], f1);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                f0[i] = hmul2_by(f0[i], m[2 * g], D == 64 ? 0 : x / 2);
+                f1[i] = hmul2_by(f1[i], m[2 * g + 1], D == 64 ? 0 : x / 2);
+              }
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                mma16816(s[g][nt], f0[0], f1[0], f0[1], f1[1], qf[nt][st][0], qf[nt][st][1]);
+                mma16816(s2[g][nt], f0[2], f1[2], f0[3], f1[3], qf[nt][st + 1][0], qf[nt][st + 1][1]);
               }
             }
-          bool jump = false;
+          }
+        }
+        // ---- scores to P
+        float x[2][NT][4];
+        float top = -INFINITY;
+        unsigned hidden = 0;  // bit (g * NT + nt) * 4 + j: the row does not see the key
+        if (edge) {
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) jump |= fmaxf(s[nt][j], s[nt][j + 2]) > ref[nt][j] + kSlack;
-          if (__any_sync(0xffffffffu, jump)) {
+          for (int g = 0; g < 2; ++g)
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-              for (int j = 0; j < 2; ++j) {
-                float m = fmaxf(s[nt][j], s[nt][j + 2]);
-                m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
-                m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
-                m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-                m = fmaxf(m, ref[nt][j]);
-                const float f = m == ref[nt][j] ? 1.f : ex2(ref[nt][j] - m);
-                ref[nt][j] = m;
-                sum[nt][j] *= f;
-#pragma unroll
-                for (int t = 0; t < kSteps; ++t) {
-                  o[t][nt][j] *= f;
-                  o[t][nt][j + 2] *= f;
+              for (int j = 0; j < 4; ++j) {
+                const int key = key0 + g * 16 + kr + (j >> 1) * 8;
+                if (key >= limit[nt][j & 1] || !(okay >> (pages_per_chunk == 2 ? g : 0) & 1)) {
+                  hidden |= 1u << ((g * NT + nt) * 4 + j);
+                  s[g][nt][j] = -INFINITY;
                 }
               }
-          }
+        }
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              s[g][nt][j] += s2[g][nt][j];
+              x[g][nt][j] = fmaf(s[g][nt][j], mul[nt][j & 1], -base[nt][j & 1]);
+              top = fmaxf(top, x[g][nt][j]);  // a first score is infinitely far above the base
+            }
+        if (__any_sync(0xffffffffu, top > kSlack + kLift)) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              float m = fmaxf(fmaxf(s[0][nt][j], s[0][nt][j + 2]), fmaxf(s[1][nt][j], s[1][nt][j + 2])) * mul[nt][j];
+              m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+              m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+              m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+              m = fmaxf(m - kLift, base[nt][j]);
+              const float f = m == base[nt][j] ? 1.f : ex2(base[nt][j] - m);
+              base[nt][j] = m;
+              sum[nt][j] *= f;
+#pragma unroll
+              for (int t = 0; t < kSteps; ++t) {
+                o[t][nt][j] *= f;
+                o[t][nt][j + 2] *= f;
+              }
+#pragma unroll
+              for (int g = 0; g < 2; ++g) {
+                x[g][nt][j] = fmaf(s[g][nt][j], mul[nt][j], -m);
+                x[g][nt][j + 2] = fmaf(s[g][nt][j + 2], mul[nt][j], -m);
+              }
+            }
+        }
+        if (edge) {
+#pragma unroll
+          for (int g = 0; g < 2; ++g)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                if (hidden >> ((g * NT + nt) * 4 + j) & 1) x[g][nt][j] = -INFINITY;
+        }
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              x[g][nt][j] = ex2(x[g][nt][j]);
+              sum[nt][j & 1] += x[g][nt][j];
+            }
+        if (edge) {
+          // What a row may not see must not reach it: 0 * NaN would.  NaN scales (of keys behind
+          // the last, or of tokens that only later rows see) count as 0 below, and a row that
+          // does see a NaN gets it through P.
+#pragma unroll
+          for (int g = 0; g < 2; ++g)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const uint8_t* row = vs + (g * 16 + kr + j * 8) * (D / 16);
+              bool nan = false;
+#pragma unroll
+              for (int i = 0; i < D / 16; ++i) nan |= e4m3_is_nan(row[i]);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+                  if (nan && !(hidden >> ((g * NT + nt) * 4 + 2 * j + k) & 1)) x[g][nt][2 * j + k] = NAN;
+            }
+        }
+        // ---- O^T += V^T P^T
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
           uint32_t pf[NT][2];
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const float base = ref[nt][j & 1] == -INFINITY ? 0.f : ref[nt][j & 1] - kLift;
-              s[nt][j] = ex2(s[nt][j] - base);
-              sum[nt][j & 1] += s[nt][j];
-            }
+            pf[nt][0] = transpose8x8(pack_f16x2(x[g][nt][0], x[g][nt][1]));
+            pf[nt][1] = transpose8x8(pack_f16x2(x[g][nt][2], x[g][nt][3]));
           }
-          // ---- V: codes of keys c, c + 4, c + 8, c + 12 of the 16
+          // codes and scales of keys c, c + 4, c + 8, c + 12 of the 16
           const uint8_t* vk = vc + (g * 16 + c) * (D / 2) + r * (D / 16);
-          uint32_t v[4][kWordsV == 0 ? 1 : kWordsV], vm[4];
           const uint8_t* vsk = vs + (g * 16 + c) * (D / 16) + (r * (D / 8)) / 16;
+          uint32_t v[4][kWordsV], vm[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             if (D == 64) {
@@ -622,37 +736,25 @@ __global__ void __launch_bounds__(kThreads) kv4_attention_kernel(const Kv4AttnPa
             }
           }
           if (edge) {
-            // What a row may not see must not reach it: 0 * NaN would.  NaN scales (of keys
-            // behind the last, or of tokens that only later rows see) count as 0 here, and a row
-            // that does see a NaN gets it through P.
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              const int key = kr + j * 8;
-              bool nan = false;
-#pragma unroll
-              for (int i = 0; i < D / 16; ++i) nan |= e4m3_is_nan(vs[key * (D / 16) + i]);
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt) {
-                if (nan && seen[nt][2 * j]) s[nt][2 * j] = NAN;
-                if (nan && seen[nt][2 * j + 1]) s[nt][2 * j + 1] = NAN;
-              }
-            }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               if (e4m3_is_nan(vm[i])) vm[i] &= 0xff00;
               if (D == 256 && e4m3_is_nan(vm[i] >> 8)) vm[i] &= 0xff;
             }
           }
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            pf[nt][0] = transpose8x8(pack_f16x2(s[nt][0], s[nt][1]));
-            pf[nt][1] = transpose8x8(pack_f16x2(s[nt][2], s[nt][3]));
+          uint32_t vm01[D == 256 ? 2 : 1], vm23[D == 256 ? 2 : 1];  // scales of two keys as f16 pairs
+          if (D == 256) {
+            vm01[0] = e4m3x2_to_f16x2(__byte_perm(vm[0], vm[1], 0x0040));
+            vm23[0] = e4m3x2_to_f16x2(__byte_perm(vm[2], vm[3], 0x0040));
+            vm01[D == 256] = e4m3x2_to_f16x2(__byte_perm(vm[0], vm[1], 0x0051));
+            vm23[D == 256] = e4m3x2_to_f16x2(__byte_perm(vm[2], vm[3], 0x0051));
+          } else {
+            vm01[0] = e4m3x2_to_f16x2(vm[0] + vm[1] * 256);
+            vm23[0] = e4m3x2_to_f16x2(vm[2] + vm[3] * 256);
           }
 #pragma unroll
           for (int w = 0; w < kWordsV; ++w) {  // a word: four tiles
-            const int sh = D == 256 ? 8 * (w / 2) : 0;
-            const uint32_t m01 = e4m3x2_to_f16x2(((vm[0] >> sh) & 0xff) | ((vm[1] >> sh) & 0xff) << 8);
-            const uint32_t m23 = e4m3x2_to_f16x2(((vm[2] >> sh) & 0xff) | ((vm[3] >> sh) & 0xff) << 8);
+            const uint32_t m01 = D == 256 ? vm01[w / 2] : vm01[0], m23 = D == 256 ? vm23[w / 2] : vm23[0];
             uint32_t lo01[4], hi01[4], lo23[4], hi23[4];
             e2m1x8_to_f16x2((v[0][w] & 0x0f0f0f0fu) | ((v[1][w] << 4) & 0xf0f0f0f0u), lo01);
             e2m1x8_to_f16x2(((v[0][w] >> 4) & 0x0f0f0f0fu) | (v[1][w] & 0xf0f0f0f0u), hi01);
@@ -683,7 +785,7 @@ __global__ void __launch_bounds__(kThreads) kv4_attention_kernel(const Kv4AttnPa
         l += __shfl_xor_sync(0xffffffffu, l, 16);
         const int row = nt * 8 + 2 * c + j;
         if (r == 0) {
-          join_ms[warp][row][0] = ref[nt][j] == -INFINITY ? -INFINITY : ref[nt][j] - kLift;
+          join_ms[warp][row][0] = base[nt][j];
           join_ms[warp][row][1] = l;
         }
         float* to = join + (warp * R + row) * (D + L::kPad) + r * (D / 8);
@@ -693,8 +795,11 @@ __global__ void __launch_bounds__(kThreads) kv4_attention_kernel(const Kv4AttnPa
               make_float4(o[t][nt][j], o[t][nt][j + 2], o[t + 1][nt][j], o[t + 1][nt][j + 2]);
       }
     __syncthreads();
-    const bool from_start = piece_begin == 0;
-    const bool to_end = piece_end == it.units;
+    const bool from_start = first == 0, to_end = first + take == it.units;
+    if (from_start && !to_end && threadIdx.x == 0) {
+      const int last = runs.of(u1 - left + it.units - 1);  // the CTA with the item's last unit
+      p.shared[blockIdx.x] = Shared{last - (int)blockIdx.x, it.s.start, it.s.n, it.h * p.group, it.rt * R};
+    }
     const int slot = 2 * blockIdx.x + (from_start ? 1 : 0);
     float* part_o = p.partial + (long long)slot * R * D;
     float* part_ms = p.partial + 2ll * p.ctas * R * D + (long long)slot * R * 2;
@@ -728,55 +833,56 @@ __global__ void __launch_bounds__(kThreads) kv4_attention_kernel(const Kv4AttnPa
       }
     }
     __syncthreads();
-    if (unit < u1) {
+    left -= take;
+    if (left > 0) {
       next_item<R>(p, it);
-      u = 0;
+      first = 0;
     }
   }
 }
 
-// Joins the pieces of the item that begins among the units of CTA blockIdx.x and goes on in
-// the next ones.  One row of the item a CTA; each warp takes every fourth piece.
+// Joins the pieces of the item that begins in the run of CTA blockIdx.x and goes on in the
+// next ones.  A CTA for each row; each warp takes every fourth piece.
 template <int D, int NT>
 __global__ void __launch_bounds__(kThreads) kv4_attention_join_kernel(const Kv4AttnParams p) {
   constexpr int R = 8 * NT;
   constexpr int kPer = D / 32;  // elements of a lane
-  __shared__ Scan sc;
   __shared__ float acc_s[kWarps][D], ms[kWarps][2];
   pdl_wait();
   pdl_trigger();
-  const long long total = scan_units<R>(p, -1, sc);
-  const int n = p.ctas, me = blockIdx.x, row = blockIdx.y;
-  const long long u0 = total * me / n, u1 = total * (me + 1) / n;
-  if (u0 >= u1 || u1 >= total) return;
-  scan_units<R>(p, u1 - 1, sc);
-  Item it;
-  const int at = find_item<R>(p, sc.b, u1 - 1 - sc.at, it);
-  const long long begin = u1 - 1 - at, end = begin + it.units;
-  if (begin < u0 || end <= u1) return;
-  int head;
-  const int t = row_token(p, it, it.rt * R + row, head);
-  if (t < 0) return;
+  const int me = blockIdx.x, row = blockIdx.y;
+  const Shared it = p.shared[me];
+  if (it.more == 0) return;
+  const int i = (it.row0 + row) / p.group;
+  if (i >= it.n) return;
+  const int t = it.start + i, head = it.head0 + (it.row0 + row) - i * p.group;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const float* all_ms = p.partial + 2ll * n * R * D;
+  const float* all_ms = p.partial + 2ll * p.ctas * R * D;
 
   float m = -INFINITY, l = 0.f, acc[kPer];
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) acc[i] = 0.f;
-  for (int x = me + warp; x < n && total * x / n < end; x += kWarps) {
-    if (total * x / n == total * (x + 1) / n) continue;  // a CTA without units
-    const long long slot = 2ll * x + (x == me ? 1 : 0);
-    const float mx = all_ms[(slot * R + row) * 2], lx = all_ms[(slot * R + row) * 2 + 1];
+  for (int k = 0; k < kPer; ++k) acc[k] = 0.f;
+#pragma unroll 4
+  for (int x = warp; x <= it.more; x += kWarps) {
+    const long long slot = 2ll * (me + x) + (x == 0 ? 1 : 0);
+    const float2 msx = *reinterpret_cast<const float2*>(all_ms + (slot * R + row) * 2);
     const float* o = p.partial + (slot * R + row) * D + lane * kPer;
-    const float top = fmaxf(m, mx);
-    const float f = m == top ? 1.f : ex2(m - top), g = mx == top ? 1.f : ex2(mx - top);
-    m = top;
-    l = l * f + lx * g;
+    float y[kPer];
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) acc[i] = acc[i] * f + o[i] * g;
+    for (int k = 0; k < kPer; k += 2) {
+      const float2 v = *reinterpret_cast<const float2*>(o + k);
+      y[k] = v.x;
+      y[k + 1] = v.y;
+    }
+    const float top = fmaxf(m, msx.x);
+    const float f = m == top ? 1.f : ex2(m - top), g = msx.x == top ? 1.f : ex2(msx.x - top);
+    m = top;
+    l = l * f + msx.y * g;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) acc[k] = acc[k] * f + y[k] * g;
   }
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) acc_s[warp][lane * kPer + i] = acc[i];
+  for (int k = 0; k < kPer; ++k) acc_s[warp][lane * kPer + k] = acc[k];
   if (lane == 0) {
     ms[warp][0] = m;
     ms[warp][1] = l;
@@ -801,18 +907,19 @@ __global__ void __launch_bounds__(kThreads) kv4_attention_join_kernel(const Kv4A
   if (threadIdx.x == 0) finish_lse(p, t, head, top, l);
 }
 
-constexpr int kMaxPerSm = 3;
+constexpr int kMaxPerSm = 4;
 
 int tile_rows(int head_dim, long long rows) { return head_dim == 256 || rows <= 8 ? 8 : 16; }
 
-template <int D, int NT, int STAGES>
+template <int D, int NT, int STAGES, int CTAS>
 int launch_attention(Kv4AttnParams& p, cudaStream_t s) {
   using L = Layout<D, NT, STAGES>;
-  const int per_sm = std::min(kMaxPerSm, std::max(1, 225 * 1024 / (L::kBytes + 4096)));
-  p.ctas = sm_count() * per_sm;
-  B2F_CUDA_TRY(cudaFuncSetAttribute(kv4_attention_kernel<D, NT, STAGES>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+  static_assert(CTAS <= kMaxPerSm && CTAS * (L::kBytes + 2048) <= 227 * 1024, "CTAS CTAs fit on an SM");
+  p.ctas = sm_count() * CTAS;
+  p.shared = reinterpret_cast<Shared*>(p.partial + 2ll * p.ctas * L::R * (D + 2));
+  B2F_CUDA_TRY(cudaFuncSetAttribute(kv4_attention_kernel<D, NT, STAGES, CTAS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                     L::kBytes));
-  B2F_CUDA_TRY(launch_pdl(kv4_attention_kernel<D, NT, STAGES>, dim3((unsigned)p.ctas), dim3(kThreads), L::kBytes, s, p));
+  B2F_CUDA_TRY(launch_pdl(kv4_attention_kernel<D, NT, STAGES, CTAS>, dim3((unsigned)p.ctas), dim3(kThreads), L::kBytes, s, p));
   B2F_CUDA_TRY(launch_pdl(kv4_attention_join_kernel<D, NT>, dim3((unsigned)p.ctas, 8 * NT), dim3(kThreads), 0, s, p));
   return B2F_OK;
 }
@@ -836,7 +943,8 @@ long long b2f_kv4_attention_workspace_bytes(int head_dim) {
   const int sms = b2f::sm_count();
   if (sms <= 0) return -1;
   const int rows = head_dim == 256 ? 8 : 16;
-  return 2ll * sms * b2f::kMaxPerSm * rows * (head_dim + 2) * 4;
+  const long long ctas = (long long)sms * b2f::kMaxPerSm;
+  return ctas * (2ll * rows * (head_dim + 2) * 4 + (long long)sizeof(b2f::Shared));
 }
 
 int b2f_kv4_attention(const b2f_kv4_attn_args* a, b2f_stream_t stream) {
@@ -867,6 +975,7 @@ int b2f_kv4_attention(const b2f_kv4_attn_args* a, b2f_stream_t stream) {
     if (a->gate_dtype == B2F_DTYPE_BF16 && (reinterpret_cast<uintptr_t>(a->gate) & 1))
       return fail(B2F_ERR_ARG, "kv4_attention: misaligned gate");
   }
+  if (!(a->q_scale > 0.f) || !std::isfinite(a->q_scale)) return fail(B2F_ERR_ARG, "kv4_attention: q_scale must be > 0");
   if (!(a->ctx_scale > 0.f) || !std::isfinite(a->ctx_scale)) return fail(B2F_ERR_ARG, "kv4_attention: ctx_scale must be > 0");
   if (a->out_dtype != B2F_DTYPE_E4M3 && a->ctx_scale != 1.0f)
     return fail(B2F_ERR_ARG, "kv4_attention: ctx_scale belongs to an e4m3 output");
@@ -889,9 +998,9 @@ int b2f_kv4_attention(const b2f_kv4_attn_args* a, b2f_stream_t stream) {
   // 16 rows a tile read every key half as often as 8 do, once there are more than 8.
   const long long most = a->batch.starts != nullptr ? a->batch.tokens : a->batch.tokens / a->batch.seqs;
   const int rows = tile_rows(d, most * p.group);
-  if (d == 64) return rows == 8 ? launch_attention<64, 1, 4>(p, s) : launch_attention<64, 2, 4>(p, s);
-  if (d == 128) return rows == 8 ? launch_attention<128, 1, 3>(p, s) : launch_attention<128, 2, 3>(p, s);
-  return launch_attention<256, 1, 2>(p, s);
+  if (d == 64) return rows == 8 ? launch_attention<64, 1, 4, 3>(p, s) : launch_attention<64, 2, 4, 2>(p, s);
+  if (d == 128) return rows == 8 ? launch_attention<128, 1, 3, 3>(p, s) : launch_attention<128, 2, 3, 2>(p, s);
+  return launch_attention<256, 1, 2, 2>(p, s);
 }
 
 }  // extern "C"

@@ -133,6 +133,7 @@ def test_cache_refusals(name):
     _refuses(f, a, "gate must", gate=4096, gate_dtype=L.DTYPE_F32)
     _refuses(f, a, "gate row pitch", gate=4096, gate_ld=1000, gate_head_stride=128)
     _refuses(f, a, "ctx_scale", ctx_scale=0.0)
+    _refuses(f, a, "q_scale", q_scale=-1.0)
     _refuses(f, a, "e4m3 output", ctx_scale=0.5)
     _refuses(f, a, "misaligned lse", lse=4097)
     if not torch.cuda.is_available():
