@@ -46,10 +46,11 @@
 namespace b2f {
 namespace {
 
-constexpr int kWarps = 4;
-constexpr int kThreads = 32 * kWarps;
+constexpr int kWarps = 4;                 // that work on keys; one more fetches them
+constexpr int kWork = 32 * kWarps;
+constexpr int kThreads = kWork + 32;
 constexpr int kChunk = 32;                // keys of a warp's step
-constexpr int kUnit = kChunk * kWarps;    // keys of a unit of work
+constexpr int kUnit = kChunk * kWarps;    // keys of a unit of work, and of a stage of the ring
 constexpr float kLift = 7.0f;             // P is scaled by 2^7 ...
 constexpr float kSlack = 8.0f;            // ... and the maximum may lag behind by 2^8
 
@@ -63,6 +64,7 @@ struct Kv4AttnParams {
   Kv4Cache c;
   Kv4Batch b;
   int heads, group, causal;
+  unsigned long long group_inv;  // 2^40 / group, rounded up
   const char* q;
   int q_dtype;
   long long q_ld;
@@ -83,6 +85,11 @@ struct Kv4AttnParams {
 };
 
 // One (sequence, kv head, row tile): its keys and rows.
+__device__ __forceinline__ int by_group(int row, unsigned long long group_inv) {
+  // exact for row * group < 2^40 (row < 2^30, group <= 2^10)
+  return (int)(row * group_inv >> 40);
+}
+
 struct Item {
   Kv4Seq s;
   int b, h, rt, rts;  // row tiles of the sequence
@@ -91,9 +98,9 @@ struct Item {
 };
 
 template <int R>
-__device__ __forceinline__ int tile_keys(const Kv4Seq& s, int rt, int group, int causal) {
-  if (!causal) return s.len;
-  const int last = (min((rt + 1) * R, s.n * group) - 1) / group;  // last token of the tile
+__device__ __forceinline__ int tile_keys(const Kv4AttnParams& p, const Kv4Seq& s, int rt) {
+  if (!p.causal) return s.len;
+  const int last = by_group(min((rt + 1) * R, s.n * p.group) - 1, p.group_inv);  // last token of the tile
   return max(s.len - s.n + last + 1, 0);
 }
 
@@ -101,11 +108,11 @@ __device__ __forceinline__ int units_of(int keys) { return (keys + kUnit - 1) / 
 
 // Units of one kv head of a sequence.
 template <int R>
-__device__ __forceinline__ long long seq_units(const Kv4Seq& s, int group, int causal) {
-  const int rts = (s.n * group + R - 1) / R;
-  if (!causal || rts <= 1) return rts == 0 ? 0 : (long long)rts * units_of(tile_keys<R>(s, 0, group, causal));
+__device__ __forceinline__ long long seq_units(const Kv4AttnParams& p, const Kv4Seq& s) {
+  const int rts = (s.n * p.group + R - 1) / R;
+  if (!p.causal || rts <= 1) return rts == 0 ? 0 : (long long)rts * units_of(tile_keys<R>(p, s, 0));
   long long u = 0;
-  for (int rt = 0; rt < rts; ++rt) u += units_of(tile_keys<R>(s, rt, group, causal));
+  for (int rt = 0; rt < rts; ++rt) u += units_of(tile_keys<R>(p, s, rt));
   return u;
 }
 
@@ -129,7 +136,7 @@ struct Runs {
 };
 
 struct Scan {
-  long long warp_sum[kWarps];
+  long long warp_sum[kThreads / 32];
   long long at;  // units before the sequence that was looked for
   int b;
 };
@@ -149,7 +156,7 @@ __device__ __forceinline__ long long scan_round(long long mine, long long& befor
   __syncthreads();
   long long lead = before;
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
+  for (int w = 0; w < kThreads / 32; ++w) {
     if (w < warp) lead += sc.warp_sum[w];
     before += sc.warp_sum[w];
   }
@@ -167,8 +174,8 @@ __device__ __forceinline__ Runs find_run(const Kv4AttnParams& p, Scan& sc, long 
     mine = 0;
     if (b < p.b.seqs) {
       const Kv4Seq s = kv4_seq(p.c, p.b, b);
-      mine = seq_units<R>(s, p.group, p.causal) * p.c.kv_heads;
-      empty |= b % gridDim.x == blockIdx.x && s.n > 0 && tile_keys<R>(s, 0, p.group, p.causal) <= 0;
+      mine = seq_units<R>(p, s) * p.c.kv_heads;
+      empty |= b % gridDim.x == blockIdx.x && s.n > 0 && tile_keys<R>(p, s, 0) <= 0;
     }
     start = scan_round(mine, before, sc);
   }
@@ -184,7 +191,7 @@ __device__ __forceinline__ Runs find_run(const Kv4AttnParams& p, Scan& sc, long 
     before = 0;
     for (int base = 0; base < p.b.seqs; base += kThreads) {
       const int b = base + (int)threadIdx.x;
-      mine = b < p.b.seqs ? seq_units<R>(kv4_seq(p.c, p.b, b), p.group, p.causal) * p.c.kv_heads : 0;
+      mine = b < p.b.seqs ? seq_units<R>(p, kv4_seq(p.c, p.b, b)) * p.c.kv_heads : 0;
       start = scan_round(mine, before, sc);
       if (u0 >= start && u0 < start + mine) {
         sc.b = b;
@@ -198,7 +205,7 @@ __device__ __forceinline__ Runs find_run(const Kv4AttnParams& p, Scan& sc, long 
 
 template <int R>
 __device__ __forceinline__ void open_item(const Kv4AttnParams& p, Item& it) {
-  it.keys = tile_keys<R>(it.s, it.rt, p.group, p.causal);
+  it.keys = tile_keys<R>(p, it.s, it.rt);
   it.units = units_of(it.keys);
 }
 
@@ -208,7 +215,7 @@ __device__ int find_item(const Kv4AttnParams& p, int b, long long unit, Item& it
   it.b = b;
   it.s = kv4_seq(p.c, p.b, b);
   it.rts = (it.s.n * p.group + R - 1) / R;
-  const long long per = seq_units<R>(it.s, p.group, p.causal);
+  const long long per = seq_units<R>(p, it.s);
   it.h = (int)divide(unit, per);
   long long rest = unit - it.h * per;
   for (it.rt = 0;; ++it.rt) {
@@ -305,7 +312,7 @@ __device__ __forceinline__ void store1(char* base, int dt, long long off, float 
 
 // Where row r of an item's tile goes: token t and query head, or t = -1.
 __device__ __forceinline__ int row_token(const Kv4AttnParams& p, const Item& it, int row, int& head) {
-  const int i = row / p.group;
+  const int i = by_group(row, p.group_inv);
   head = it.h * p.group + (row - i * p.group);
   return i < it.s.n ? it.s.start + i : -1;
 }
@@ -352,10 +359,10 @@ __device__ __forceinline__ void finish_lse(const Kv4AttnParams& p, int t, int he
 template <int D, int NT, int STAGES>
 struct Layout {
   static constexpr int R = 8 * NT;
-  static constexpr int kCodes = kChunk * D / 2, kScales = kChunk * D / 16;
+  static constexpr int kCodes = kUnit * D / 2, kScales = kUnit * D / 16;
   static constexpr int kStage = 2 * (kCodes + kScales);  // K codes, K scales, V codes, V scales
   static constexpr int kPad = 4;                         // floats between rows of the join
-  static constexpr int kRing = kWarps * STAGES * kStage;
+  static constexpr int kRing = STAGES * kStage;
   static constexpr int kJoin = kWarps * R * (D + kPad) * 4;
   static constexpr int kBytes = kRing + kJoin;
 };
@@ -365,21 +372,26 @@ __global__ void __launch_bounds__(kThreads, CTAS) kv4_attention_kernel(const Kv4
   using L = Layout<D, NT, STAGES>;
   constexpr int R = L::R;
   constexpr int kSteps = D / 16;         // k16 steps of Q.K; m16 tiles of O^T
-  constexpr int kWordsK = D / 32;        // 32-bit words of K codes (16 queries' worth) of a thread
+  constexpr int KU = 1, VU = 1;          // loops left as loops: the instruction cache is a limit here
   constexpr int kWordsV = D / 64;        // words of V codes of a thread and key
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ Scan sc;
-  __shared__ __align__(8) uint64_t bars[kWarps][STAGES];
-  __shared__ int stage_ok[kWarps][STAGES];
+  __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES];
+  __shared__ unsigned stage_ok[STAGES];  // bit 4 i: page i of the unit is there
+  __shared__ int aborted;                // a wait ran out: no more work, no more copies
   __shared__ float join_ms[kWarps][R][2];
+  __shared__ uint4 q_frag[NT * D / 32][32];  // B operands of two steps of a lane
+  __shared__ float q_drop[R];
 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int r = lane >> 2, c = lane & 3;
-  uint8_t* ring = smem + warp * STAGES * L::kStage;
   float* join = reinterpret_cast<float*>(smem + L::kRing);
-
-  if (lane == 0) {
-    for (int s = 0; s < STAGES; ++s) mbar_init(&bars[warp][s], 1);
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], kWarps);
+    }
+    aborted = 0;
     fence_mbarrier_init();
   }
   pdl_wait();
@@ -395,7 +407,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) kv4_attention_kernel(const Kv4
     it.b = b;
     it.rts = (it.s.n * p.group + R - 1) / R;
     for (it.rt = 0; it.rt < it.rts; ++it.rt) {
-      if (tile_keys<R>(it.s, it.rt, p.group, p.causal) > 0) break;  // later tiles see more
+      if (tile_keys<R>(p, it.s, it.rt) > 0) break;  // later tiles see more
       for (int x = threadIdx.x; x < p.c.kv_heads * R * (D / 4); x += kThreads) {
         it.h = x / (R * (D / 4));
         const int y = x - it.h * (R * (D / 4));
@@ -414,93 +426,86 @@ __global__ void __launch_bounds__(kThreads, CTAS) kv4_attention_kernel(const Kv4
   Item it;                    // the item that is worked on, from unit `first` on
   int first = find_item<R>(p, sc.b, u0 - sc.at, it);
   long long left = u1 - u0;   // units from there to the end of the CTA's run
-  Item ahead = it;            // the item whose pages are fetched
-  long long ahead_left = left;
-
-  // ---- the fetching side: a lane of 4 * (page of the chunk) + part of the block copies its part
-  const int log2p = p.c.page_log2;
-  const int pages_per_chunk = log2p == 4 ? 2 : 1;
-  const int part = lane & 3, sub = lane >> 2;
-  const bool copies = lane < 4 * pages_per_chunk;
-  const int row_bytes = part & 1 ? D / 16 : D / 2;
-  const uint32_t copy_bytes = (log2p == 4 ? 16 : 32) * row_bytes;
-  const uint32_t page_bytes = (log2p == 4 ? 16 : 32) * (D / 8 * 9);  // all parts of a page's share
-  const int from_part = (part >> 1) * (p.c.codes_bytes + p.c.scales_bytes) + (part & 1 ? p.c.codes_bytes : 0);
-  uint8_t* const to_part = ring + (part >> 1) * (L::kCodes + L::kScales) + (part & 1 ? L::kCodes : 0) + sub * 16 * row_bytes;
-  const uint64_t policy = policy_evict_normal();
-  bool alive = true;       // false once a copy did not arrive in time: no more work, no more copies
-  int ahead_key, ahead_end;            // this warp's next chunk of the item, and where its keys end
-  const uint8_t* ahead_block;
-  const int* ahead_pages;
-  int next_page = -2;                  // page of the lane's next copy; -2: none
-  int fetch_stage = 0, in_ring = 0;    // chunks whose copies were started and not yet worked on
-  auto open_ahead = [&](int unit) {
-    const int take = (int)min((long long)(ahead.units - unit), ahead_left);
-    ahead_left -= take;
-    ahead_key = unit * kUnit + warp * kChunk;
-    ahead_end = min((unit + take) * kUnit, ahead.keys);
-    ahead_block = p.c.storage + (long long)ahead.h * p.c.block_bytes + from_part;
-    ahead_pages = p.c.table + (long long)ahead.s.row * p.c.table_ld;
-  };
-  auto find_page = [&]() {  // of the next chunk; moves on to the next item with a chunk for this warp
-    while (ahead_key >= ahead_end && ahead_left > 0) {
-      next_item<R>(p, ahead);
-      open_ahead(0);
-    }
-    next_page = -2;
-    if (copies && ahead_key + sub * 16 < ahead_end) {
-      next_page = ahead_pages[(ahead_key + sub * 16) >> log2p];
-      if ((unsigned)next_page >= (unsigned)p.c.pages) {
-        record_error(kDevBadArgs);
-        next_page = -2;
-      }
-    }
-  };
-  auto fetch = [&]() {
-    if (ahead_key >= ahead_end || !alive) return;
-    const unsigned good = __ballot_sync(0xffffffffu, next_page >= 0) & 0x11;
-    if (lane == 0) {
-      stage_ok[warp][fetch_stage] = (good & 1) | good >> 3;
-      mbar_arrive_expect_tx(&bars[warp][fetch_stage], page_bytes * __popc(good));
-    }
-    __syncwarp();
-    if (next_page >= 0)
-      bulk_load(to_part + fetch_stage * L::kStage,
-                ahead_block + next_page * p.c.page_stride + (ahead_key & (p.c.page_size - 1)) * row_bytes,
-                copy_bytes, &bars[warp][fetch_stage], policy);
-    fetch_stage = fetch_stage + 1 == STAGES ? 0 : fetch_stage + 1;
-    ++in_ring;
-    ahead_key += kUnit;
-    find_page();
-  };
-  open_ahead(first);
-  find_page();
-  for (int s = 0; s < STAGES; ++s) fetch();
-
   int stage = 0;
   uint32_t phase = 0;
+  const int log2p = p.c.page_log2;
+
+  if (warp == kWarps) {
+    // ---- the fetching warp: lane 4 * (page of the unit) + part copies that part of the page
+    const int part = lane & 3, sub = lane >> 2;
+    const bool copies = sub < (kUnit >> log2p);
+    const int row_bytes = part & 1 ? D / 16 : D / 2;
+    const int from_part = (part >> 1) * (p.c.codes_bytes + p.c.scales_bytes) + (part & 1 ? p.c.codes_bytes : 0);
+    uint8_t* const to = smem + (part >> 1) * (L::kCodes + L::kScales) + (part & 1 ? L::kCodes : 0) +
+                        (sub << log2p) * row_bytes;
+    const uint64_t policy = policy_evict_normal();
+    int fetched = 0;
+    while (left > 0) {
+      const int take = (int)min((long long)(it.units - first), left);
+      const uint8_t* const block = p.c.storage + (long long)it.h * p.c.block_bytes + from_part;
+      const int* const pages = p.c.table + (long long)it.s.row * p.c.table_ld;
+      auto page_at = [&](int unit) {
+        const int key = unit * kUnit + (sub << log2p);
+        return copies && unit < first + take && key < it.keys ? pages[key >> log2p] : -1;
+      };
+      int page = page_at(first);
+      for (int u = first; u < first + take; ++u) {
+        const int next = page_at(u + 1);
+        if (fetched >= STAGES) {
+          if (!__all_sync(0xffffffffu, mbar_wait(&empty[stage], phase ^ 1, kDevTimeoutProducer, &aborted))) {
+            left = 0;
+            break;
+          }
+        }
+        if (copies && u * kUnit + (sub << log2p) < it.keys && (unsigned)page >= (unsigned)p.c.pages)
+          record_error(kDevBadArgs);
+        const bool ok = (unsigned)page < (unsigned)p.c.pages;
+        const unsigned good = __ballot_sync(0xffffffffu, ok) & 0x11111111u;
+        if (lane == 0) {
+          stage_ok[stage] = good;
+          mbar_arrive_expect_tx(&full[stage], (uint32_t)__popc(good) * (uint32_t)p.c.block_bytes);
+        }
+        __syncwarp();
+        if (ok)
+          bulk_load(to + stage * L::kStage, block + page * p.c.page_stride, (uint32_t)(row_bytes << log2p),
+                    &full[stage], policy);
+        page = next;
+        ++fetched;
+        if (++stage == STAGES) {
+          stage = 0;
+          phase ^= 1;
+        }
+      }
+      if (left > 0) left -= take;
+      if (left > 0) {
+        next_item<R>(p, it);
+        first = 0;
+      }
+    }
+    if (aborted) {  // no copy is left in flight when the CTA ends
+      for (int s = 0; s < min(fetched, STAGES); ++s) {
+        stage = stage == 0 ? STAGES - 1 : stage - 1;
+        if (stage == STAGES - 1) phase ^= 1;
+        mbar_wait(&full[stage], phase, kDevTimeoutDrain, nullptr);
+      }
+    }
+    return;
+  }
+
   while (left > 0) {
     const int take = (int)min((long long)(it.units - first), left);  // units [first, first + take) of the item
-    const int end = min((first + take) * kUnit, it.keys);
-    // ---- the queries of the tile, and what a score is multiplied by
-    uint32_t qf[NT][kSteps][2];
-    float mul[NT][2];
-    int limit[NT][2];  // keys that the column sees
-    int lowest = 0x7fffffff;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
+    // ---- the queries of the tile as operands, in shared memory; what a score is multiplied by
+    if (warp < NT) {
       int head;
-      const int t = row_token(p, it, it.rt * R + nt * 8 + r, head);
-      float top = 0.f;
-      float x[2 * kWordsK][4];
-      const long long at = (long long)t * p.q_ld + (long long)head * D;
+      const int t = row_token(p, it, it.rt * R + warp * 8 + r, head);
+      const long long at = (long long)t * p.q_ld + (long long)head * D + c * 16;
+      float top = 0.f, x[D / 64][16];
 #pragma unroll
-      for (int half = 0; half < (D == 256 ? 2 : 1); ++half) {
-        constexpr int kPer = D == 256 ? 8 : 2 * kWordsK;  // fours of a run
+      for (int i = 0; i < D / 64; ++i) {
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-          float* y = x[half * kPer + i];
-          const long long e = at + half * 128 + c * (kPer * 4) + i * 4;
+        for (int k = 0; k < 16; k += 4) {
+          float* y = x[i] + k;
+          const long long e = at + i * 64 + k;
           if (t < 0) {
             y[0] = y[1] = y[2] = y[3] = 0.f;
           } else if (p.q_dtype == kBF16) {
@@ -520,19 +525,28 @@ __global__ void __launch_bounds__(kThreads, CTAS) kv4_attention_kernel(const Kv4
       const int ex = (__float_as_int(top) >> 23) & 0xff;
       const int up = ex == 0 || ex == 255 ? 0 : min(max(127 + 14 - ex, -120), 120);
       const float lift = __int_as_float((127 + up) << 23), drop = __int_as_float((127 - up) << 23);
+      if (c == 0) q_drop[warp * 8 + r] = drop;
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s) {
-        qf[nt][s][0] = pack_f16x2(x[s][0] * lift, x[s][1] * lift);
-        qf[nt][s][1] = pack_f16x2(x[s][2] * lift, x[s][3] * lift);
-      }
+      for (int i = 0; i < D / 64; ++i)
+#pragma unroll
+        for (int k = 0; k < 16; k += 8)
+          q_frag[(warp * (D / 64) + i) * 2 + k / 8][lane] =
+              make_uint4(pack_f16x2(x[i][k] * lift, x[i][k + 1] * lift), pack_f16x2(x[i][k + 2] * lift, x[i][k + 3] * lift),
+                         pack_f16x2(x[i][k + 4] * lift, x[i][k + 5] * lift), pack_f16x2(x[i][k + 6] * lift, x[i][k + 7] * lift));
+    }
+    named_bar_sync(1, kWork);
+    float mul[NT][2];
+    int limit[NT][2];  // keys that the column sees
+    int lowest = 0x7fffffff;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        mul[nt][j] = __shfl_sync(0xffffffffu, drop, (2 * c + j) * 4) * p.scale_log2;
+        mul[nt][j] = q_drop[nt * 8 + 2 * c + j] * p.scale_log2;
         const int row = it.rt * R + nt * 8 + 2 * c + j;
-        limit[nt][j] = p.causal ? min(it.s.len - it.s.n + row / p.group + 1, it.keys) : it.keys;
+        limit[nt][j] = p.causal ? min(it.s.len - it.s.n + by_group(row, p.group_inv) + 1, it.keys) : it.keys;
         if (row < it.s.n * p.group) lowest = min(lowest, limit[nt][j]);
       }
-    }
     lowest = __reduce_min_sync(0xffffffffu, lowest);
 
     // P = 2^(score - base); base is 7 below the largest score seen when it was last moved
@@ -550,22 +564,17 @@ __global__ void __launch_bounds__(kThreads, CTAS) kv4_attention_kernel(const Kv4
         for (int j = 0; j < 4; ++j) o[s][nt][j] = 0.f;
     }
 
-    for (int key0 = first * kUnit + warp * kChunk; key0 < end; key0 += kUnit) {
-      if (in_ring > 0 &&
-          !__all_sync(0xffffffffu, mbar_wait(&bars[warp][stage], phase, kDevTimeoutMma, nullptr)))
-        alive = false;
-      --in_ring;
-      const uint8_t* kc = ring + stage * L::kStage;
-      const uint8_t* ks = kc + L::kCodes;
-      const uint8_t* vc = ks + L::kScales;
-      const uint8_t* vs = vc + L::kCodes;
-      const int okay = stage_ok[warp][stage];
-      const bool edge = key0 + kChunk > lowest || okay != (1 << pages_per_chunk) - 1;
-      if (++stage == STAGES) {
-        stage = 0;
-        phase ^= 1;
-      }
-      if (alive) {
+    for (int u = first; u < first + take; ++u) {
+      const int key0 = u * kUnit + warp * kChunk;
+      const bool alive = __all_sync(0xffffffffu, mbar_wait(&full[stage], phase, kDevTimeoutMma, &aborted));
+      if (alive && key0 < it.keys) {
+        const uint8_t* kc = smem + stage * L::kStage + warp * kChunk * (D / 2);
+        const uint8_t* ks = smem + stage * L::kStage + L::kCodes + warp * kChunk * (D / 16);
+        const uint8_t* vc = kc + L::kCodes + L::kScales;
+        const uint8_t* vs = ks + L::kCodes + L::kScales;
+        // bit 0 (1): the page of the first (second) 16 keys is there
+        const unsigned okay = log2p == 4 ? stage_ok[stage] >> (8 * warp) : (stage_ok[stage] >> (4 * ((warp * kChunk) >> log2p)) & 1) * 0x11;
+        const bool edge = key0 + kChunk > lowest || (okay & 0x11) != 0x11;
         // ---- S^T: two times 16 keys x R rows, each in two chains of sums
         float s[2][NT][4], s2[2][NT][4];
 #pragma unroll
@@ -575,43 +584,39 @@ __global__ void __launch_bounds__(kThreads, CTAS) kv4_attention_kernel(const Kv4
 #pragma unroll
             for (int j = 0; j < 4; ++j) s[g][nt][j] = s2[g][nt][j] = 0.f;
         const int kr = (r >> 1) + (r & 1) * 4;  // key of slot r (of the first 16); slot r + 8: kr + 8
+#pragma unroll KU
+        for (int i = 0; i < D / 64; ++i) {  // a group of 16 elements for each c: four steps
+          uint4 q[NT][2];
 #pragma unroll
-        for (int half = 0; half < (D == 256 ? 2 : 1); ++half) {
-          constexpr int kW = D == 64 ? 2 : 4;  // words of a run of codes
-          uint32_t w[4][kW], m[4];             // codes of the keys kr + 8 i, scales of two groups as f16
+          for (int nt = 0; nt < NT; ++nt) {
+            q[nt][0] = q_frag[(nt * (D / 64) + i) * 2][lane];
+            q[nt][1] = q_frag[(nt * (D / 64) + i) * 2 + 1][lane];
+          }
+          uint2 w[4];  // codes of the keys kr + 8 k, and their scales
+          uint32_t m[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int key = kr + 8 * i;
-            if (D == 64) {
-              const uint2 a = *reinterpret_cast<const uint2*>(kc + key * 32 + c * 8);
-              w[i][0] = a.x; w[i][1] = a.y;
-              m[i] = e4m3x2_to_f16x2(ks[key * 4 + c]);
-            } else {
-              const uint4 a = *reinterpret_cast<const uint4*>(kc + key * (D / 2) + half * 64 + c * 16);
-              w[i][0] = a.x; w[i][1] = a.y; w[i][kW - 2] = a.z; w[i][kW - 1] = a.w;
-              m[i] = e4m3x2_to_f16x2(*reinterpret_cast<const uint16_t*>(ks + key * (D / 16) + 8 * half + 2 * c));
-            }
+          for (int k = 0; k < 4; ++k) {
+            w[k] = *reinterpret_cast<const uint2*>(kc + (kr + 8 * k) * (D / 2) + i * 32 + c * 8);
+            m[k] = e4m3x2_to_f16x2(ks[(kr + 8 * k) * (D / 16) + i * 4 + c]);
           }
 #pragma unroll
-          for (int x = 0; x < kW; ++x) {  // a word is two steps; two words share a scale
-            const int st = 2 * (half * kW + x);
+          for (int g = 0; g < 2; ++g)
 #pragma unroll
-            for (int g = 0; g < 2; ++g) {
+            for (int k = 0; k < 2; ++k) {
               uint32_t f0[4], f1[4];
-              e2m1x8_to_f16x2(w[2 * g][x], f0);
-              e2m1x8_to_f16x2(w[2 * g + 1][x], f1);
+              e2m1x8_to_f16x2(k ? w[2 * g].y : w[2 * g].x, f0);
+              e2m1x8_to_f16x2(k ? w[2 * g + 1].y : w[2 * g + 1].x, f1);
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                f0[i] = hmul2_by(f0[i], m[2 * g], D == 64 ? 0 : x / 2);
-                f1[i] = hmul2_by(f1[i], m[2 * g + 1], D == 64 ? 0 : x / 2);
+              for (int j = 0; j < 4; ++j) {
+                f0[j] = hmul2_by(f0[j], m[2 * g], 0);
+                f1[j] = hmul2_by(f1[j], m[2 * g + 1], 0);
               }
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) {
-                mma16816(s[g][nt], f0[0], f1[0], f0[1], f1[1], qf[nt][st][0], qf[nt][st][1]);
-                mma16816(s2[g][nt], f0[2], f1[2], f0[3], f1[3], qf[nt][st + 1][0], qf[nt][st + 1][1]);
+                mma16816(s[g][nt], f0[0], f1[0], f0[1], f1[1], q[nt][k].x, q[nt][k].y);
+                mma16816(s2[g][nt], f0[2], f1[2], f0[3], f1[3], q[nt][k].z, q[nt][k].w);
               }
             }
-          }
         }
         // ---- scores to P
         float x[2][NT][4];
@@ -625,7 +630,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) kv4_attention_kernel(const Kv4
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
                 const int key = key0 + g * 16 + kr + (j >> 1) * 8;
-                if (key >= limit[nt][j & 1] || !(okay >> (pages_per_chunk == 2 ? g : 0) & 1)) {
+                if (key >= limit[nt][j & 1] || !(okay >> (4 * g) & 1)) {
                   hidden |= 1u << ((g * NT + nt) * 4 + j);
                   s[g][nt][j] = -INFINITY;
                 }
@@ -704,13 +709,22 @@ __global__ void __launch_bounds__(kThreads, CTAS) kv4_attention_kernel(const Kv4
             }
         }
         // ---- O^T += V^T P^T
+        uint32_t pf[NT][2], pf2[NT][2];
 #pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            pf[nt][k] = transpose8x8(pack_f16x2(x[0][nt][2 * k], x[0][nt][2 * k + 1]));
+            pf2[nt][k] = transpose8x8(pack_f16x2(x[1][nt][2 * k], x[1][nt][2 * k + 1]));
+          }
+#pragma unroll VU
         for (int g = 0; g < 2; ++g) {
-          uint32_t pf[NT][2];
+          if (g) {
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            pf[nt][0] = transpose8x8(pack_f16x2(x[g][nt][0], x[g][nt][1]));
-            pf[nt][1] = transpose8x8(pack_f16x2(x[g][nt][2], x[g][nt][3]));
+            for (int nt = 0; nt < NT; ++nt) {
+              pf[nt][0] = pf2[nt][0];
+              pf[nt][1] = pf2[nt][1];
+            }
           }
           // codes and scales of keys c, c + 4, c + 8, c + 12 of the 16
           const uint8_t* vk = vc + (g * 16 + c) * (D / 2) + r * (D / 16);
@@ -771,7 +785,11 @@ __global__ void __launch_bounds__(kThreads, CTAS) kv4_attention_kernel(const Kv4
         }
       }
       __syncwarp();  // the stage has been read by all lanes
-      fetch();
+      if (lane == 0) mbar_arrive(&empty[stage]);
+      if (++stage == STAGES) {
+        stage = 0;
+        phase ^= 1;
+      }
     }
 
     // ---- the piece is done: join the warps
@@ -794,7 +812,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) kv4_attention_kernel(const Kv4
           *reinterpret_cast<float4*>(to + 2 * t) =
               make_float4(o[t][nt][j], o[t][nt][j + 2], o[t + 1][nt][j], o[t + 1][nt][j + 2]);
       }
-    __syncthreads();
+    named_bar_sync(1, kWork);
     const bool from_start = first == 0, to_end = first + take == it.units;
     if (from_start && !to_end && threadIdx.x == 0) {
       const int last = runs.of(u1 - left + it.units - 1);  // the CTA with the item's last unit
@@ -803,7 +821,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) kv4_attention_kernel(const Kv4
     const int slot = 2 * blockIdx.x + (from_start ? 1 : 0);
     float* part_o = p.partial + (long long)slot * R * D;
     float* part_ms = p.partial + 2ll * p.ctas * R * D + (long long)slot * R * 2;
-    for (int x = threadIdx.x; x < R * (D / 4); x += kThreads) {
+    for (int x = threadIdx.x; x < R * (D / 4); x += kWork) {
       const int row = x / (D / 4), d0 = (x % (D / 4)) * 4;
       float m = -INFINITY;
 #pragma unroll
@@ -832,7 +850,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) kv4_attention_kernel(const Kv4
         }
       }
     }
-    __syncthreads();
+    named_bar_sync(1, kWork);
     left -= take;
     if (left > 0) {
       next_item<R>(p, it);
@@ -844,7 +862,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) kv4_attention_kernel(const Kv4
 // Joins the pieces of the item that begins in the run of CTA blockIdx.x and goes on in the
 // next ones.  A CTA for each row; each warp takes every fourth piece.
 template <int D, int NT>
-__global__ void __launch_bounds__(kThreads) kv4_attention_join_kernel(const Kv4AttnParams p) {
+__global__ void __launch_bounds__(kWork) kv4_attention_join_kernel(const Kv4AttnParams p) {
   constexpr int R = 8 * NT;
   constexpr int kPer = D / 32;  // elements of a lane
   __shared__ float acc_s[kWarps][D], ms[kWarps][2];
@@ -853,7 +871,7 @@ __global__ void __launch_bounds__(kThreads) kv4_attention_join_kernel(const Kv4A
   const int me = blockIdx.x, row = blockIdx.y;
   const Shared it = p.shared[me];
   if (it.more == 0) return;
-  const int i = (it.row0 + row) / p.group;
+  const int i = by_group(it.row0 + row, p.group_inv);
   if (i >= it.n) return;
   const int t = it.start + i, head = it.head0 + (it.row0 + row) - i * p.group;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -898,7 +916,7 @@ __global__ void __launch_bounds__(kThreads) kv4_attention_join_kernel(const Kv4A
     f[w] = ms[w][0] == top ? 1.f : ex2(ms[w][0] - top);
     l += ms[w][1] * f[w];
   }
-  for (int d = threadIdx.x; d < D; d += kThreads) {
+  for (int d = threadIdx.x; d < D; d += kWork) {
     float x[1] = {0.f};
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) x[0] += acc_s[w][d] * f[w];
@@ -914,13 +932,13 @@ int tile_rows(int head_dim, long long rows) { return head_dim == 256 || rows <= 
 template <int D, int NT, int STAGES, int CTAS>
 int launch_attention(Kv4AttnParams& p, cudaStream_t s) {
   using L = Layout<D, NT, STAGES>;
-  static_assert(CTAS <= kMaxPerSm && CTAS * (L::kBytes + 2048) <= 227 * 1024, "CTAS CTAs fit on an SM");
+  static_assert(CTAS <= kMaxPerSm && CTAS * (L::kBytes + NT * D * 16 + 2048) <= 227 * 1024, "CTAS CTAs fit on an SM");
   p.ctas = sm_count() * CTAS;
   p.shared = reinterpret_cast<Shared*>(p.partial + 2ll * p.ctas * L::R * (D + 2));
   B2F_CUDA_TRY(cudaFuncSetAttribute(kv4_attention_kernel<D, NT, STAGES, CTAS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                     L::kBytes));
   B2F_CUDA_TRY(launch_pdl(kv4_attention_kernel<D, NT, STAGES, CTAS>, dim3((unsigned)p.ctas), dim3(kThreads), L::kBytes, s, p));
-  B2F_CUDA_TRY(launch_pdl(kv4_attention_join_kernel<D, NT>, dim3((unsigned)p.ctas, 8 * NT), dim3(kThreads), 0, s, p));
+  B2F_CUDA_TRY(launch_pdl(kv4_attention_join_kernel<D, NT>, dim3((unsigned)p.ctas, 8 * NT), dim3(kWork), 0, s, p));
   return B2F_OK;
 }
 
@@ -957,7 +975,7 @@ int b2f_kv4_attention(const b2f_kv4_attn_args* a, b2f_stream_t stream) {
   const int d = a->cache.head_dim, hk = a->cache.kv_heads;
   if (a->heads <= 0 || a->heads % hk) return fail(B2F_ERR_ARG, "kv4_attention: heads must be a multiple of kv_heads");
   if (a->heads / hk > 1024) return fail(B2F_ERR_ARG, "kv4_attention: more than 1024 query heads a kv head");
-  if ((long long)a->batch.tokens * a->heads > 0x3fffffffll) return fail(B2F_ERR_ARG, "kv4_attention: too many rows");
+  if (a->batch.tokens > (1 << 23) || (long long)a->batch.tokens * a->heads > 0x3fffffffll) return fail(B2F_ERR_ARG, "kv4_attention: too many rows");
   if (a->q == nullptr || a->out == nullptr) return fail(B2F_ERR_ARG, "kv4_attention: null tensor");
   for (int dt : {a->q_dtype, a->out_dtype})
     if (dt != B2F_DTYPE_BF16 && dt != B2F_DTYPE_F16 && dt != B2F_DTYPE_E4M3)
@@ -985,6 +1003,7 @@ int b2f_kv4_attention(const b2f_kv4_attn_args* a, b2f_stream_t stream) {
   if (a->workspace == nullptr || a->workspace_bytes < need || (reinterpret_cast<uintptr_t>(a->workspace) & 15))
     return fail(B2F_ERR_ARG, "kv4_attention: workspace too small or misaligned");
   p.heads = a->heads; p.group = a->heads / hk; p.causal = a->causal != 0;
+  p.group_inv = ((1ull << 40) + p.group - 1) / p.group;
   p.q = reinterpret_cast<const char*>(a->q); p.q_dtype = a->q_dtype; p.q_ld = a->q_ld;
   const float sm = a->sm_scale > 0.f ? a->sm_scale : 1.0f / std::sqrt((float)d);
   p.scale_log2 = sm * a->q_scale * a->cache.k_scale * 1.4426950408889634f;
