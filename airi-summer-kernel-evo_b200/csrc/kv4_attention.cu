@@ -258,6 +258,16 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// The same with zeros for d.
+__device__ __forceinline__ void mma16816_from0(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                               uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%10, %10, %10, %10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+
 __device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
   uint32_t r;
   asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
@@ -269,6 +279,18 @@ __device__ __forceinline__ uint32_t hmul2_by(uint32_t a, uint32_t b, int upper) 
   const __half2 x = *reinterpret_cast<const __half2*>(&a), y = *reinterpret_cast<const __half2*>(&b);
   const __half2 z = __hmul2(x, upper ? __high2half2(y) : __low2half2(y));
   return *reinterpret_cast<const uint32_t*>(&z);
+}
+
+// Barrier of `threads` threads; whether `mine` holds for all of them.
+__device__ __forceinline__ bool named_bar_all(int id, int threads, bool mine) {
+  uint32_t all;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %3, 0;\n\t"
+      "barrier.cta.red.and.pred q, %1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(all)
+      : "r"(id), "r"(threads), "r"((uint32_t)mine)
+      : "memory");
+  return all != 0;
 }
 
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
@@ -310,11 +332,11 @@ __device__ __forceinline__ void store1(char* base, int dt, long long off, float 
   }
 }
 
-// Where row r of an item's tile goes: token t and query head, or t = -1.
-__device__ __forceinline__ int row_token(const Kv4AttnParams& p, const Item& it, int row, int& head) {
+// Where a row (query head x new token, of a kv head h) goes: its token and query head; -1: none.
+__device__ __forceinline__ int row_token(const Kv4AttnParams& p, int row, int h, int start, int n, int& head) {
   const int i = by_group(row, p.group_inv);
-  head = it.h * p.group + (row - i * p.group);
-  return i < it.s.n ? it.s.start + i : -1;
+  head = h * p.group + (row - i * p.group);
+  return i < n ? start + i : -1;
 }
 
 // Normalises, gates and stores `n` neighbouring elements (o, unnormalised) of one row.
@@ -359,29 +381,39 @@ __device__ __forceinline__ void finish_lse(const Kv4AttnParams& p, int t, int he
 template <int D, int NT, int STAGES>
 struct Layout {
   static constexpr int R = 8 * NT;
-  static constexpr int kCodes = kUnit * D / 2, kScales = kUnit * D / 16;
-  static constexpr int kStage = 2 * (kCodes + kScales);  // K codes, K scales, V codes, V scales
-  static constexpr int kPad = 4;                         // floats between rows of the join
+  static constexpr int kStage = kUnit * D / 8 * 9;       // the blocks of a unit's pages, one after the other
+  static constexpr int kRow = 64 + 4;                    // floats of a row of the join: 64 elements at a time
   static constexpr int kRing = STAGES * kStage;
-  static constexpr int kJoin = kWarps * R * (D + kPad) * 4;
+  static constexpr int kJoin = kWarps * R * kRow * 4;
   static constexpr int kBytes = kRing + kJoin;
+};
+
+// What the fetching warp tells the others of the piece of an item that comes next.
+struct Piece {
+  int first, take;     // units [first, first + take) of the item; take 0: no more pieces
+  int keys;            // of the item
+  int start, n, seen;  // first token, tokens, and keys that are older than the first token
+  int h, row0;         // kv head, first row of the tile
+  int whole;           // the piece is the whole item
 };
 
 template <int D, int NT, int STAGES, int CTAS>
 __global__ void __launch_bounds__(kThreads, CTAS) kv4_attention_kernel(const Kv4AttnParams p) {
   using L = Layout<D, NT, STAGES>;
   constexpr int R = L::R;
-  constexpr int kSteps = D / 16;         // k16 steps of Q.K; m16 tiles of O^T
-  constexpr int KU = 1, VU = 1;          // loops left as loops: the instruction cache is a limit here
-  constexpr int kWordsV = D / 64;        // words of V codes of a thread and key
+  constexpr int kTiles = D / 16;            // m16 tiles of O^T
+  constexpr int kRuns = D == 256 ? 2 : 1;   // runs of neighbouring K codes of a thread and key
+  constexpr int kWordsK = D / 32 / kRuns;   // 32-bit words of a run: two steps each
+  constexpr int kWordsV = D / 64;           // words of V codes of a thread and key
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ Scan sc;
-  __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES];
-  __shared__ unsigned stage_ok[STAGES];  // bit 4 i: page i of the unit is there
+  __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES], q_full[2], q_empty[2];
+  __shared__ unsigned stage_ok[STAGES];  // bit i: page i of the unit is there
   __shared__ int aborted;                // a wait ran out: no more work, no more copies
+  __shared__ Piece pieces[2];
+  __shared__ uint4 q_frag[2][NT * D / 32][32];  // B operands of two steps of a lane
+  __shared__ float q_drop[2][R];
   __shared__ float join_ms[kWarps][R][2];
-  __shared__ uint4 q_frag[NT * D / 32][32];  // B operands of two steps of a lane
-  __shared__ float q_drop[R];
 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int r = lane >> 2, c = lane & 3;
@@ -390,6 +422,10 @@ __global__ void __launch_bounds__(kThreads, CTAS) kv4_attention_kernel(const Kv4
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], kWarps);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&q_full[s], 1);
+      mbar_init(&q_empty[s], kWarps);
     }
     aborted = 0;
     fence_mbarrier_init();
@@ -412,7 +448,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) kv4_attention_kernel(const Kv4
         it.h = x / (R * (D / 4));
         const int y = x - it.h * (R * (D / 4));
         int head;
-        const int t = row_token(p, it, it.rt * R + y / (D / 4), head);
+        const int t = row_token(p, it.rt * R + y / (D / 4), it.h, it.s.start, it.s.n, head);
         const float zero[4] = {0.f, 0.f, 0.f, 0.f};
         if (t >= 0) {
           finish_row<4>(p, t, head, (y % (D / 4)) * 4, zero, 0.f);
@@ -423,118 +459,165 @@ __global__ void __launch_bounds__(kThreads, CTAS) kv4_attention_kernel(const Kv4
   }
   if (threadIdx.x == 0) p.shared[blockIdx.x].more = 0;
   if (u0 >= u1) return;
-  Item it;                    // the item that is worked on, from unit `first` on
-  int first = find_item<R>(p, sc.b, u0 - sc.at, it);
-  long long left = u1 - u0;   // units from there to the end of the CTA's run
-  int stage = 0;
-  uint32_t phase = 0;
+
+  int stage = 0, buf = 0;
+  uint32_t phase = 0, q_phase = 0;
   const int log2p = p.c.page_log2;
 
   if (warp == kWarps) {
-    // ---- the fetching warp: lane 4 * (page of the unit) + part copies that part of the page
-    const int part = lane & 3, sub = lane >> 2;
-    const bool copies = sub < (kUnit >> log2p);
-    const int row_bytes = part & 1 ? D / 16 : D / 2;
-    const int from_part = (part >> 1) * (p.c.codes_bytes + p.c.scales_bytes) + (part & 1 ? p.c.codes_bytes : 0);
-    uint8_t* const to = smem + (part >> 1) * (L::kCodes + L::kScales) + (part & 1 ? L::kCodes : 0) +
-                        (sub << log2p) * row_bytes;
+    // ---- the fetching warp: a lane for each page of a unit; the block of a head is one piece
+    Item it;
+    int first = find_item<R>(p, sc.b, u0 - sc.at, it);
+    long long left = u1 - u0;
+    const bool copies = lane < (kUnit >> log2p);
     const uint64_t policy = policy_evict_normal();
-    int fetched = 0;
+    int fetched = 0, told = 0;
+    bool ok = true;
     while (left > 0) {
       const int take = (int)min((long long)(it.units - first), left);
-      const uint8_t* const block = p.c.storage + (long long)it.h * p.c.block_bytes + from_part;
+      const uint8_t* const block = p.c.storage + (long long)it.h * p.c.block_bytes;
       const int* const pages = p.c.table + (long long)it.s.row * p.c.table_ld;
       auto page_at = [&](int unit) {
-        const int key = unit * kUnit + (sub << log2p);
+        const int key = unit * kUnit + (lane << log2p);
         return copies && unit < first + take && key < it.keys ? pages[key >> log2p] : -1;
       };
-      int page = page_at(first);
-      for (int u = first; u < first + take; ++u) {
-        const int next = page_at(u + 1);
-        if (fetched >= STAGES) {
-          if (!__all_sync(0xffffffffu, mbar_wait(&empty[stage], phase ^ 1, kDevTimeoutProducer, &aborted))) {
-            left = 0;
-            break;
-          }
-        }
-        if (copies && u * kUnit + (sub << log2p) < it.keys && (unsigned)page >= (unsigned)p.c.pages)
-          record_error(kDevBadArgs);
-        const bool ok = (unsigned)page < (unsigned)p.c.pages;
-        const unsigned good = __ballot_sync(0xffffffffu, ok) & 0x11111111u;
+      auto fetch = [&](int u, int page) {
+        if (fetched >= STAGES)
+          ok = ok && __all_sync(0xffffffffu, mbar_wait(&empty[stage], phase ^ 1, kDevTimeoutProducer, &aborted));
+        if (!ok) return;
+        const bool there = (unsigned)page < (unsigned)p.c.pages;
+        if (!there && copies && u * kUnit + (lane << log2p) < it.keys) record_error(kDevBadArgs);
+        const unsigned good = __ballot_sync(0xffffffffu, there);
         if (lane == 0) {
           stage_ok[stage] = good;
           mbar_arrive_expect_tx(&full[stage], (uint32_t)__popc(good) * (uint32_t)p.c.block_bytes);
         }
         __syncwarp();
-        if (ok)
-          bulk_load(to + stage * L::kStage, block + page * p.c.page_stride, (uint32_t)(row_bytes << log2p),
-                    &full[stage], policy);
-        page = next;
+        if (there)
+          bulk_load(smem + stage * L::kStage + lane * p.c.block_bytes, block + page * p.c.page_stride,
+                    (uint32_t)p.c.block_bytes, &full[stage], policy);
         ++fetched;
         if (++stage == STAGES) {
           stage = 0;
           phase ^= 1;
         }
+      };
+      int page = page_at(first);
+      // the queries of the tile: thread (r, c) takes the elements of row r in the order of its codes
+      float x[NT][kRuns][4 * kWordsK * 2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        int head;
+        const int t = row_token(p, it.rt * R + nt * 8 + r, it.h, it.s.start, it.s.n, head);
+        const long long at = (long long)t * p.q_ld + (long long)head * D + c * (8 * kWordsK);
+#pragma unroll
+        for (int i = 0; i < kRuns; ++i)
+#pragma unroll
+          for (int k = 0; k < 8 * kWordsK; k += 4) {
+            float* y = x[nt][i] + k;
+            const long long e = at + i * 128 + k;
+            if (t < 0) {
+              y[0] = y[1] = y[2] = y[3] = 0.f;
+            } else if (p.q_dtype == kBF16) {
+              load4<kBF16>(p.q, e, y);
+            } else if (p.q_dtype == kF16) {
+              load4<kF16>(p.q, e, y);
+            } else {
+              load4<kE4M3>(p.q, e, y);
+            }
+          }
       }
-      if (left > 0) left -= take;
+      int next = page_at(first + 1);
+      fetch(first, page);
+      if (told >= 2)
+        ok = ok && __all_sync(0xffffffffu, mbar_wait(&q_empty[buf], q_phase ^ 1, kDevTimeoutProducer, &aborted));
+      if (!ok) break;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float top = 0.f;
+#pragma unroll
+        for (int i = 0; i < kRuns; ++i)
+#pragma unroll
+          for (int k = 0; k < 8 * kWordsK; ++k) top = fmaxf(top, fabsf(x[nt][i][k]));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        // 2^(14 - exponent of top), and its inverse; 1 for a row of zeros or with an infinity
+        const int ex = (__float_as_int(top) >> 23) & 0xff;
+        const int up = ex == 0 || ex == 255 ? 0 : min(max(127 + 14 - ex, -120), 120);
+        const float lift = __int_as_float((127 + up) << 23), drop = __int_as_float((127 - up) << 23);
+        if (c == 0) q_drop[buf][nt * 8 + r] = drop;
+#pragma unroll
+        for (int i = 0; i < kRuns; ++i)
+#pragma unroll
+          for (int k = 0; k < kWordsK; ++k) {
+            const float* y = x[nt][i] + 8 * k;
+            q_frag[buf][(nt * kRuns + i) * kWordsK + k][lane] =
+                make_uint4(pack_f16x2(y[0] * lift, y[1] * lift), pack_f16x2(y[2] * lift, y[3] * lift),
+                           pack_f16x2(y[4] * lift, y[5] * lift), pack_f16x2(y[6] * lift, y[7] * lift));
+          }
+      }
+      if (lane == 0) {
+        const bool to_end = first + take == it.units;
+        pieces[buf] = Piece{first, take, it.keys, it.s.start, it.s.n, it.s.len - it.s.n, it.h, it.rt * R, first == 0 && to_end};
+        if (first == 0 && !to_end) {
+          const int last = runs.of(u1 - left + it.units - 1);  // the CTA with the item's last unit
+          p.shared[blockIdx.x] = Shared{last - (int)blockIdx.x, it.s.start, it.s.n, it.h * p.group, it.rt * R};
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&q_full[buf]);
+      ++told;
+      if (++buf == 2) {
+        buf = 0;
+        q_phase ^= 1;
+      }
+      for (int u = first + 1; u < first + take; ++u) {
+        page = next;
+        next = page_at(u + 1);
+        fetch(u, page);
+      }
+      left -= take;
       if (left > 0) {
         next_item<R>(p, it);
         first = 0;
       }
     }
-    if (aborted) {  // no copy is left in flight when the CTA ends
+    if (ok) {
+      if (told >= 2) mbar_wait(&q_empty[buf], q_phase ^ 1, kDevTimeoutProducer, &aborted);
+      if (lane == 0) {
+        pieces[buf].take = 0;
+        mbar_arrive(&q_full[buf]);
+      }
+    } else {  // no copy is left in flight when the CTA ends
       for (int s = 0; s < min(fetched, STAGES); ++s) {
-        stage = stage == 0 ? STAGES - 1 : stage - 1;
-        if (stage == STAGES - 1) phase ^= 1;
+        if (--stage < 0) {
+          stage = STAGES - 1;
+          phase ^= 1;
+        }
         mbar_wait(&full[stage], phase, kDevTimeoutDrain, nullptr);
       }
     }
     return;
   }
 
-  while (left > 0) {
-    const int take = (int)min((long long)(it.units - first), left);  // units [first, first + take) of the item
-    // ---- the queries of the tile as operands, in shared memory; what a score is multiplied by
-    if (warp < NT) {
-      int head;
-      const int t = row_token(p, it, it.rt * R + warp * 8 + r, head);
-      const long long at = (long long)t * p.q_ld + (long long)head * D + c * 16;
-      float top = 0.f, x[D / 64][16];
-#pragma unroll
-      for (int i = 0; i < D / 64; ++i) {
-#pragma unroll
-        for (int k = 0; k < 16; k += 4) {
-          float* y = x[i] + k;
-          const long long e = at + i * 64 + k;
-          if (t < 0) {
-            y[0] = y[1] = y[2] = y[3] = 0.f;
-          } else if (p.q_dtype == kBF16) {
-            load4<kBF16>(p.q, e, y);
-          } else if (p.q_dtype == kF16) {
-            load4<kF16>(p.q, e, y);
-          } else {
-            load4<kE4M3>(p.q, e, y);
-          }
-#pragma unroll
-          for (int j = 0; j < 4; ++j) top = fmaxf(top, fabsf(y[j]));
-        }
-      }
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      // 2^(14 - exponent of top), and its inverse; 1 for a row of zeros or with an infinity
-      const int ex = (__float_as_int(top) >> 23) & 0xff;
-      const int up = ex == 0 || ex == 255 ? 0 : min(max(127 + 14 - ex, -120), 120);
-      const float lift = __int_as_float((127 + up) << 23), drop = __int_as_float((127 - up) << 23);
-      if (c == 0) q_drop[warp * 8 + r] = drop;
-#pragma unroll
-      for (int i = 0; i < D / 64; ++i)
-#pragma unroll
-        for (int k = 0; k < 16; k += 8)
-          q_frag[(warp * (D / 64) + i) * 2 + k / 8][lane] =
-              make_uint4(pack_f16x2(x[i][k] * lift, x[i][k + 1] * lift), pack_f16x2(x[i][k + 2] * lift, x[i][k + 3] * lift),
-                         pack_f16x2(x[i][k + 4] * lift, x[i][k + 5] * lift), pack_f16x2(x[i][k + 6] * lift, x[i][k + 7] * lift));
-    }
-    named_bar_sync(1, kWork);
+  // Where the warp's codes and scales lie in a stage (of K; those of V are v_part behind), and how
+  // far the second 16 of its 32 keys are from the first; the bits of their pages in stage_ok.
+  const int page0 = (warp * kChunk) >> log2p, slot0 = (warp * kChunk) & (p.c.page_size - 1);
+  const int codes_at = page0 * p.c.block_bytes + slot0 * (D / 2);
+  const int scales_at = page0 * p.c.block_bytes + p.c.codes_bytes + slot0 * (D / 16);
+  const int v_part = p.c.codes_bytes + p.c.scales_bytes;
+  const int codes_2nd = log2p == 4 ? p.c.block_bytes : 16 * (D / 2);
+  const int scales_2nd = log2p == 4 ? p.c.block_bytes : 16 * (D / 16);
+  const int page1 = page0 + (log2p == 4 ? 1 : 0);
+  const unsigned mine = 1u << page0 | 1u << page1;
+
+  for (;;) {
+    // The barrier lets the four warps agree (a warp that gave up must not leave the others at the
+    // next one), and the join of the piece before has been read when it is passed.
+    if (!named_bar_all(1, kWork, mbar_wait(&q_full[buf], q_phase, kDevTimeoutMma, &aborted))) return;
+    bool alive = true;
+    const Piece it = pieces[buf];
+    if (it.take == 0) return;
     float mul[NT][2];
     int limit[NT][2];  // keys that the column sees
     int lowest = 0x7fffffff;
@@ -542,15 +625,15 @@ __global__ void __launch_bounds__(kThreads, CTAS) kv4_attention_kernel(const Kv4
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        mul[nt][j] = q_drop[nt * 8 + 2 * c + j] * p.scale_log2;
-        const int row = it.rt * R + nt * 8 + 2 * c + j;
-        limit[nt][j] = p.causal ? min(it.s.len - it.s.n + by_group(row, p.group_inv) + 1, it.keys) : it.keys;
-        if (row < it.s.n * p.group) lowest = min(lowest, limit[nt][j]);
+        mul[nt][j] = q_drop[buf][nt * 8 + 2 * c + j] * p.scale_log2;
+        const int i = by_group(it.row0 + nt * 8 + 2 * c + j, p.group_inv);
+        limit[nt][j] = p.causal ? min(it.seen + i + 1, it.keys) : it.keys;
+        if (i < it.n) lowest = min(lowest, limit[nt][j]);
       }
     lowest = __reduce_min_sync(0xffffffffu, lowest);
 
     // P = 2^(score - base); base is 7 below the largest score seen when it was last moved
-    float base[NT][2], sum[NT][2], o[kSteps][NT][4];
+    float base[NT][2], sum[NT][2], o[kTiles][NT][4];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -559,68 +642,66 @@ __global__ void __launch_bounds__(kThreads, CTAS) kv4_attention_kernel(const Kv4
         sum[nt][j] = 0.f;
       }
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s)
+      for (int t = 0; t < kTiles; ++t)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) o[s][nt][j] = 0.f;
+        for (int j = 0; j < 4; ++j) o[t][nt][j] = 0.f;
     }
 
-    for (int u = first; u < first + take; ++u) {
+    for (int u = it.first; u < it.first + it.take; ++u) {
       const int key0 = u * kUnit + warp * kChunk;
-      const bool alive = __all_sync(0xffffffffu, mbar_wait(&full[stage], phase, kDevTimeoutMma, &aborted));
+      alive = alive && __all_sync(0xffffffffu, mbar_wait(&full[stage], phase, kDevTimeoutMma, &aborted));
       if (alive && key0 < it.keys) {
-        const uint8_t* kc = smem + stage * L::kStage + warp * kChunk * (D / 2);
-        const uint8_t* ks = smem + stage * L::kStage + L::kCodes + warp * kChunk * (D / 16);
-        const uint8_t* vc = kc + L::kCodes + L::kScales;
-        const uint8_t* vs = ks + L::kCodes + L::kScales;
-        // bit 0 (1): the page of the first (second) 16 keys is there
-        const unsigned okay = log2p == 4 ? stage_ok[stage] >> (8 * warp) : (stage_ok[stage] >> (4 * ((warp * kChunk) >> log2p)) & 1) * 0x11;
-        const bool edge = key0 + kChunk > lowest || (okay & 0x11) != 0x11;
-        // ---- S^T: two times 16 keys x R rows, each in two chains of sums
-        float s[2][NT][4], s2[2][NT][4];
-#pragma unroll
-        for (int g = 0; g < 2; ++g)
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) s[g][nt][j] = s2[g][nt][j] = 0.f;
+        const uint8_t* kc = smem + stage * L::kStage + codes_at;
+        const uint8_t* ks = smem + stage * L::kStage + scales_at;
+        const unsigned okay = stage_ok[stage];
+        const bool edge = key0 + kChunk > lowest || (okay & mine) != mine;
+        // ---- S^T: two times 16 keys x R rows
+        float s[2][NT][4];
         const int kr = (r >> 1) + (r & 1) * 4;  // key of slot r (of the first 16); slot r + 8: kr + 8
-#pragma unroll KU
-        for (int i = 0; i < D / 64; ++i) {  // a group of 16 elements for each c: four steps
-          uint4 q[NT][2];
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            q[nt][0] = q_frag[(nt * (D / 64) + i) * 2][lane];
-            q[nt][1] = q_frag[(nt * (D / 64) + i) * 2 + 1][lane];
-          }
-          uint2 w[4];  // codes of the keys kr + 8 k, and their scales
-          uint32_t m[4];
+        for (int i = 0; i < kRuns; ++i) {
+          uint32_t w[4][kWordsK], m[4];  // codes of the keys kr + 8 k, scales of two groups as f16
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            w[k] = *reinterpret_cast<const uint2*>(kc + (kr + 8 * k) * (D / 2) + i * 32 + c * 8);
-            m[k] = e4m3x2_to_f16x2(ks[(kr + 8 * k) * (D / 16) + i * 4 + c]);
+            const int key = kr + 8 * (k & 1);
+            const uint8_t* codes = kc + (k >= 2 ? codes_2nd : 0);
+            const uint8_t* scales = ks + (k >= 2 ? scales_2nd : 0);
+            if (D == 64) {
+              const uint2 a = *reinterpret_cast<const uint2*>(codes + key * 32 + c * 8);
+              w[k][0] = a.x; w[k][1] = a.y;
+              m[k] = e4m3x2_to_f16x2(scales[key * 4 + c]);
+            } else {
+              const uint4 a = *reinterpret_cast<const uint4*>(codes + key * (D / 2) + i * 64 + c * 16);
+              w[k][0] = a.x; w[k][1] = a.y; w[k][kWordsK - 2] = a.z; w[k][kWordsK - 1] = a.w;
+              m[k] = e4m3x2_to_f16x2(*reinterpret_cast<const uint16_t*>(scales + key * (D / 16) + 8 * i + 2 * c));
+            }
           }
 #pragma unroll
-          for (int g = 0; g < 2; ++g)
+          for (int x = 0; x < kWordsK; ++x) {  // a word is two steps; two words share a scale
+            uint4 q[NT];
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
+            for (int nt = 0; nt < NT; ++nt) q[nt] = q_frag[buf][(nt * kRuns + i) * kWordsK + x][lane];
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
               uint32_t f0[4], f1[4];
-              e2m1x8_to_f16x2(k ? w[2 * g].y : w[2 * g].x, f0);
-              e2m1x8_to_f16x2(k ? w[2 * g + 1].y : w[2 * g + 1].x, f1);
+              e2m1x8_to_f16x2(w[2 * g][x], f0);
+              e2m1x8_to_f16x2(w[2 * g + 1][x], f1);
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
-                f0[j] = hmul2_by(f0[j], m[2 * g], 0);
-                f1[j] = hmul2_by(f1[j], m[2 * g + 1], 0);
+                f0[j] = hmul2_by(f0[j], m[2 * g], x / 2);
+                f1[j] = hmul2_by(f1[j], m[2 * g + 1], x / 2);
               }
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) {
-                mma16816(s[g][nt], f0[0], f1[0], f0[1], f1[1], q[nt][k].x, q[nt][k].y);
-                mma16816(s2[g][nt], f0[2], f1[2], f0[3], f1[3], q[nt][k].z, q[nt][k].w);
+                if (i == 0 && x == 0) mma16816_from0(s[g][nt], f0[0], f1[0], f0[1], f1[1], q[nt].x, q[nt].y);
+                else mma16816(s[g][nt], f0[0], f1[0], f0[1], f1[1], q[nt].x, q[nt].y);
+                mma16816(s[g][nt], f0[2], f1[2], f0[3], f1[3], q[nt].z, q[nt].w);
               }
             }
+          }
         }
         // ---- scores to P
         float x[2][NT][4];
-        float top = -INFINITY;
         unsigned hidden = 0;  // bit (g * NT + nt) * 4 + j: the row does not see the key
         if (edge) {
 #pragma unroll
@@ -630,21 +711,22 @@ __global__ void __launch_bounds__(kThreads, CTAS) kv4_attention_kernel(const Kv4
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
                 const int key = key0 + g * 16 + kr + (j >> 1) * 8;
-                if (key >= limit[nt][j & 1] || !(okay >> (4 * g) & 1)) {
+                if (key >= limit[nt][j & 1] || !(okay >> (g ? page1 : page0) & 1)) {
                   hidden |= 1u << ((g * NT + nt) * 4 + j);
                   s[g][nt][j] = -INFINITY;
                 }
               }
         }
+        float top = -INFINITY;
 #pragma unroll
         for (int g = 0; g < 2; ++g)
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              s[g][nt][j] += s2[g][nt][j];
-              x[g][nt][j] = fmaf(s[g][nt][j], mul[nt][j & 1], -base[nt][j & 1]);
-              top = fmaxf(top, x[g][nt][j]);  // a first score is infinitely far above the base
+            for (int j = 0; j < 4; j += 2) {
+              x[g][nt][j] = fmaf(s[g][nt][j], mul[nt][0], -base[nt][0]);
+              x[g][nt][j + 1] = fmaf(s[g][nt][j + 1], mul[nt][1], -base[nt][1]);
+              top = fmax3(top, x[g][nt][j], x[g][nt][j + 1]);  // a first score is infinitely far above the base
             }
         if (__any_sync(0xffffffffu, top > kSlack + kLift)) {
 #pragma unroll
@@ -660,7 +742,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) kv4_attention_kernel(const Kv4
               base[nt][j] = m;
               sum[nt][j] *= f;
 #pragma unroll
-              for (int t = 0; t < kSteps; ++t) {
+              for (int t = 0; t < kTiles; ++t) {
                 o[t][nt][j] *= f;
                 o[t][nt][j + 2] *= f;
               }
@@ -697,7 +779,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) kv4_attention_kernel(const Kv4
           for (int g = 0; g < 2; ++g)
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-              const uint8_t* row = vs + (g * 16 + kr + j * 8) * (D / 16);
+              const uint8_t* row = ks + v_part + (g ? scales_2nd : 0) + (kr + j * 8) * (D / 16);
               bool nan = false;
 #pragma unroll
               for (int i = 0; i < D / 16; ++i) nan |= e4m3_is_nan(row[i]);
@@ -709,26 +791,17 @@ __global__ void __launch_bounds__(kThreads, CTAS) kv4_attention_kernel(const Kv4
             }
         }
         // ---- O^T += V^T P^T
-        uint32_t pf[NT][2], pf2[NT][2];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            pf[nt][k] = transpose8x8(pack_f16x2(x[0][nt][2 * k], x[0][nt][2 * k + 1]));
-            pf2[nt][k] = transpose8x8(pack_f16x2(x[1][nt][2 * k], x[1][nt][2 * k + 1]));
-          }
-#pragma unroll VU
         for (int g = 0; g < 2; ++g) {
-          if (g) {
+          uint32_t pf[NT][2];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              pf[nt][0] = pf2[nt][0];
-              pf[nt][1] = pf2[nt][1];
-            }
+          for (int nt = 0; nt < NT; ++nt) {
+            pf[nt][0] = transpose8x8(pack_f16x2(x[g][nt][0], x[g][nt][1]));
+            pf[nt][1] = transpose8x8(pack_f16x2(x[g][nt][2], x[g][nt][3]));
           }
           // codes and scales of keys c, c + 4, c + 8, c + 12 of the 16
-          const uint8_t* vk = vc + (g * 16 + c) * (D / 2) + r * (D / 16);
-          const uint8_t* vsk = vs + (g * 16 + c) * (D / 16) + (r * (D / 8)) / 16;
+          const uint8_t* vk = kc + v_part + (g ? codes_2nd : 0) + c * (D / 2) + r * (D / 16);
+          const uint8_t* vsk = ks + v_part + (g ? scales_2nd : 0) + c * (D / 16) + (r * (D / 8)) / 16;
           uint32_t v[4][kWordsV], vm[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -791,6 +864,13 @@ __global__ void __launch_bounds__(kThreads, CTAS) kv4_attention_kernel(const Kv4
         phase ^= 1;
       }
     }
+    // the queries and the piece have been read
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&q_empty[buf]);
+    if (++buf == 2) {
+      buf = 0;
+      q_phase ^= 1;
+    }
 
     // ---- the piece is done: join the warps
 #pragma unroll
@@ -806,55 +886,56 @@ __global__ void __launch_bounds__(kThreads, CTAS) kv4_attention_kernel(const Kv4
           join_ms[warp][row][0] = base[nt][j];
           join_ms[warp][row][1] = l;
         }
-        float* to = join + (warp * R + row) * (D + L::kPad) + r * (D / 8);
-#pragma unroll
-        for (int t = 0; t < kSteps; t += 2)
-          *reinterpret_cast<float4*>(to + 2 * t) =
-              make_float4(o[t][nt][j], o[t][nt][j + 2], o[t + 1][nt][j], o[t + 1][nt][j + 2]);
+        sum[nt][j] = l;
       }
-    named_bar_sync(1, kWork);
-    const bool from_start = first == 0, to_end = first + take == it.units;
-    if (from_start && !to_end && threadIdx.x == 0) {
-      const int last = runs.of(u1 - left + it.units - 1);  // the CTA with the item's last unit
-      p.shared[blockIdx.x] = Shared{last - (int)blockIdx.x, it.s.start, it.s.n, it.h * p.group, it.rt * R};
-    }
-    const int slot = 2 * blockIdx.x + (from_start ? 1 : 0);
+    const int slot = 2 * blockIdx.x + (it.first == 0 ? 1 : 0);
     float* part_o = p.partial + (long long)slot * R * D;
     float* part_ms = p.partial + 2ll * p.ctas * R * D + (long long)slot * R * 2;
-    for (int x = threadIdx.x; x < R * (D / 4); x += kWork) {
-      const int row = x / (D / 4), d0 = (x % (D / 4)) * 4;
-      float m = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) m = fmaxf(m, join_ms[w][row][0]);
-      float l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int h = 0; h < D / 64; ++h) {  // 8 of the D / 8 elements of a thread at a time
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        const float mw = join_ms[w][row][0];
-        const float f = mw == -INFINITY ? (join_ms[w][row][1] != join_ms[w][row][1] ? 1.f : 0.f) : ex2(mw - m);
-        const float4 y = *reinterpret_cast<const float4*>(join + (w * R + row) * (D + L::kPad) + d0);
-        l += join_ms[w][row][1] * f;
-        acc[0] += y.x * f; acc[1] += y.y * f; acc[2] += y.z * f; acc[3] += y.w * f;
-      }
-      if (from_start && to_end) {
-        int head;
-        const int t = row_token(p, it, it.rt * R + row, head);
-        if (t >= 0) {
-          finish_row<4>(p, t, head, d0, acc, l);
-          if (d0 == 0) finish_lse(p, t, head, m, l);
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float* to = join + (warp * R + nt * 8 + 2 * c + j) * L::kRow + r * 8;
+#pragma unroll
+          for (int t = 0; t < 4; t += 2)
+            *reinterpret_cast<float4*>(to + 2 * t) = make_float4(o[4 * h + t][nt][j], o[4 * h + t][nt][j + 2],
+                                                                 o[4 * h + t + 1][nt][j], o[4 * h + t + 1][nt][j + 2]);
         }
-      } else {
-        *reinterpret_cast<float4*>(part_o + row * D + d0) = make_float4(acc[0], acc[1], acc[2], acc[3]);
-        if (d0 == 0) {
-          part_ms[2 * row] = m;
-          part_ms[2 * row + 1] = l;
+      named_bar_sync(1, kWork);
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        const int row = i * 8 + threadIdx.x / 16, e = threadIdx.x % 16 * 4;
+        const int d0 = (e >> 3) * (D / 8) + 8 * h + (e & 7);
+        float m = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) m = fmaxf(m, join_ms[w][row][0]);
+        float l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          const float mw = join_ms[w][row][0], lw = join_ms[w][row][1];
+          const float f = mw == m ? 1.f : ex2(mw - m);  // a warp without a key: 0, or 1 of nothing
+          const float4 y = *reinterpret_cast<const float4*>(join + (w * R + row) * L::kRow + e);
+          l += lw * f;
+          acc[0] += y.x * f; acc[1] += y.y * f; acc[2] += y.z * f; acc[3] += y.w * f;
+        }
+        if (it.whole) {
+          int head;
+          const int t = row_token(p, it.row0 + row, it.h, it.start, it.n, head);
+          if (t >= 0) {
+            finish_row<4>(p, t, head, d0, acc, l);
+            if (d0 == 0) finish_lse(p, t, head, m, l);
+          }
+        } else {
+          *reinterpret_cast<float4*>(part_o + row * D + d0) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+          if (d0 == 0) {
+            part_ms[2 * row] = m;
+            part_ms[2 * row + 1] = l;
+          }
         }
       }
-    }
-    named_bar_sync(1, kWork);
-    left -= take;
-    if (left > 0) {
-      next_item<R>(p, it);
-      first = 0;
+      if (h + 1 < D / 64) named_bar_sync(1, kWork);
     }
   }
 }
@@ -932,7 +1013,7 @@ int tile_rows(int head_dim, long long rows) { return head_dim == 256 || rows <= 
 template <int D, int NT, int STAGES, int CTAS>
 int launch_attention(Kv4AttnParams& p, cudaStream_t s) {
   using L = Layout<D, NT, STAGES>;
-  static_assert(CTAS <= kMaxPerSm && CTAS * (L::kBytes + NT * D * 16 + 2048) <= 227 * 1024, "CTAS CTAs fit on an SM");
+  static_assert(CTAS <= kMaxPerSm && CTAS * (L::kBytes + NT * D * 32 + 2048) <= 227 * 1024, "CTAS CTAs fit on an SM");
   p.ctas = sm_count() * CTAS;
   p.shared = reinterpret_cast<Shared*>(p.partial + 2ll * p.ctas * L::R * (D + 2));
   B2F_CUDA_TRY(cudaFuncSetAttribute(kv4_attention_kernel<D, NT, STAGES, CTAS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
