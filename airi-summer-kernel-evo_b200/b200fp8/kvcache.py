@@ -25,8 +25,12 @@ import torch
 
 from . import _lib
 from ._lib import check
-from .ops import _DT, _stream
+from .ops import _DT, _raw_stream
 
+_IN_KINDS = (torch.bfloat16, torch.float8_e4m3fn, torch.float16, torch.float32, torch.uint8)
+_READ_KINDS = (torch.bfloat16, torch.float16, torch.float32)
+_QUERY_KINDS = (torch.bfloat16, torch.float8_e4m3fn, torch.float16, torch.uint8)
+_GATE_KINDS = (torch.float8_e4m3fn, torch.bfloat16, torch.uint8)
 _PAGE_SIZES = (16, 32, 64)
 _HEAD_DIMS = (64, 128, 256)
 
@@ -78,8 +82,16 @@ class Fp4Cache:
         self.page_size, self.head_dim = page_size, head_dim
         self.k_scale, self.v_scale = float(k_scale), float(v_scale)
         self.device = storage.device
+        self._index = storage.get_device()
+        self._cols, self._seqs = self.kv_heads * head_dim, table.shape[0]
+        lib = _lib.lib()
+        self._write, self._read, self._attention = (lib.b2f_kv4_write, lib.b2f_kv4_read,
+                                                    lib.b2f_kv4_attention)
+        with torch.cuda.device(self._index):
+            self._work_ints = -(-int(lib.b2f_kv4_attention_workspace_bytes(head_dim)) // 4)
         c = _lib.Kv4Cache()
-        c.page_stride, c.pages, c.kv_heads = storage.stride(1), self.pages, self.kv_heads
+        c.storage, c.page_stride = storage.data_ptr(), storage.stride(1)
+        c.pages, c.kv_heads = self.pages, self.kv_heads
         c.head_dim, c.page_size = head_dim, page_size
         c.k_scale, c.v_scale = self.k_scale, self.v_scale
         c.table, c.table_rows, c.table_cols = table.data_ptr(), *table.shape
@@ -93,54 +105,63 @@ class Fp4Cache:
         p.table, p.table_rows, p.table_cols = table.data_ptr(), *table.shape
         p.table_ld, p.lens, p.refs = table.stride(0), lens.data_ptr(), refs.data_ptr()
         self._pool = p
-        self._work_bytes = None
 
     # ------------------------------------------------------------------ helpers
 
     def _run(self, fn, *args) -> None:
         """Calls ``fn(*args, stream)`` with this cache's device current, on its current stream."""
-        if torch.cuda.current_device() == self.device.index:
-            check(fn(*args, _stream()))
+        if torch.cuda.current_device() == self._index:
+            code = fn(*args, _raw_stream(self._index))
         else:
-            with torch.cuda.device(self.device):
-                check(fn(*args, _stream()))
+            with torch.cuda.device(self._index):
+                code = fn(*args, _raw_stream(self._index))
+        if code:
+            check(code)
 
-    def _here(self, *tensors: Optional[torch.Tensor]) -> None:
-        for t in tensors:
-            if t is not None and t.device != self.device:
-                if not t.is_cuda:
-                    raise ValueError("b200fp8 ops take CUDA tensors only (no CPU fallback)")
-                raise ValueError(f"tensor on {t.device}, the cache is on {self.device}")
+    def _here(self, t: torch.Tensor, name: str) -> None:
+        if t.get_device() != self._index:
+            if not t.is_cuda:
+                raise ValueError("b200fp8 ops take CUDA tensors only (no CPU fallback)")
+            raise ValueError(f"{name} is on {t.device}, the cache is on {self.device}")
 
-    def _list(self, t: Optional[torch.Tensor], name: str) -> None:
-        if t is not None and (t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous()):
+    def _list(self, t: torch.Tensor, name: str) -> int:
+        """Length of an int32 list on this cache's device."""
+        self._here(t, name)
+        if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous():
             raise TypeError(f"{name} must be a contiguous int32 vector")
+        return t.shape[0]
 
-    def _fill(self, a, layer: int, tokens: int, rows, starts) -> None:
-        """Cache and batch of an argument block."""
+    def _batch(self, a, layer: int, tokens: int, rows, starts) -> None:
+        """Fills in the cache and the batch of an argument block."""
         if not 0 <= layer < self.layers:
             raise ValueError(f"layer {layer} of {self.layers}")
-        self._here(rows, starts)
-        self._list(rows, "rows")
-        self._list(starts, "starts")
-        seqs = rows.shape[0] if rows is not None else (
-            starts.shape[0] - 1 if starts is not None else self.table.shape[0])
-        if starts is not None and starts.shape[0] != seqs + 1:
-            raise ValueError("starts must have one entry more than there are sequences")
-        if starts is None and (seqs == 0 or tokens % seqs):
-            raise ValueError("without starts, every sequence has the same number of new tokens")
         a.cache = self._cache
-        a.cache.storage = self.storage.data_ptr() + layer * self.storage.stride(0)
+        if layer:
+            a.cache.storage = self._cache.storage + layer * self._pool.layer_stride
         b = a.batch
+        if rows is not None:
+            seqs = self._list(rows, "rows")
+            b.rows = rows.data_ptr()
+        elif starts is not None:
+            seqs = starts.shape[0] - 1
+        else:
+            seqs = self._seqs
+        if starts is not None:
+            if self._list(starts, "starts") != seqs + 1:
+                raise ValueError("starts must have one entry more than there are sequences")
+            b.starts = starts.data_ptr()
+        elif seqs == 0 or tokens % seqs:
+            raise ValueError("without starts, every sequence has the same number of new tokens")
         b.seqs, b.tokens = seqs, tokens
-        b.rows = None if rows is None else rows.data_ptr()
-        b.starts = None if starts is None else starts.data_ptr()
 
-    def _matrix(self, t: torch.Tensor, name: str, heads: int, dtypes) -> None:
-        if t.dim() != 2 or t.stride(1) != 1 or t.shape[1] != heads * self.head_dim:
-            raise ValueError(f"{name} must be a row-major [tokens, {heads * self.head_dim}] tensor")
-        if t.dtype not in dtypes:
-            raise TypeError(f"{name} must be one of {[str(d) for d in dtypes]}")
+    def _matrix(self, t: torch.Tensor, name: str, tokens: int, cols: int, kinds) -> int:
+        """Row pitch of a row-major [tokens, cols] tensor on this cache's device."""
+        self._here(t, name)
+        if t.shape != (tokens, cols) or (cols > 1 and t.stride(1) != 1):
+            raise ValueError(f"{name} must be a row-major [{tokens}, {cols}] tensor")
+        if t.dtype not in kinds:
+            raise TypeError(f"{name} must be one of {[str(d) for d in kinds]}")
+        return t.stride(0)
 
     # ------------------------------------------------------------------ tokens
 
@@ -152,20 +173,18 @@ class Fp4Cache:
         sequence at position length - n + i.  ``starts`` int32 [seqs + 1] cuts the packed
         tokens into sequences (None: equal parts), ``rows`` int32 [seqs] names their table
         rows (None: in order; distinct)."""
-        self._here(k, v)
-        kinds = (torch.float32, torch.bfloat16, torch.float16, torch.float8_e4m3fn, torch.uint8)
-        self._matrix(k, "k", self.kv_heads, kinds)
-        self._matrix(v, "v", self.kv_heads, kinds)
-        if k.shape != v.shape or k.dtype != v.dtype:
-            raise ValueError("k and v must have one shape and type")
-        if k.shape[0] == 0:
-            return
         a = _lib.Kv4WriteArgs()
-        self._fill(a, layer, k.shape[0], rows, starts)
-        a.k, a.k_ld, a.k_in_scale = k.data_ptr(), k.stride(0), k_in_scale
-        a.v, a.v_ld, a.v_in_scale = v.data_ptr(), v.stride(0), v_in_scale
+        tokens = k.shape[0]
+        a.k_ld = self._matrix(k, "k", tokens, self._cols, _IN_KINDS)
+        a.v_ld = self._matrix(v, "v", tokens, self._cols, _IN_KINDS)
+        if k.dtype != v.dtype:
+            raise TypeError("k and v must have one type")
+        if tokens == 0:
+            return
+        self._batch(a, layer, tokens, rows, starts)
+        a.k, a.k_in_scale, a.v, a.v_in_scale = k.data_ptr(), k_in_scale, v.data_ptr(), v_in_scale
         a.dtype = _DT[k.dtype]
-        self._run(_lib.lib().b2f_kv4_write, ctypes.byref(a))
+        self._run(self._write, a)
 
     def read(self, tokens: int, *, layer: int = 0, rows: Optional[torch.Tensor] = None,
              starts: Optional[torch.Tensor] = None, dtype: torch.dtype = torch.bfloat16,
@@ -174,24 +193,20 @@ class Fp4Cache:
         """The values that the cache holds for the last tokens of the sequences, placed as in
         :meth:`write`: (k, v), [tokens, kv_heads * head_dim] each, f32, bf16 or f16.  Rows of
         given ``k`` / ``v`` that belong to no sequence are left as they are."""
-        cols = self.kv_heads * self.head_dim
         if k is None:
-            k = torch.empty((tokens, cols), dtype=dtype, device=self.device)
+            k = self.lens.new_empty((tokens, self._cols), dtype=dtype)
         if v is None:
-            v = torch.empty((tokens, cols), dtype=k.dtype, device=self.device)
-        self._here(k, v)
-        kinds = (torch.float32, torch.bfloat16, torch.float16)
-        self._matrix(k, "k", self.kv_heads, kinds)
-        self._matrix(v, "v", self.kv_heads, kinds)
-        if k.shape != v.shape or k.dtype != v.dtype or k.shape[0] != tokens:
-            raise ValueError("k and v must have one type and [tokens, kv_heads * head_dim] elements")
+            v = torch.empty_like(k)
+        a = _lib.Kv4ReadArgs()
+        a.k_ld = self._matrix(k, "k", tokens, self._cols, _READ_KINDS)
+        a.v_ld = self._matrix(v, "v", tokens, self._cols, _READ_KINDS)
+        if k.dtype != v.dtype:
+            raise TypeError("k and v must have one type")
         if tokens == 0:
             return k, v
-        a = _lib.Kv4ReadArgs()
-        self._fill(a, layer, tokens, rows, starts)
-        a.k, a.k_ld, a.v, a.v_ld = k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0)
-        a.dtype = _DT[k.dtype]
-        self._run(_lib.lib().b2f_kv4_read, ctypes.byref(a))
+        self._batch(a, layer, tokens, rows, starts)
+        a.k, a.v, a.dtype = k.data_ptr(), v.data_ptr(), _DT[k.dtype]
+        self._run(self._read, a)
         return k, v
 
     def attention(self, q: torch.Tensor, *, heads: int, layer: int = 0,
@@ -205,48 +220,41 @@ class Fp4Cache:
         value = stored * q_scale) over the cached keys of their sequences, the new ones among
         them (see b2f_kv4_attention).  ``out`` bf16, f16 or e4m3 (stored = value / ctx_scale).
         With ``return_lse`` returns (out, lse f32 [tokens, heads])."""
-        self._here(q, gate, out, lse)
-        kinds = (torch.bfloat16, torch.float16, torch.float8_e4m3fn, torch.uint8)
-        self._matrix(q, "q", heads, kinds)
-        tokens = q.shape[0]
+        a = _lib.Kv4AttnArgs()
+        tokens, cols = q.shape[0], heads * self.head_dim
+        a.q_ld = self._matrix(q, "q", tokens, cols, _QUERY_KINDS)
         if out is None:
-            out = torch.empty((tokens, heads * self.head_dim), dtype=out_dtype, device=self.device)
-        self._matrix(out, "out", heads, kinds)
-        if out.shape[0] != tokens:
-            raise ValueError("out must have a row for every token")
+            out = q.new_empty((tokens, cols), dtype=out_dtype)
+        a.out_ld = self._matrix(out, "out", tokens, cols, _QUERY_KINDS)
         if return_lse and lse is None:
-            lse = torch.empty((tokens, heads), dtype=torch.float32, device=self.device)
-        if lse is not None and (lse.dtype != torch.float32 or lse.shape != (tokens, heads)
-                                or not lse.is_contiguous()):
-            raise ValueError("lse must be contiguous float32 [tokens, heads]")
-        if gate is not None and (gate.dim() != 2 or gate.stride(1) != 1 or gate.shape[0] != tokens
-                                 or gate.dtype not in (torch.float8_e4m3fn, torch.uint8,
-                                                       torch.bfloat16)):
-            raise ValueError("gate must be row-major e4m3 or bf16 with a row for every token")
+            lse = q.new_empty((tokens, heads), dtype=torch.float32)
+        if lse is not None:
+            self._here(lse, "lse")
+            if (lse.dtype != torch.float32 or lse.shape != (tokens, heads)
+                    or not lse.is_contiguous()):
+                raise ValueError("lse must be contiguous float32 [tokens, heads]")
+            a.lse = lse.data_ptr()
+        if gate is not None:
+            self._here(gate, "gate")
+            stride = self.head_dim if gate_head_stride is None else gate_head_stride
+            if (gate.dim() != 2 or gate.shape[0] != tokens or gate.stride(1) != 1
+                    or gate.dtype not in _GATE_KINDS
+                    or gate.shape[1] < (heads - 1) * stride + self.head_dim):
+                raise ValueError("gate must be row-major e4m3 or bf16, with a row for every token "
+                                 "and a column for every element of every head")
+            a.gate, a.gate_dtype, a.gate_ld = gate.data_ptr(), _DT[gate.dtype], gate.stride(0)
+            a.gate_head_stride, a.gate_scale = stride, gate_scale
         if tokens == 0:
             return (out, lse) if return_lse else out
-        a = _lib.Kv4AttnArgs()
-        self._fill(a, layer, tokens, rows, starts)
-        a.heads, a.causal = heads, 1 if causal else 0
-        a.q, a.q_dtype, a.q_ld, a.q_scale = q.data_ptr(), _DT[q.dtype], q.stride(0), q_scale
-        a.sm_scale = sm_scale
-        if gate is not None:
-            a.gate, a.gate_dtype, a.gate_ld = gate.data_ptr(), _DT[gate.dtype], gate.stride(0)
-            a.gate_head_stride = self.head_dim if gate_head_stride is None else gate_head_stride
-            if gate.shape[1] < (heads - 1) * a.gate_head_stride + self.head_dim:
-                raise ValueError("gate has too few columns")
-        a.gate_scale = gate_scale
-        a.out, a.out_dtype, a.out_ld, a.ctx_scale = (out.data_ptr(), _DT[out.dtype], out.stride(0),
-                                                     ctx_scale)
-        a.lse = None if lse is None else lse.data_ptr()
+        self._batch(a, layer, tokens, rows, starts)
+        a.heads, a.causal, a.q, a.q_dtype = heads, causal, q.data_ptr(), _DT[q.dtype]
+        a.q_scale, a.sm_scale = q_scale, sm_scale
+        a.out, a.out_dtype, a.ctx_scale = out.data_ptr(), _DT[out.dtype], ctx_scale
         # A workspace of this call's own, from the caching allocator of the current stream: calls
         # on other streams, and in graphs, never share it.
-        if self._work_bytes is None:
-            with torch.cuda.device(self.device):
-                self._work_bytes = int(_lib.lib().b2f_kv4_attention_workspace_bytes(self.head_dim))
-        work = torch.empty(self._work_bytes, dtype=torch.uint8, device=self.device)
-        a.workspace, a.workspace_bytes = work.data_ptr(), self._work_bytes
-        self._run(_lib.lib().b2f_kv4_attention, ctypes.byref(a))
+        work = self.lens.new_empty(self._work_ints)
+        a.workspace, a.workspace_bytes = work.data_ptr(), 4 * self._work_ints
+        self._run(self._attention, a)
         return (out, lse) if return_lse else out
 
     # ------------------------------------------------------------------ pages
@@ -254,48 +262,39 @@ class Fp4Cache:
     def extend(self, counts: torch.Tensor, rows: Optional[torch.Tensor] = None) -> None:
         """Lengthens rows (None: rows 0 .. n - 1) by ``counts`` tokens (int32 [n], n <= 1024) and
         gives them the pages for it, or does nothing when the pages do not suffice."""
-        self._here(counts, rows)
-        self._list(counts, "counts")
-        self._list(rows, "rows")
-        if rows is not None and rows.shape != counts.shape:
+        n = self._list(counts, "counts")
+        if rows is not None and self._list(rows, "rows") != n:
             raise ValueError("rows and counts must have one length")
-        if counts.shape[0]:
-            self._run(_lib.lib().b2f_kv4_extend, ctypes.byref(self._pool),
-                      None if rows is None else rows.data_ptr(), counts.data_ptr(),
-                      counts.shape[0])
+        if n:
+            self._run(_lib.lib().b2f_kv4_extend, self._pool,
+                      None if rows is None else rows.data_ptr(), counts.data_ptr(), n)
 
     def fork(self, src: torch.Tensor, dst: torch.Tensor) -> None:
-        """Makes the empty rows ``dst`` copies of rows ``src`` (int32 [n]; src may repeat): full
-        pages are shared, a last page that is not full is copied."""
-        self._here(src, dst)
-        self._list(src, "src")
-        self._list(dst, "dst")
-        n = src.shape[0]
-        if dst.shape[0] != n:
+        """Makes the empty rows ``dst`` copies of rows ``src`` (int32 [n], n <= 1024; src may
+        repeat): full pages are shared, a last page that is not full is copied."""
+        n = self._list(src, "src")
+        if self._list(dst, "dst") != n:
             raise ValueError("src and dst must have one length")
         if n:
-            work = torch.empty(n + 1, dtype=torch.int32, device=self.device)
-            self._run(_lib.lib().b2f_kv4_fork, ctypes.byref(self._pool), src.data_ptr(),
-                      dst.data_ptr(), n, work.data_ptr(), 4 * (n + 1))
+            work = self.lens.new_empty(n + 1)
+            self._run(_lib.lib().b2f_kv4_fork, self._pool, src.data_ptr(), dst.data_ptr(), n,
+                      work.data_ptr(), 4 * (n + 1))
 
     def free(self, rows: Optional[torch.Tensor] = None) -> None:
         """Empties ``rows`` (int32 [n]; None: all); pages that no other row uses become free."""
-        self._here(rows)
-        self._list(rows, "rows")
-        if rows is not None and rows.shape[0]:
-            self._run(_lib.lib().b2f_kv4_free, ctypes.byref(self._pool), rows.data_ptr(),
-                      rows.shape[0])
-        elif rows is None:
-            every = torch.arange(self.table.shape[0], dtype=torch.int32, device=self.device)
-            for part in every.split(1024):
-                self._run(_lib.lib().b2f_kv4_free, ctypes.byref(self._pool), part.data_ptr(),
-                          part.shape[0])
+        free = _lib.lib().b2f_kv4_free
+        if rows is None:
+            rows = torch.arange(self._seqs, dtype=torch.int32, device=self.device)
+        n = self._list(rows, "rows")
+        for at in range(0, n, 1024):
+            self._run(free, self._pool, rows.data_ptr() + 4 * at, min(1024, n - at))
 
     def compact(self) -> None:
         """Moves the pages in use to the front of the pool; the table follows."""
-        n = int(_lib.lib().b2f_kv4_compact_workspace_bytes(self.pages))
-        work = torch.empty(n, dtype=torch.uint8, device=self.device)
-        self._run(_lib.lib().b2f_kv4_compact, ctypes.byref(self._pool), work.data_ptr(), n)
+        lib = _lib.lib()
+        ints = int(lib.b2f_kv4_compact_workspace_bytes(self.pages)) // 4
+        work = self.lens.new_empty(ints)
+        self._run(lib.b2f_kv4_compact, self._pool, work.data_ptr(), 4 * ints)
 
     def copy_pages(self, src: Sequence[int], dst: Sequence[int]) -> None:
         """Copies pages ``src[i]`` to ``dst[i]`` in all layers (host lists); table and counts
@@ -305,8 +304,7 @@ class Fp4Cache:
             raise ValueError("src and dst must have one length")
         if n:
             ints = ctypes.c_int * n
-            self._run(_lib.lib().b2f_kv4_copy_pages, ctypes.byref(self._pool), ints(*src),
-                      ints(*dst), n)
+            self._run(_lib.lib().b2f_kv4_copy_pages, self._pool, ints(*src), ints(*dst), n)
 
     def free_pages(self) -> int:
         """Pages that no row uses (waits for the device)."""

@@ -34,6 +34,11 @@ def _stream() -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
+def _raw_stream(index: int) -> int:
+    """The handle of the current stream of device ``index``."""
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
@@ -483,64 +488,73 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
     transposed map).  Outputs, [rows, heads * head_dim], have the inputs' type unless
     ``out_dtype`` says otherwise (e4m3: stored = value / out_scale); ``q_out`` / ``k_out`` may be
     the inputs themselves.  Returns (q_out, k_out)."""
-    _check_cuda(q, k, positions, q_weight, k_weight, q_out, k_out, plan.freqs)
+    index = q.get_device()
+    for t in (q, k, positions, q_weight, k_weight, q_out, k_out, plan.freqs):
+        if t is not None and t.get_device() != index or index < 0:
+            _check_cuda(q, t)
+            raise ValueError("all tensors, and the plan, must be on one device")
     d = plan.head_dim
     rows = q.shape[0]
     if (k is None) != (kv_heads == 0):
         raise ValueError("k and kv_heads go together")
-    if k is not None and (k.dtype != q.dtype or k.shape[0] != rows):
-        raise ValueError("q and k must have one type and number of rows")
-    if (positions.dtype not in (torch.int32, torch.int64) or positions.dim() != 1
-            or positions.shape[0] != rows or not positions.is_contiguous()):
+    if (positions.dtype not in (torch.int32, torch.int64) or positions.shape != (rows,)
+            or not positions.is_contiguous()):
         raise TypeError("positions must be contiguous int32 or int64 [rows]")
-    for w in (q_weight, k_weight):
-        if w is not None and (w.dtype != torch.float32 or not w.is_contiguous() or w.numel() != d):
-            raise TypeError("weights must be contiguous float32 [head_dim]")
-    if k is not None and (q_weight is None) != (k_weight is None):
-        raise ValueError("q_weight and k_weight go together")
-    dtype = out_dtype if out_dtype is not None else (
-        q_out.dtype if q_out is not None else k_out.dtype if k_out is not None else q.dtype)
-    if q_out is None:
-        q_out = torch.empty((rows, heads * d), dtype=dtype, device=q.device)
-    if k is not None and k_out is None:
-        k_out = torch.empty((rows, kv_heads * d), dtype=dtype, device=q.device)
+    if out_dtype is None:
+        out_dtype = (q_out.dtype if q_out is not None else
+                     k_out.dtype if k_out is not None else q.dtype)
     a = _lib.RotaryArgs()
-    _lib.lib().b2f_rotary_args_init(ctypes.byref(a))
-    a.rows, a.q_heads, a.k_heads = rows, heads, kv_heads
-    a.head_dim, a.rotary_dim = d, plan.rotary_dim
-    a.interleaved, a.inverse = int(plan.interleaved), int(inverse)
+    if q_weight is not None or k_weight is not None:
+        if k is not None and (q_weight is None or k_weight is None):
+            raise ValueError("q_weight and k_weight go together")
+        for w in (q_weight, k_weight):
+            if w is not None and (w.dtype != torch.float32 or not w.is_contiguous()
+                                  or w.numel() != d):
+                raise TypeError("weights must be contiguous float32 [head_dim]")
+        a.q_weight, a.k_weight = _ptr(q_weight), _ptr(k_weight)
+    if q_out is None:
+        q_out = q.new_empty((rows, heads * d), dtype=out_dtype)
     a.q_head_stride = d if q_head_stride is None else q_head_stride
-    a.k_head_stride = d if k_head_stride is None else k_head_stride
-    for x, y, n, hs, nm in ((q, q_out, heads, a.q_head_stride, "q"),
-                            (k, k_out, kv_heads, a.k_head_stride, "k")):
-        if x is None:
-            continue
-        if x.dim() != 2 or x.stride(1) != 1 or x.dtype not in _DT:
-            raise ValueError(f"{nm} must be a row-major 2-D tensor of f32, bf16, f16 or e4m3")
-        if n <= 0 or x.shape[1] < (n - 1) * hs + d:
-            raise ValueError(f"{nm} has too few columns for {n} heads")
-        if (y.dim() != 2 or y.stride(1) != 1 or y.dtype != dtype or y.dtype not in _DT
-                or y.shape != (rows, n * d)):
-            raise ValueError(f"{nm}_out must be a row-major [{rows}, {n * d}] tensor of {dtype}")
-        if x.device != positions.device or y.device != positions.device:
-            raise ValueError("all tensors must be on one device")
-    if plan.freqs.device != positions.device:
-        raise ValueError(f"the plan is on {plan.freqs.device}, the tensors are on "
-                         f"{positions.device}")
+    a.q_ld, a.q_out_ld = _rotary_side("q", q, q_out, q.dtype, out_dtype, rows, heads, d,
+                                      a.q_head_stride)
+    a.q, a.q_out = q.data_ptr(), q_out.data_ptr()
+    if k is not None:
+        if k_out is None:
+            k_out = q.new_empty((rows, kv_heads * d), dtype=out_dtype)
+        a.k_head_stride = d if k_head_stride is None else k_head_stride
+        a.k_ld, a.k_out_ld = _rotary_side("k", k, k_out, q.dtype, out_dtype, rows, kv_heads, d,
+                                          a.k_head_stride)
+        a.k, a.k_out = k.data_ptr(), k_out.data_ptr()
     if rows == 0:
         return q_out, k_out
-    a.q, a.q_ld, a.q_out, a.q_out_ld = q.data_ptr(), q.stride(0), q_out.data_ptr(), q_out.stride(0)
-    if k is not None:
-        a.k, a.k_ld, a.k_out, a.k_out_ld = (k.data_ptr(), k.stride(0), k_out.data_ptr(),
-                                            k_out.stride(0))
-    a.in_dtype, a.in_scale, a.out_dtype, a.out_scale = _DT[q.dtype], in_scale, _DT[dtype], out_scale
-    a.q_weight, a.k_weight = _ptr(q_weight), _ptr(k_weight)
+    a.rows, a.q_heads, a.k_heads, a.head_dim, a.rotary_dim = rows, heads, kv_heads, d, plan.rotary_dim
+    a.interleaved, a.inverse = plan.interleaved, inverse
+    a.in_dtype, a.in_scale, a.out_dtype, a.out_scale = _DT[q.dtype], in_scale, _DT[out_dtype], out_scale
     a.weight_offset, a.eps = weight_offset, eps
     a.positions, a.position_bits = positions.data_ptr(), 8 * positions.element_size()
     a.freqs, a.magnitude = plan.freqs.data_ptr(), plan.magnitude
-    with torch.cuda.device(q.device):
-        check(_lib.lib().b2f_rotary(ctypes.byref(a), _stream()))
+    if torch.cuda.current_device() == index:
+        code = _lib.lib().b2f_rotary(a, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            code = _lib.lib().b2f_rotary(a, _raw_stream(index))
+    check(code)
     return q_out, k_out
+
+
+def _rotary_side(name, x, y, dtype, out_dtype, rows, heads, d, stride):
+    """Checks one input and output of :func:`rotary`; their row pitches."""
+    if (x.dim() != 2 or x.shape[0] != rows or x.stride(1) != 1 or x.dtype != dtype
+            or dtype not in _DT):
+        raise ValueError(f"{name} must be row-major [{rows}, columns], f32, bf16, f16 or e4m3 "
+                         "(q and k alike)")
+    if heads <= 0 or x.shape[1] < (heads - 1) * stride + d:
+        raise ValueError(f"{name} has too few columns for {heads} heads")
+    if (y.shape != (rows, heads * d) or y.stride(1) != 1 or y.dtype != out_dtype
+            or out_dtype not in _DT):
+        raise ValueError(f"{name}_out must be a row-major [{rows}, {heads * d}] tensor of "
+                         f"{out_dtype}")
+    return x.stride(0), y.stride(0)
 
 
 def quantize_fp8(x: torch.Tensor, *, scale: Optional[float] = None,
