@@ -7,21 +7,43 @@
 
 namespace b2f {
 
+// Four elements as they lie in memory, for loads that are issued long before their use.
 template <int DT>
-__device__ __forceinline__ void load4(const char* base, long long off, float* x) {
-  if (DT == kF32) {
-    const float4 v = *reinterpret_cast<const float4*>(base + off * 4);
-    x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
-  } else if (DT == kE4M3) {
-    const uint32_t v = *reinterpret_cast<const uint32_t*>(base + off);
-    const float2 a = e4m3x2_to_f32x2(uint16_t(v)), b = e4m3x2_to_f32x2(uint16_t(v >> 16));
+struct Raw4 {
+  uint2 v;
+};
+template <>
+struct Raw4<kF32> {
+  float4 v;
+};
+template <>
+struct Raw4<kE4M3> {
+  uint32_t v;
+};
+
+template <int DT>
+__device__ __forceinline__ Raw4<DT> load_raw4(const char* base, long long off) {
+  constexpr int kBytes = DT == kF32 ? 4 : DT == kE4M3 ? 1 : 2;
+  return *reinterpret_cast<const Raw4<DT>*>(base + off * kBytes);
+}
+
+template <int DT>
+__device__ __forceinline__ void unpack4(const Raw4<DT>& r, float* x) {
+  if constexpr (DT == kF32) {
+    x[0] = r.v.x; x[1] = r.v.y; x[2] = r.v.z; x[3] = r.v.w;
+  } else if constexpr (DT == kE4M3) {
+    const float2 a = e4m3x2_to_f32x2(uint16_t(r.v)), b = e4m3x2_to_f32x2(uint16_t(r.v >> 16));
     x[0] = a.x; x[1] = a.y; x[2] = b.x; x[3] = b.y;
   } else {
-    const uint2 v = *reinterpret_cast<const uint2*>(base + off * 2);
-    const float2 a = DT == kBF16 ? unpack_bf16x2(v.x) : unpack_f16x2(v.x);
-    const float2 b = DT == kBF16 ? unpack_bf16x2(v.y) : unpack_f16x2(v.y);
+    const float2 a = DT == kBF16 ? unpack_bf16x2(r.v.x) : unpack_f16x2(r.v.x);
+    const float2 b = DT == kBF16 ? unpack_bf16x2(r.v.y) : unpack_f16x2(r.v.y);
     x[0] = a.x; x[1] = a.y; x[2] = b.x; x[3] = b.y;
   }
+}
+
+template <int DT>
+__device__ __forceinline__ void load4(const char* base, long long off, float* x) {
+  unpack4<DT>(load_raw4<DT>(base, off), x);
 }
 
 // Round-to-nearest-even; e4m3 saturates.

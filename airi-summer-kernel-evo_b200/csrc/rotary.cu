@@ -14,7 +14,7 @@
 // Bound: memory (each element is read and written once).  A lane owns four pairs of a head
 // (8 elements), so a rotation needs no shuffle; a warp owns one token and walks over its
 // heads with the four sines and cosines of the lane in registers (their cost is shared by
-// all heads of q and k), loads of UNROLL heads in flight.  With few tokens the heads of a
+// all heads of q and k), the next head loaded ahead.  With few tokens the heads of a
 // token are dealt to several warps (see the launch).
 #include <algorithm>
 #include <cmath>
@@ -28,9 +28,9 @@ namespace b2f {
 namespace {
 
 struct RotaryParams {
-  int rows, q_heads, heads, head_dim, rotary_dim;  // heads: q and k together
-  int lanes_log2;                                  // lanes of a head
-  int warps_per_row, iters_per_warp;
+  int rows, q_heads, k_heads, head_dim, rotary_dim;
+  int lanes_log2;                              // lanes of a head
+  int rounds, warps_per_row, rounds_per_warp;  // a round: the heads that a warp has at a time
   int inverse, position_bits;
   const char* q;
   const char* k;
@@ -52,7 +52,7 @@ constexpr int kRotaryWarps = 4;
 
 // The lane's 8 elements sit at e0 .. e0 + 3 and e1 .. e1 + 3; in the half layout these are
 // the first and the second member of its four pairs, else two times two neighbouring pairs.
-template <int TI, int TO, bool INTERLEAVED, int UNROLL>
+template <int TI, int TO, bool INTERLEAVED, bool NORM, int AHEAD>
 __global__ void __launch_bounds__(32 * kRotaryWarps) rotary_kernel(const RotaryParams p) {
   pdl_wait();
   pdl_trigger();
@@ -75,6 +75,44 @@ __global__ void __launch_bounds__(32 * kRotaryWarps) rotary_kernel(const RotaryP
     e1 = half + j * 4;
   }
 
+  // Rounds of hpw heads: first those of q, then those of k.  The elements of the next AHEAD rounds
+  // are in flight while those of this one are turned, the first ones while the angles are made.
+  const int q_rounds = (p.q_heads + hpw - 1) >> (5 - p.lanes_log2);
+  const int first = part * p.rounds_per_warp;
+  const int last = min(first + p.rounds_per_warp, p.rounds);
+  constexpr int kIn = TI == kF32 ? 4 : TI == kE4M3 ? 1 : 2, kOut = TO == kF32 ? 4 : TO == kE4M3 ? 1 : 2;
+  const char* in;
+  char* out;
+  auto start = [&](int it) {  // where the lane's head of round `it` is read
+    in = it < q_rounds ? p.q + (row * p.q_ld + (it * hpw + sub) * p.q_hstride) * kIn
+                       : p.k + (row * p.k_ld + ((it - q_rounds) * hpw + sub) * p.k_hstride) * kIn;
+  };
+  auto start_out = [&](int it) {
+    out = it < q_rounds ? p.q_out + (row * p.q_out_ld + (long long)(it * hpw + sub) * p.head_dim) * kOut
+                        : p.k_out + (row * p.k_out_ld + (long long)((it - q_rounds) * hpw + sub) * p.head_dim) * kOut;
+  };
+  auto there = [&](int it) {
+    return active && (it < q_rounds ? it * hpw + sub < p.q_heads : (it - q_rounds) * hpw + sub < p.k_heads);
+  };
+  Raw4<TI> lo[AHEAD], hi[AHEAD];
+  int next = first;  // the round that is loaded next
+  auto load = [&](Raw4<TI>& x, Raw4<TI>& y) {
+    if (next < last) {
+      if (next == first || next == q_rounds) start(next);
+      else in += (next < q_rounds ? p.q_hstride : p.k_hstride) * (hpw * kIn);
+      if (there(next)) {
+        x = load_raw4<TI>(in, e0);
+        y = load_raw4<TI>(in, e1);
+      }
+      ++next;
+    }
+  };
+#pragma unroll
+  for (int u = 0; u < AHEAD; ++u) {
+    lo[u] = hi[u] = Raw4<TI>{};
+    load(lo[u], hi[u]);
+  }
+
   float c[4] = {1.f, 1.f, 1.f, 1.f}, s[4] = {0.f, 0.f, 0.f, 0.f};
   if (turns) {
     const long long pos = p.position_bits == 64
@@ -90,69 +128,62 @@ __global__ void __launch_bounds__(32 * kRotaryWarps) rotary_kernel(const RotaryP
     }
   }
 
-  const int first = part * p.iters_per_warp;
-  const int last = min(first + p.iters_per_warp, (p.heads + hpw - 1) / hpw);
-  for (int it = first; it < last; it += UNROLL) {
-    float x[UNROLL][8];
+  float wt[8];
+  start_out(first);
+  for (int base = first; base < last; base += AHEAD) {
 #pragma unroll
-    for (int u = 0; u < UNROLL; ++u) {
-      const int h = (it + u) * hpw + sub;
-      if (it + u < last && h < p.heads && active) {
-        const bool is_q = h < p.q_heads;
-        const long long at = is_q ? row * p.q_ld + h * p.q_hstride
-                                  : row * p.k_ld + (h - p.q_heads) * p.k_hstride;
-        const char* base = is_q ? p.q : p.k;
-        load4<TI>(base, at + e0, x[u]);
-        load4<TI>(base, at + e1, x[u] + 4);
-      } else {
+   for (int u = 0; u < AHEAD; ++u) {
+    const int it = base + u;
+    if (it >= last) break;
+    const bool live = there(it);
+    float x[8];
+    unpack4<TI>(lo[u], x);
+    unpack4<TI>(hi[u], x + 4);
+    load(lo[u], hi[u]);
+    if (NORM && (it == first || it == q_rounds)) {
+      const char* weight = reinterpret_cast<const char*>(it < q_rounds ? p.q_weight : p.k_weight);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[u][i] = 0.f;
+      for (int i = 0; i < 8; ++i) wt[i] = 0.f;
+      if (active) {
+        load4<kF32>(weight, e0, wt);
+        load4<kF32>(weight, e1, wt + 4);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) wt[i] += p.weight_offset;
       }
     }
 #pragma unroll
-    for (int u = 0; u < UNROLL; ++u) {
-      const int h = (it + u) * hpw + sub;
-      const bool is_q = h < p.q_heads;
-      const bool live = it + u < last && h < p.heads && active;
+    for (int i = 0; i < 8; ++i) x[i] *= p.in_scale;
+    if (NORM) {
+      float sum = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[u][i] *= p.in_scale;
-      if (p.q_weight != nullptr) {  // the same for all lanes: the shuffles below are whole
-        float sum = 0.f;
+      for (int i = 0; i < 8; ++i) sum = fmaf(x[i], x[i], sum);
+      if (!live) sum = 0.f;
+      for (int o = 1; o < lph; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      const float inv = rsqrtf(sum / float(p.head_dim) + p.eps);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sum = fmaf(x[u][i], x[u][i], sum);
-        for (int o = 1; o < lph; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        const float inv = rsqrtf(sum / float(p.head_dim) + p.eps);
-        const float* wt = is_q ? p.q_weight : p.k_weight;
-        if (live) {
+      for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * wt[i];
+    }
+    if (turns) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            x[u][i] = x[u][i] * inv * (wt[e0 + i] + p.weight_offset);
-            x[u][i + 4] = x[u][i + 4] * inv * (wt[e1 + i] + p.weight_offset);
-          }
-        }
-      }
-      if (turns) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float& a = INTERLEAVED ? x[u][2 * i] : x[u][i];
-          float& b = INTERLEAVED ? x[u][2 * i + 1] : x[u][i + 4];
-          const float a0 = a, b0 = b;
-          a = fmaf(-b0, s[i], a0 * c[i]);
-          b = fmaf(a0, s[i], b0 * c[i]);
-        }
-      }
-      if (live) {
-        if (TO == kE4M3) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) x[u][i] = __fdiv_rn(x[u][i], p.out_scale);
-        }
-        char* base = is_q ? p.q_out : p.k_out;
-        const long long at = is_q ? row * p.q_out_ld + (long long)h * p.head_dim
-                                  : row * p.k_out_ld + (long long)(h - p.q_heads) * p.head_dim;
-        store4<TO>(base, at + e0, x[u]);
-        store4<TO>(base, at + e1, x[u] + 4);
+      for (int i = 0; i < 4; ++i) {
+        float& a = INTERLEAVED ? x[2 * i] : x[i];
+        float& b = INTERLEAVED ? x[2 * i + 1] : x[i + 4];
+        const float a0 = a, b0 = b;
+        a = fmaf(-b0, s[i], a0 * c[i]);
+        b = fmaf(a0, s[i], b0 * c[i]);
       }
     }
+    if (live) {
+      if (TO == kE4M3) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = __fdiv_rn(x[i], p.out_scale);
+      }
+      store4<TO>(out, e0, x);
+      store4<TO>(out, e1, x + 4);
+    }
+    if (it + 1 == q_rounds) start_out(it + 1);
+    else out += (long long)p.head_dim * (hpw * kOut);
+   }
   }
 }
 
@@ -160,9 +191,13 @@ template <int TI, int TO>
 cudaError_t launch_rotary(const RotaryParams& p, bool interleaved, cudaStream_t s) {
   const long long warps = (long long)p.rows * p.warps_per_row;
   const dim3 grid((unsigned)((warps + kRotaryWarps - 1) / kRotaryWarps));
-  if (interleaved)
-    return launch_pdl(rotary_kernel<TI, TO, true, 4>, grid, dim3(32 * kRotaryWarps), 0, s, p);
-  return launch_pdl(rotary_kernel<TI, TO, false, 4>, grid, dim3(32 * kRotaryWarps), 0, s, p);
+  const dim3 block(32 * kRotaryWarps);
+  constexpr int A = TI == kF32 ? 2 : 4;
+  if (p.q_weight != nullptr)
+    return interleaved ? launch_pdl(rotary_kernel<TI, TO, true, true, A>, grid, block, 0, s, p)
+                       : launch_pdl(rotary_kernel<TI, TO, false, true, A>, grid, block, 0, s, p);
+  return interleaved ? launch_pdl(rotary_kernel<TI, TO, true, false, A>, grid, block, 0, s, p)
+                     : launch_pdl(rotary_kernel<TI, TO, false, false, A>, grid, block, 0, s, p);
 }
 
 template <int TI>
@@ -215,6 +250,8 @@ int b2f_rotary(const b2f_rotary_args* a, b2f_stream_t stream) {
     return fail(B2F_ERR_ARG, "rotary: out_scale belongs to an e4m3 output");
   if (a->q_heads && a->k_heads && (a->q_weight == nullptr) != (a->k_weight == nullptr))
     return fail(B2F_ERR_ARG, "rotary: q_weight and k_weight go together");
+  if ((reinterpret_cast<uintptr_t>(a->q_weight) | reinterpret_cast<uintptr_t>(a->k_weight)) & 15)
+    return fail(B2F_ERR_ARG, "rotary: weights must be 16-byte aligned");
   if ((a->q_weight || a->k_weight) && a->inverse)
     return fail(B2F_ERR_ARG, "rotary: the head norm has no inverse");
   const int is = a->in_dtype == B2F_DTYPE_F32 ? 4 : a->in_dtype == B2F_DTYPE_E4M3 ? 1 : 2;
@@ -232,7 +269,7 @@ int b2f_rotary(const b2f_rotary_args* a, b2f_stream_t stream) {
       return fail(B2F_ERR_ARG, "rotary: tensors and rows must be aligned to four elements");
   }
   RotaryParams p = {};
-  p.rows = a->rows; p.q_heads = a->q_heads; p.heads = a->q_heads + a->k_heads;
+  p.rows = a->rows; p.q_heads = a->q_heads; p.k_heads = a->k_heads;
   p.head_dim = d; p.rotary_dim = a->rotary_dim;
   p.lanes_log2 = d <= 64 ? 3 : d <= 128 ? 4 : 5;
   p.inverse = a->inverse; p.position_bits = a->position_bits;
@@ -245,13 +282,13 @@ int b2f_rotary(const b2f_rotary_args* a, b2f_stream_t stream) {
   p.positions = a->positions; p.freqs = a->freqs; p.magnitude = a->magnitude;
   p.q_out = reinterpret_cast<char*>(a->q_out); p.k_out = reinterpret_cast<char*>(a->k_out);
   p.q_out_ld = a->q_out_ld; p.k_out_ld = a->k_out_ld; p.out_scale = a->out_scale;
-  // One warp per token where tokens fill the GPU (16 warps on each of 148 SMs); fewer tokens
-  // have their heads dealt to more warps, four head groups (one round of loads) at the least.
+  // One warp per token where tokens fill the GPU (32 warps on each of 148 SMs); fewer tokens
+  // have their heads dealt to more warps.
   const int hpw = 32 >> p.lanes_log2;
-  const int iters = (p.heads + hpw - 1) / hpw;
-  const int want = std::max(1, std::min((iters + 3) / 4, (16 * 148 + p.rows - 1) / p.rows));
-  p.iters_per_warp = (iters + want - 1) / want;
-  p.warps_per_row = (iters + p.iters_per_warp - 1) / p.iters_per_warp;
+  p.rounds = (p.q_heads + hpw - 1) / hpw + (p.k_heads + hpw - 1) / hpw;
+  const int want = std::max(1, std::min(p.rounds, (32 * 148 + p.rows - 1) / p.rows));
+  p.rounds_per_warp = (p.rounds + want - 1) / want;
+  p.warps_per_row = (p.rounds + p.rounds_per_warp - 1) / p.rounds_per_warp;
   if ((long long)p.rows * p.warps_per_row / kRotaryWarps >= 0x7fffffffll)
     return fail(B2F_ERR_ARG, "rotary: too many rows");
   cudaStream_t s = (cudaStream_t)stream;

@@ -73,6 +73,7 @@ def test_rotary_refusals():
     _refuses(f, a, "out_scale", out_scale=0.0)
     _refuses(f, a, "e4m3 output", out_scale=0.5)
     _refuses(f, a, "go together", q_weight=4096)
+    _refuses(f, a, "weights must be", q_weight=4104, k_weight=4096)
     _refuses(f, a, "inverse", q_weight=4096, k_weight=4096, inverse=1)
 
 
