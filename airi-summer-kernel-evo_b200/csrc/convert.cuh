@@ -46,6 +46,57 @@ __device__ __forceinline__ void load4(const char* base, long long off, float* x)
   unpack4<DT>(load_raw4<DT>(base, off), x);
 }
 
+// Sixteen elements (16-byte aligned) as they lie in memory.
+template <int DT>
+struct Raw16 {
+  static constexpr int kVecs = DT == kF32 ? 4 : DT == kE4M3 ? 1 : 2;
+  uint4 v[kVecs];
+};
+
+template <int DT>
+__device__ __forceinline__ Raw16<DT> load_raw16(const char* base, long long off) {
+  Raw16<DT> r;
+  const uint4* p = reinterpret_cast<const uint4*>(base + off * Raw16<DT>::kVecs);
+#pragma unroll
+  for (int i = 0; i < Raw16<DT>::kVecs; ++i) r.v[i] = p[i];
+  return r;
+}
+
+template <int DT>
+__device__ __forceinline__ void unpack16(const Raw16<DT>& r, float* x) {
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(&r);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    Raw4<DT> q;
+    if constexpr (DT == kF32)
+      q.v = make_float4(__uint_as_float(w[4 * i]), __uint_as_float(w[4 * i + 1]), __uint_as_float(w[4 * i + 2]),
+                        __uint_as_float(w[4 * i + 3]));
+    else if constexpr (DT == kE4M3)
+      q.v = w[i];
+    else
+      q.v = make_uint2(w[2 * i], w[2 * i + 1]);
+    unpack4<DT>(q, x + 4 * i);
+  }
+}
+
+// Sixteen elements to f32, bf16 or f16, 16-byte aligned.
+template <int DT>
+__device__ __forceinline__ void store16(char* base, long long off, const float* x) {
+  if constexpr (DT == kF32) {
+    float4* p = reinterpret_cast<float4*>(base + off * 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) p[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+  } else {
+    uint4* p = reinterpret_cast<uint4*>(base + off * 2);
+    uint32_t w[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      w[i] = DT == kBF16 ? pack_bf16x2(x[2 * i], x[2 * i + 1]) : pack_f16x2(x[2 * i], x[2 * i + 1]);
+    p[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    p[1] = make_uint4(w[4], w[5], w[6], w[7]);
+  }
+}
+
 // Round-to-nearest-even; e4m3 saturates.
 template <int DT>
 __device__ __forceinline__ void store4(char* base, long long off, const float* x) {

@@ -75,15 +75,19 @@ __device__ __forceinline__ Kv4Seq kv4_seq(const Kv4Cache& c, const Kv4Batch& bt,
   return s;
 }
 
-// The sequence of packed token t, -1 for a row behind the last sequence.
+// The sequence of packed token t, -1 for a row outside of all sequences.  All lanes of a warp ask
+// for the same token; each round probes 32 places, so that 1024 sequences take two.
 __device__ __forceinline__ int kv4_owner(const Kv4Batch& bt, int t) {
   if (bt.starts == nullptr) return t / bt.each;
-  if (t >= bt.starts[bt.seqs] || t < bt.starts[0]) return -1;
-  int lo = 0, hi = bt.seqs;  // starts[lo] <= t < starts[hi]
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (bt.starts[mid] <= t) lo = mid;
-    else hi = mid;
+  const int lane = threadIdx.x & 31;
+  int lo = 0, n = bt.seqs;  // starts[lo] <= t < starts[lo + n], if t is in a sequence at all
+  if (t < bt.starts[0] || t >= bt.starts[bt.seqs]) return -1;
+  while (n > 1) {
+    const int step = (n + 31) >> 5, at = lane * step;
+    const unsigned below = __ballot_sync(0xffffffffu, at < n && bt.starts[lo + at] <= t);
+    const int k = below == 0 ? 0 : 31 - __clz(below);
+    lo += k * step;
+    n = min(step, n - k * step);
   }
   return lo;
 }

@@ -68,6 +68,7 @@ struct Kv4MoveParams {
   long long k_ld, v_ld;
   float k_in, v_in;
   int warps_per_token;
+  int groups_log2;  // of the groups of 16 of a head
 };
 
 constexpr int kMoveWarps = 4;
@@ -83,65 +84,87 @@ __device__ __forceinline__ uint32_t e2m1x8(const float* y) {
   return r;
 }
 
-// Where group g of a token lies: its part of the block, and the element it starts at.
+// Where group g of a token lies: K (0) or V (1), the kv head, the group within the head.
 struct Kv4Group {
-  int part, head, in_head;  // part 0: K, 1: V
+  int part, head, in_head;
 };
-__device__ __forceinline__ Kv4Group kv4_group(const Kv4Cache& c, int g) {
-  const int per = c.head_dim >> 4, half = c.kv_heads * per;
+__device__ __forceinline__ Kv4Group kv4_group(const Kv4MoveParams& p, int g) {
+  const int half = p.c.kv_heads << p.groups_log2;
   Kv4Group r;
   r.part = g >= half;
   const int x = g - (r.part ? half : 0);
-  r.head = x / per;
-  r.in_head = x - r.head * per;
+  r.head = x >> p.groups_log2;
+  r.in_head = x & ((1 << p.groups_log2) - 1);
   return r;
+}
+__device__ __forceinline__ long long kv4_element(const Kv4MoveParams& p, int t, const Kv4Group& at) {
+  return (long long)t * (at.part ? p.v_ld : p.k_ld) + at.head * p.c.head_dim + at.in_head * 16;
+}
+__device__ __forceinline__ uint8_t* kv4_block(const Kv4Cache& c, int page, const Kv4Group& at) {
+  return c.storage + (long long)page * c.page_stride + (long long)at.head * c.block_bytes +
+         at.part * (c.codes_bytes + c.scales_bytes);
 }
 
 template <int DT>
 __global__ void __launch_bounds__(32 * kMoveWarps) kv4_write_kernel(const Kv4MoveParams p) {
+  constexpr int N = DT == kF32 ? 2 : 4;  // groups of a lane in flight
   pdl_wait();
   pdl_trigger();
   const long long w = (long long)blockIdx.x * kMoveWarps + (threadIdx.x >> 5);
   const int t = int(w / p.warps_per_token);
   if (t >= p.b.tokens) return;
+  const Kv4Cache& c = p.c;
+  const int groups = 2 * c.kv_heads << p.groups_log2, step = 32 * p.warps_per_token;
+  int g0 = int(w - (long long)t * p.warps_per_token) * 32 + (threadIdx.x & 31);
+  Raw16<DT> raw[N];
+  auto load = [&]() {
+#pragma unroll
+    for (int u = 0; u < N; ++u)
+      if (g0 + u * step < groups) {
+        const Kv4Group at = kv4_group(p, g0 + u * step);
+        raw[u] = load_raw16<DT>(at.part ? p.v : p.k, kv4_element(p, t, at));
+      }
+  };
+  load();  // in flight while the token's place is looked up
   int slot;
   const int page = kv4_place(p.c, p.b, t, slot);
   if (page < 0) return;
-  const Kv4Cache& c = p.c;
-  const int groups = 2 * c.kv_heads * (c.head_dim >> 4);
-  const int lane = int(w % p.warps_per_token) * 32 + (threadIdx.x & 31);
-  uint8_t* to = c.storage + (long long)page * c.page_stride;
-  for (int g = lane; g < groups; g += 32 * p.warps_per_token) {
-    const Kv4Group at = kv4_group(c, g);
-    const char* src = at.part ? p.v : p.k;
-    const long long e = (long long)t * (at.part ? p.v_ld : p.k_ld) + at.head * c.head_dim + at.in_head * 16;
-    float x[16];
+  while (true) {
 #pragma unroll
-    for (int i = 0; i < 16; i += 4) load4<DT>(src, e + i, x + i);
-    const float in = at.part ? p.v_in : p.k_in, scale = at.part ? c.v_scale : c.k_scale;
-    float top = 0.f;
-    bool nan = false;
+    for (int u = 0; u < N; ++u) {
+      if (g0 + u * step >= groups) break;
+      const Kv4Group at = kv4_group(p, g0 + u * step);
+      float x[16];
+      unpack16<DT>(raw[u], x);
+      const float in = at.part ? p.v_in : p.k_in, scale = at.part ? c.v_scale : c.k_scale;
+      float top = 0.f;
+      bool nan = false;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      x[i] *= in;
-      nan |= x[i] != x[i];
-      top = fmaxf(top, fabsf(x[i]));
+      for (int i = 0; i < 16; ++i) {
+        x[i] *= in;
+        nan |= x[i] != x[i];
+        top = fmaxf(top, fabsf(x[i]));
+      }
+      if (nan) top = __int_as_float(0x7fc00000);
+      const uint16_t s8 = f32x2_to_e4m3x2(__fdiv_rn(top, 6.0f * scale), 0.f) & 0xff;
+      const float s = e4m3_to_f32(uint8_t(s8)) * scale;
+      const bool some = s > 0.f;  // false for NaN too
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] = some ? __fdiv_rn(x[i], s) : 0.f;
+      uint8_t* block = kv4_block(c, page, at);
+      *reinterpret_cast<uint2*>(block + slot * (c.head_dim >> 1) + at.in_head * 8) =
+          make_uint2(e2m1x8(x), e2m1x8(x + 8));
+      block[c.codes_bytes + slot * (c.head_dim >> 4) + at.in_head] = uint8_t(s8);
     }
-    if (nan) top = __int_as_float(0x7fc00000);
-    const uint16_t s8 = f32x2_to_e4m3x2(__fdiv_rn(top, 6.0f * scale), 0.f) & 0xff;
-    const float s = e4m3_to_f32(uint8_t(s8)) * scale;
-    const bool some = s > 0.f;  // false for NaN too
-#pragma unroll
-    for (int i = 0; i < 16; ++i) x[i] = some ? __fdiv_rn(x[i], s) : 0.f;
-    uint8_t* block = to + (long long)at.head * c.block_bytes + at.part * (c.codes_bytes + c.scales_bytes);
-    *reinterpret_cast<uint2*>(block + slot * (c.head_dim >> 1) + at.in_head * 8) =
-        make_uint2(e2m1x8(x), e2m1x8(x + 8));
-    block[c.codes_bytes + slot * (c.head_dim >> 4) + at.in_head] = uint8_t(s8);
+    g0 += N * step;
+    if (g0 >= groups) return;
+    load();
   }
 }
 
 template <int DT>
 __global__ void __launch_bounds__(32 * kMoveWarps) kv4_read_kernel(const Kv4MoveParams p) {
+  constexpr int N = 4;  // groups of a lane in flight
   pdl_wait();
   pdl_trigger();
   const long long w = (long long)blockIdx.x * kMoveWarps + (threadIdx.x >> 5);
@@ -151,35 +174,40 @@ __global__ void __launch_bounds__(32 * kMoveWarps) kv4_read_kernel(const Kv4Move
   const int page = kv4_place(p.c, p.b, t, slot);
   if (page == -2) return;
   const Kv4Cache& c = p.c;
-  const int groups = 2 * c.kv_heads * (c.head_dim >> 4);
-  const int lane = int(w % p.warps_per_token) * 32 + (threadIdx.x & 31);
-  const uint8_t* from = c.storage + (page < 0 ? 0ll : (long long)page * c.page_stride);
-  for (int g = lane; g < groups; g += 32 * p.warps_per_token) {
-    const Kv4Group at = kv4_group(c, g);
-    const uint8_t* block = from + (long long)at.head * c.block_bytes + at.part * (c.codes_bytes + c.scales_bytes);
-    uint2 codes = make_uint2(0, 0);
-    float s = 0.f;
-    if (page >= 0) {
-      codes = *reinterpret_cast<const uint2*>(block + slot * (c.head_dim >> 1) + at.in_head * 8);
-      s = e4m3_to_f32(block[c.codes_bytes + slot * (c.head_dim >> 4) + at.in_head]) *
-          (at.part ? c.v_scale : c.k_scale);
-    }
-    float x[16];
+  const int groups = 2 * c.kv_heads << p.groups_log2, step = 32 * p.warps_per_token;
+  for (int g0 = int(w - (long long)t * p.warps_per_token) * 32 + (threadIdx.x & 31); g0 < groups; g0 += N * step) {
+    uint2 codes[N];
+    uint8_t s8[N];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      uint32_t f[4];
-      e2m1x8_to_f16x2(h ? codes.y : codes.x, f);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 v = unpack_f16x2(f[i]);
-        x[8 * h + 2 * i] = v.x * s;
-        x[8 * h + 2 * i + 1] = v.y * s;
+    for (int u = 0; u < N; ++u) {
+      codes[u] = make_uint2(0, 0);
+      s8[u] = 0;
+      if (page >= 0 && g0 + u * step < groups) {
+        const Kv4Group at = kv4_group(p, g0 + u * step);
+        const uint8_t* block = kv4_block(c, page, at);
+        codes[u] = *reinterpret_cast<const uint2*>(block + slot * (c.head_dim >> 1) + at.in_head * 8);
+        s8[u] = block[c.codes_bytes + slot * (c.head_dim >> 4) + at.in_head];
       }
     }
-    char* dst = at.part ? p.v_out : p.k_out;
-    const long long e = (long long)t * (at.part ? p.v_ld : p.k_ld) + at.head * c.head_dim + at.in_head * 16;
 #pragma unroll
-    for (int i = 0; i < 16; i += 4) store4<DT>(dst, e + i, x + i);
+    for (int u = 0; u < N; ++u) {
+      if (g0 + u * step >= groups) break;
+      const Kv4Group at = kv4_group(p, g0 + u * step);
+      const float s = e4m3_to_f32(s8[u]) * (at.part ? c.v_scale : c.k_scale);
+      float x[16];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t f[4];
+        e2m1x8_to_f16x2(h ? codes[u].y : codes[u].x, f);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 v = unpack_f16x2(f[i]);
+          x[8 * h + 2 * i] = v.x * s;
+          x[8 * h + 2 * i + 1] = v.y * s;
+        }
+      }
+      store16<DT>(at.part ? p.v_out : p.k_out, kv4_element(p, t, at), x);
+    }
   }
 }
 
@@ -199,6 +227,7 @@ const char* prepare_move(const b2f_kv4_cache& c, const b2f_kv4_batch& b, const v
     return "tensors must be 16-byte aligned";
   p->k_ld = k_ld;
   p->v_ld = v_ld;
+  p->groups_log2 = c.head_dim == 64 ? 2 : c.head_dim == 128 ? 3 : 4;
   // A warp a token once there are enough of them (8 for each of 148 SMs); fewer tokens have
   // their groups dealt to more warps, one round of 32 groups at the least.
   const int rounds = (int)((2 * cols / 16 + 31) / 32);
