@@ -92,15 +92,34 @@ __device__ __forceinline__ int kv4_owner(const Kv4Batch& bt, int t) {
   return lo;
 }
 
-// Page and slot of packed token t; page -1 where it has none, -2 behind the last sequence.
+// Page and slot of packed token t (the same for all lanes of a warp); page -1 where it has none,
+// -2 outside of all sequences.
 __device__ __forceinline__ int kv4_place(const Kv4Cache& c, const Kv4Batch& bt, int t, int& slot) {
   slot = 0;
-  const int b = kv4_owner(bt, t);
-  if (b < 0) return -2;
-  const Kv4Seq s = kv4_seq(c, bt, b);
-  if (s.row < 0 || s.n == 0) return -1;
+  Kv4Seq s;
+  if (bt.starts != nullptr && bt.seqs < 32) {
+    // every lane looks up one sequence, so that the lookups do not wait for the search
+    const int lane = threadIdx.x & 31;
+    const int start = lane <= bt.seqs ? bt.starts[lane] : 0x7fffffff;
+    int row = lane < bt.seqs ? (bt.rows != nullptr ? bt.rows[lane] : lane) : -1;
+    if (row >= c.table_rows) row = -1;
+    const int len = row >= 0 ? c.lens[row] : 0;
+    const unsigned below = __ballot_sync(0xffffffffu, start <= t);
+    const int b = below == 0 ? -1 : 31 - __clz(below);
+    if (b < 0 || b >= bt.seqs) return -2;
+    s.start = __shfl_sync(0xffffffffu, start, b);
+    s.n = __shfl_sync(0xffffffffu, start, b + 1) - s.start;
+    s.row = __shfl_sync(0xffffffffu, row, b);
+    s.len = __shfl_sync(0xffffffffu, len, b);
+  } else {
+    const int b = kv4_owner(bt, t);
+    if (b < 0) return -2;
+    s = kv4_seq(c, bt, b);
+    if (s.row >= 0) s.len = c.lens[s.row];
+  }
   const int pos = s.len - s.n + (t - s.start);
-  if (pos < 0 || t - s.start >= s.n) {
+  if (s.row < 0 || pos < 0 || t < s.start || t - s.start >= s.n ||
+      s.len > (long long)c.table_cols << c.page_log2) {
     record_error(kDevBadArgs);
     return -1;
   }

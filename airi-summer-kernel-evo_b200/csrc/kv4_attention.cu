@@ -49,8 +49,6 @@ namespace {
 constexpr int kWarps = 4;                 // that work on keys; one more fetches them
 constexpr int kWork = 32 * kWarps;
 constexpr int kThreads = kWork + 32;
-constexpr int kChunk = 32;                // keys of a warp's step
-constexpr int kUnit = kChunk * kWarps;    // keys of a unit of work, and of a stage of the ring
 constexpr float kLift = 7.0f;             // P is scaled by 2^7 ...
 constexpr float kSlack = 8.0f;            // ... and the maximum may lag behind by 2^8
 
@@ -73,6 +71,7 @@ struct Kv4AttnParams {
   const char* gate;
   int gate_dtype;
   long long gate_ld, gate_hstride;
+  int gate_aligned;  // four neighbouring gates can be loaded at once
   float gate_scale;
   char* out;
   int out_dtype;
@@ -104,15 +103,16 @@ __device__ __forceinline__ int tile_keys(const Kv4AttnParams& p, const Kv4Seq& s
   return max(s.len - s.n + last + 1, 0);
 }
 
-__device__ __forceinline__ int units_of(int keys) { return (keys + kUnit - 1) / kUnit; }
+template <int U>
+__device__ __forceinline__ int units_of(int keys) { return (keys + U - 1) / U; }
 
 // Units of one kv head of a sequence.
-template <int R>
+template <int R, int U>
 __device__ __forceinline__ long long seq_units(const Kv4AttnParams& p, const Kv4Seq& s) {
   const int rts = (s.n * p.group + R - 1) / R;
-  if (!p.causal || rts <= 1) return rts == 0 ? 0 : (long long)rts * units_of(tile_keys<R>(p, s, 0));
+  if (!p.causal || rts <= 1) return rts == 0 ? 0 : (long long)rts * units_of<U>(tile_keys<R>(p, s, 0));
   long long u = 0;
-  for (int rt = 0; rt < rts; ++rt) u += units_of(tile_keys<R>(p, s, rt));
+  for (int rt = 0; rt < rts; ++rt) u += units_of<U>(tile_keys<R>(p, s, rt));
   return u;
 }
 
@@ -165,7 +165,7 @@ __device__ __forceinline__ long long scan_round(long long mine, long long& befor
 
 // This CTA's run of units [u0, u1), with the sequence of u0 in sc.b and the units before it in
 // sc.at.  `blank`: this CTA has to look after sequences with rows that see no key.
-template <int R>
+template <int R, int U>
 __device__ __forceinline__ Runs find_run(const Kv4AttnParams& p, Scan& sc, long long& u0, long long& u1, bool& blank) {
   long long before = 0, mine = 0, start = 0;
   bool empty = false;
@@ -174,7 +174,7 @@ __device__ __forceinline__ Runs find_run(const Kv4AttnParams& p, Scan& sc, long 
     mine = 0;
     if (b < p.b.seqs) {
       const Kv4Seq s = kv4_seq(p.c, p.b, b);
-      mine = seq_units<R>(p, s) * p.c.kv_heads;
+      mine = seq_units<R, U>(p, s) * p.c.kv_heads;
       empty |= b % gridDim.x == blockIdx.x && s.n > 0 && tile_keys<R>(p, s, 0) <= 0;
     }
     start = scan_round(mine, before, sc);
@@ -191,7 +191,7 @@ __device__ __forceinline__ Runs find_run(const Kv4AttnParams& p, Scan& sc, long 
     before = 0;
     for (int base = 0; base < p.b.seqs; base += kThreads) {
       const int b = base + (int)threadIdx.x;
-      mine = b < p.b.seqs ? seq_units<R>(p, kv4_seq(p.c, p.b, b)) * p.c.kv_heads : 0;
+      mine = b < p.b.seqs ? seq_units<R, U>(p, kv4_seq(p.c, p.b, b)) * p.c.kv_heads : 0;
       start = scan_round(mine, before, sc);
       if (u0 >= start && u0 < start + mine) {
         sc.b = b;
@@ -203,23 +203,23 @@ __device__ __forceinline__ Runs find_run(const Kv4AttnParams& p, Scan& sc, long 
   return runs;
 }
 
-template <int R>
+template <int R, int U>
 __device__ __forceinline__ void open_item(const Kv4AttnParams& p, Item& it) {
   it.keys = tile_keys<R>(p, it.s, it.rt);
-  it.units = units_of(it.keys);
+  it.units = units_of<U>(it.keys);
 }
 
 // The item of unit `unit` of sequence b, and the unit's place in it.
-template <int R>
+template <int R, int U>
 __device__ int find_item(const Kv4AttnParams& p, int b, long long unit, Item& it) {
   it.b = b;
   it.s = kv4_seq(p.c, p.b, b);
   it.rts = (it.s.n * p.group + R - 1) / R;
-  const long long per = seq_units<R>(p, it.s);
+  const long long per = seq_units<R, U>(p, it.s);
   it.h = (int)divide(unit, per);
   long long rest = unit - it.h * per;
   for (it.rt = 0;; ++it.rt) {
-    open_item<R>(p, it);
+    open_item<R, U>(p, it);
     if (rest < it.units || it.rt + 1 >= it.rts) break;
     rest -= it.units;
   }
@@ -227,7 +227,7 @@ __device__ int find_item(const Kv4AttnParams& p, int b, long long unit, Item& it
 }
 
 // The next item that has units.  There is one: the caller still has units to do.
-template <int R>
+template <int R, int U>
 __device__ void next_item(const Kv4AttnParams& p, Item& it) {
   do {
     if (++it.rt >= it.rts) {
@@ -245,7 +245,7 @@ __device__ void next_item(const Kv4AttnParams& p, Item& it) {
         } while (it.rts == 0);
       }
     }
-    open_item<R>(p, it);
+    open_item<R, U>(p, it);
   } while (it.units == 0);
 }
 
@@ -339,22 +339,9 @@ __device__ __forceinline__ int row_token(const Kv4AttnParams& p, int row, int h,
   return i < n ? start + i : -1;
 }
 
-// Normalises, gates and stores `n` neighbouring elements (o, unnormalised) of one row.
 template <int N>
-__device__ __forceinline__ void finish_row(const Kv4AttnParams& p, int t, int head, int d0, const float* o,
-                                           float sum) {
-  const float inv = sum > 0.f || sum != sum ? 1.0f / sum : 0.f;
+__device__ __forceinline__ void store_row(const Kv4AttnParams& p, int t, int head, int d0, const float* x) {
   const long long at = (long long)t * p.out_ld + (long long)head * p.c.head_dim + d0;
-  float x[N];
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    x[i] = o[i] * inv * p.out_mul;
-    if (p.gate != nullptr) {
-      const float g = load1(p.gate, p.gate_dtype, (long long)t * p.gate_ld + head * p.gate_hstride + d0 + i) * p.gate_scale;
-      x[i] = x[i] / (1.0f + __expf(-g));
-    }
-    if (p.out_dtype == kE4M3) x[i] = __fdiv_rn(x[i], p.ctx_scale);
-  }
   if (N % 4 == 0) {
 #pragma unroll
     for (int i = 0; i < N; i += 4) {
@@ -370,6 +357,36 @@ __device__ __forceinline__ void finish_row(const Kv4AttnParams& p, int t, int he
   }
 }
 
+// Normalises, gates and stores N neighbouring elements (o, unnormalised) of one row.  A row that
+// saw no key (sum 0) is zeros, whatever its gate.
+template <int N>
+__device__ __forceinline__ void finish_row(const Kv4AttnParams& p, int t, int head, int d0, const float* o,
+                                           float sum) {
+  float x[N];
+  const float mul = p.out_mul / sum;
+#pragma unroll
+  for (int i = 0; i < N; ++i) x[i] = o[i] * mul;
+  if (p.gate != nullptr) {
+    const long long at = (long long)t * p.gate_ld + head * p.gate_hstride + d0;
+    float g[N];
+    if (N == 4 && p.gate_aligned) {
+      if (p.gate_dtype == kBF16) load4<kBF16>(p.gate, at, g);
+      else load4<kE4M3>(p.gate, at, g);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) g[i] = load1(p.gate, p.gate_dtype, at + i);
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = x[i] / (1.0f + __expf(-g[i] * p.gate_scale));
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (p.out_dtype == kE4M3) x[i] = __fdiv_rn(x[i], p.ctx_scale);
+    if (sum == 0.f) x[i] = 0.f;
+  }
+  store_row<N>(p, t, head, d0, x);
+}
+
 // log sum exp of a row: P was 2^(score * log2 e - ref), sum over the keys.
 __device__ __forceinline__ void finish_lse(const Kv4AttnParams& p, int t, int head, float ref, float sum) {
   if (p.lse == nullptr) return;
@@ -378,9 +395,11 @@ __device__ __forceinline__ void finish_lse(const Kv4AttnParams& p, int t, int he
                                          : sum != sum ? sum : -INFINITY;
 }
 
+// kChunk: keys of a step of a warp; kUnit: of a unit of work, and of a stage of the ring.
 template <int D, int NT, int STAGES>
 struct Layout {
   static constexpr int R = 8 * NT;
+  static constexpr int kChunk = D == 256 ? 16 : 32, kUnit = kChunk * kWarps;
   static constexpr int kStage = kUnit * D / 8 * 9;       // the blocks of a unit's pages, one after the other
   static constexpr int kRow = 64 + 4;                    // floats of a row of the join: 64 elements at a time
   static constexpr int kRing = STAGES * kStage;
@@ -400,7 +419,8 @@ struct Piece {
 template <int D, int NT, int STAGES, int CTAS>
 __global__ void __launch_bounds__(kThreads, CTAS) kv4_attention_kernel(const Kv4AttnParams p) {
   using L = Layout<D, NT, STAGES>;
-  constexpr int R = L::R;
+  constexpr int R = L::R, U = L::kUnit, kUnit = U, kChunk = L::kChunk;
+  constexpr int G = kChunk / 16;            // sixteens of keys of a step
   constexpr int kTiles = D / 16;            // m16 tiles of O^T
   constexpr int kRuns = D == 256 ? 2 : 1;   // runs of neighbouring K codes of a thread and key
   constexpr int kWordsK = D / 32 / kRuns;   // 32-bit words of a run: two steps each
@@ -435,7 +455,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) kv4_attention_kernel(const Kv4
 
   long long u0, u1;
   bool blank;
-  const Runs runs = find_run<R>(p, sc, u0, u1, blank);
+  const Runs runs = find_run<R, U>(p, sc, u0, u1, blank);
   // rows that see no key at all: zeros
   for (int b = blockIdx.x; blank && b < p.b.seqs; b += gridDim.x) {
     Item it;
@@ -445,13 +465,12 @@ __global__ void __launch_bounds__(kThreads, CTAS) kv4_attention_kernel(const Kv4
     for (it.rt = 0; it.rt < it.rts; ++it.rt) {
       if (tile_keys<R>(p, it.s, it.rt) > 0) break;  // later tiles see more
       for (int x = threadIdx.x; x < p.c.kv_heads * R * (D / 4); x += kThreads) {
-        it.h = x / (R * (D / 4));
-        const int y = x - it.h * (R * (D / 4));
+        const int h = x / (R * (D / 4)), y = x - h * (R * (D / 4));
         int head;
-        const int t = row_token(p, it.rt * R + y / (D / 4), it.h, it.s.start, it.s.n, head);
+        const int t = row_token(p, it.rt * R + y / (D / 4), h, it.s.start, it.s.n, head);
         const float zero[4] = {0.f, 0.f, 0.f, 0.f};
         if (t >= 0) {
-          finish_row<4>(p, t, head, (y % (D / 4)) * 4, zero, 0.f);
+          store_row<4>(p, t, head, (y % (D / 4)) * 4, zero);
           if (y % (D / 4) == 0) finish_lse(p, t, head, 0.f, 0.f);
         }
       }
@@ -467,7 +486,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) kv4_attention_kernel(const Kv4
   if (warp == kWarps) {
     // ---- the fetching warp: a lane for each page of a unit; the block of a head is one piece
     Item it;
-    int first = find_item<R>(p, sc.b, u0 - sc.at, it);
+    int first = find_item<R, U>(p, sc.b, u0 - sc.at, it);
     long long left = u1 - u0;
     const bool copies = lane < (kUnit >> log2p);
     const uint64_t policy = policy_evict_normal();
@@ -578,7 +597,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) kv4_attention_kernel(const Kv4
       }
       left -= take;
       if (left > 0) {
-        next_item<R>(p, it);
+        next_item<R, U>(p, it);
         first = 0;
       }
     }
@@ -601,14 +620,14 @@ __global__ void __launch_bounds__(kThreads, CTAS) kv4_attention_kernel(const Kv4
   }
 
   // Where the warp's codes and scales lie in a stage (of K; those of V are v_part behind), and how
-  // far the second 16 of its 32 keys are from the first; the bits of their pages in stage_ok.
+  // far a second 16 of its keys are from the first; the bits of their pages in stage_ok.
   const int page0 = (warp * kChunk) >> log2p, slot0 = (warp * kChunk) & (p.c.page_size - 1);
   const int codes_at = page0 * p.c.block_bytes + slot0 * (D / 2);
   const int scales_at = page0 * p.c.block_bytes + p.c.codes_bytes + slot0 * (D / 16);
   const int v_part = p.c.codes_bytes + p.c.scales_bytes;
   const int codes_2nd = log2p == 4 ? p.c.block_bytes : 16 * (D / 2);
   const int scales_2nd = log2p == 4 ? p.c.block_bytes : 16 * (D / 16);
-  const int page1 = page0 + (log2p == 4 ? 1 : 0);
+  const int page1 = page0 + (log2p == 4 && G == 2 ? 1 : 0);
   const unsigned mine = 1u << page0 | 1u << page1;
 
   for (;;) {
@@ -655,14 +674,14 @@ __global__ void __launch_bounds__(kThreads, CTAS) kv4_attention_kernel(const Kv4
         const uint8_t* ks = smem + stage * L::kStage + scales_at;
         const unsigned okay = stage_ok[stage];
         const bool edge = key0 + kChunk > lowest || (okay & mine) != mine;
-        // ---- S^T: two times 16 keys x R rows
-        float s[2][NT][4];
+        // ---- S^T: 16 keys x R rows, G times
+        float s[G][NT][4];
         const int kr = (r >> 1) + (r & 1) * 4;  // key of slot r (of the first 16); slot r + 8: kr + 8
 #pragma unroll
         for (int i = 0; i < kRuns; ++i) {
-          uint32_t w[4][kWordsK], m[4];  // codes of the keys kr + 8 k, scales of two groups as f16
+          uint32_t w[2 * G][kWordsK], m[2 * G];  // codes of the keys kr + 8 k, scales of two groups as f16
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
+          for (int k = 0; k < 2 * G; ++k) {
             const int key = kr + 8 * (k & 1);
             const uint8_t* codes = kc + (k >= 2 ? codes_2nd : 0);
             const uint8_t* scales = ks + (k >= 2 ? scales_2nd : 0);
@@ -682,7 +701,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) kv4_attention_kernel(const Kv4
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) q[nt] = q_frag[buf][(nt * kRuns + i) * kWordsK + x][lane];
 #pragma unroll
-            for (int g = 0; g < 2; ++g) {
+            for (int g = 0; g < G; ++g) {
               uint32_t f0[4], f1[4];
               e2m1x8_to_f16x2(w[2 * g][x], f0);
               e2m1x8_to_f16x2(w[2 * g + 1][x], f1);
@@ -701,11 +720,11 @@ __global__ void __launch_bounds__(kThreads, CTAS) kv4_attention_kernel(const Kv4
           }
         }
         // ---- scores to P
-        float x[2][NT][4];
+        float x[G][NT][4];
         unsigned hidden = 0;  // bit (g * NT + nt) * 4 + j: the row does not see the key
         if (edge) {
 #pragma unroll
-          for (int g = 0; g < 2; ++g)
+          for (int g = 0; g < G; ++g)
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -719,7 +738,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) kv4_attention_kernel(const Kv4
         }
         float top = -INFINITY;
 #pragma unroll
-        for (int g = 0; g < 2; ++g)
+        for (int g = 0; g < G; ++g)
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -733,7 +752,9 @@ __global__ void __launch_bounds__(kThreads, CTAS) kv4_attention_kernel(const Kv4
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-              float m = fmaxf(fmaxf(s[0][nt][j], s[0][nt][j + 2]), fmaxf(s[1][nt][j], s[1][nt][j + 2])) * mul[nt][j];
+              float m = fmaxf(s[0][nt][j], s[0][nt][j + 2]);
+              if (G == 2) m = fmax3(m, s[G - 1][nt][j], s[G - 1][nt][j + 2]);
+              m *= mul[nt][j];
               m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
               m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
               m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
@@ -747,7 +768,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) kv4_attention_kernel(const Kv4
                 o[t][nt][j + 2] *= f;
               }
 #pragma unroll
-              for (int g = 0; g < 2; ++g) {
+              for (int g = 0; g < G; ++g) {
                 x[g][nt][j] = fmaf(s[g][nt][j], mul[nt][j], -m);
                 x[g][nt][j + 2] = fmaf(s[g][nt][j + 2], mul[nt][j], -m);
               }
@@ -755,7 +776,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) kv4_attention_kernel(const Kv4
         }
         if (edge) {
 #pragma unroll
-          for (int g = 0; g < 2; ++g)
+          for (int g = 0; g < G; ++g)
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -763,7 +784,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) kv4_attention_kernel(const Kv4
                 if (hidden >> ((g * NT + nt) * 4 + j) & 1) x[g][nt][j] = -INFINITY;
         }
 #pragma unroll
-        for (int g = 0; g < 2; ++g)
+        for (int g = 0; g < G; ++g)
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -776,7 +797,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) kv4_attention_kernel(const Kv4
           // the last, or of tokens that only later rows see) count as 0 below, and a row that
           // does see a NaN gets it through P.
 #pragma unroll
-          for (int g = 0; g < 2; ++g)
+          for (int g = 0; g < G; ++g)
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
               const uint8_t* row = ks + v_part + (g ? scales_2nd : 0) + (kr + j * 8) * (D / 16);
@@ -792,7 +813,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) kv4_attention_kernel(const Kv4
         }
         // ---- O^T += V^T P^T
 #pragma unroll
-        for (int g = 0; g < 2; ++g) {
+        for (int g = 0; g < G; ++g) {
           uint32_t pf[NT][2];
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
@@ -1090,6 +1111,8 @@ int b2f_kv4_attention(const b2f_kv4_attn_args* a, b2f_stream_t stream) {
   p.scale_log2 = sm * a->q_scale * a->cache.k_scale * 1.4426950408889634f;
   p.out_mul = a->cache.v_scale;
   p.gate = reinterpret_cast<const char*>(a->gate); p.gate_dtype = a->gate_dtype;
+  const int four = a->gate_dtype == B2F_DTYPE_BF16 ? 8 : 4;
+  p.gate_aligned = reinterpret_cast<uintptr_t>(a->gate) % four == 0 && a->gate_ld % 4 == 0 && a->gate_head_stride % 4 == 0;
   p.gate_ld = a->gate_ld; p.gate_hstride = a->gate_head_stride; p.gate_scale = a->gate_scale;
   p.out = reinterpret_cast<char*>(a->out); p.out_dtype = a->out_dtype; p.out_ld = a->out_ld;
   p.ctx_scale = a->ctx_scale; p.lse = a->lse;
@@ -1100,7 +1123,7 @@ int b2f_kv4_attention(const b2f_kv4_attn_args* a, b2f_stream_t stream) {
   const int rows = tile_rows(d, most * p.group);
   if (d == 64) return rows == 8 ? launch_attention<64, 1, 4, 3>(p, s) : launch_attention<64, 2, 4, 2>(p, s);
   if (d == 128) return rows == 8 ? launch_attention<128, 1, 3, 3>(p, s) : launch_attention<128, 2, 3, 2>(p, s);
-  return launch_attention<256, 1, 2, 2>(p, s);
+  return launch_attention<256, 1, 3, 3>(p, s);
 }
 
 }  // extern "C"
