@@ -429,6 +429,51 @@ class QwenBlock(_Graphable):
         _mark(marks, "mlp")
         return self.out
 
+    def step(self, hidden: torch.Tensor, cache, plan, *, positions: torch.Tensor, layer: int = 0,
+             rows: Optional[torch.Tensor] = None, starts: Optional[torch.Tensor] = None,
+             hidden_scale: float = 1.0) -> torch.Tensor:
+        """The block over the new tokens of any number of sequences, single tokens or chunks of
+        prompts, with the keys and values of all earlier tokens in ``cache``
+        (:class:`b200fp8.kvcache.Fp4Cache`, extended by these tokens already) as layer ``layer``.
+
+        ``hidden`` [tokens, hidden] and ``positions`` int32 [tokens] are packed as ``starts`` and
+        ``rows`` say (see :meth:`Fp4Cache.write`); ``plan`` is the
+        :class:`b200fp8.rotary.RotaryPlan` of the block's rotary_dim.  The stages and their
+        quantisation points are those of :meth:`forward`, except that keys and values are read
+        back from the 4-bit cache.  Nothing depends on the block's own batch and seq."""
+        h, hk, dh = self.h, self.hk, self.dh
+        if plan.head_dim != dh or plan.rotary_dim != self.rot or plan.interleaved:
+            raise ValueError("the plan must have the block's head_dim and rotary_dim, half layout")
+        if cache.kv_heads != hk or cache.head_dim != dh:
+            raise ValueError("the cache must have the block's kv_heads and head_dim")
+        if hidden.dim() != 2 or hidden.shape[1] != self.hidden:
+            raise ValueError(f"hidden must be [tokens, {self.hidden}]")
+        n1, _ = ops.norm_quant(hidden, self.in_norm, kind="rms", weight_offset=1.0, eps=self.eps,
+                               x_scale=hidden_scale, q_scale=self.ns)
+        proj = _gemm(n1, self.w_cat, col_scale=self.cs_cat, out_dtype=_E4M3, out_scale=self.qs)
+        q, k = ops.rotary(proj[:, self.q_off:], proj[:, self.k_off:], positions, plan, heads=h,
+                          kv_heads=hk, q_head_stride=self.q_hstride, in_scale=self.qs,
+                          q_weight=self.q_norm, k_weight=self.k_norm, weight_offset=1.0,
+                          eps=self.eps, out_dtype=_E4M3, out_scale=self.qs)
+        cache.write(k, proj[:, self.v_off:self.v_off + hk * dh], layer=layer, rows=rows,
+                    starts=starts, k_in_scale=self.qs, v_in_scale=self.qs)
+        ctx = cache.attention(q, heads=h, layer=layer, rows=rows, starts=starts, q_scale=self.qs,
+                              gate=proj[:, self.g_off:], gate_scale=self.qs,
+                              gate_head_stride=self.q_hstride, out_dtype=_E4M3,
+                              ctx_scale=self.cs)
+        r1 = _gemm(ctx, self.o_w, scale_a=self.cs, scale_b=self.o_s,
+                   residual=hidden if self.add_residual else None, residual_scale=hidden_scale,
+                   out_dtype=self.r1.dtype if self.has_mlp else self.out.dtype)
+        if not self.has_mlp:
+            return r1
+        n2, _ = ops.norm_quant(r1, self.post_norm, kind="rms", weight_offset=1.0, eps=self.eps,
+                               q_scale=self.ns)
+        gu = _gemm(n2, self.gu_w, col_scale=self.gu_cs, out_dtype=_E4M3, out_scale=self.mps)
+        act = ops.swiglu_fp8(gu[:, :self.inter], gu[:, self.inter:], in_scale=self.mps,
+                             out_scale=self.mas)
+        return _gemm(act, self.down_w, scale_a=self.mas, scale_b=self.down_s, residual=r1,
+                     out_dtype=self.out.dtype)
+
     def forward_abi(self, hidden: torch.Tensor, hidden_scale: float = 1.0) -> torch.Tensor:
         """The same forward through the native entry point b2f_qwen_block; writes and
         returns ``self.out``."""

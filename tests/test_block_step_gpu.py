@@ -1,0 +1,101 @@
+"""QwenBlock.step (chunks of prompts and single tokens over the 4-bit cache) against the block
+oracle whose keys and values went through the cache's format; the bar of the other block tests
+(0.08, plus one bf16 rounding of the output)."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from block_inputs import qwen_weights
+from helpers import gen
+from oracle import blocks as ob
+from oracle import serving
+
+pytestmark = pytest.mark.gpu
+
+
+def _ints(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_chunks_and_single_tokens_match_the_oracle(interleaved, monkeypatch):
+    from b200fp8 import blocks, device_status, kvcache, rotary
+    g = gen(77 + interleaved)
+    batch, seq, ks = 2, 48, 1 / 32
+    geo = (dict(hidden=512, heads=4, kv_heads=1, head_dim=256, rotary_dim=64, theta=1e7)
+           if interleaved else
+           dict(hidden=768, heads=8, kv_heads=2, head_dim=128, rotary_dim=128, theta=1e6))
+    w = qwen_weights(seq=seq, g=g, interleaved=interleaved, mlp=1024 if interleaved else 0,
+                     reference=interleaved, **geo)
+    x = torch.randn((batch * seq, geo["hidden"]), generator=g).to(torch.bfloat16)
+
+    plain = ob.oatt.attention
+    monkeypatch.setattr(ob.oatt, "attention", lambda q, k, v, **kw: plain(
+        q, serving.pack(k, ks)[2].float(), serving.pack(v, ks)[2].float(), **kw))
+    ref = ob.qwen_block(x.float(), w, batch=batch, residual_dtype=torch.bfloat16,
+                        out_dtype=torch.bfloat16)
+
+    blk = blocks.QwenBlock(w, batch=1, seq=seq, residual_dtype=torch.bfloat16,
+                           out_dtype=torch.bfloat16)
+    plan = rotary.RotaryPlan(geo["head_dim"], rotary_dim=geo["rotary_dim"], theta=geo["theta"],
+                             device="cuda")
+    cache = kvcache.Fp4Cache(layers=2, pages=16, page_size=16, kv_heads=geo["kv_heads"],
+                             head_dim=geo["head_dim"], max_seqs=3, max_pages=5, k_scale=ks,
+                             v_scale=ks)
+    rows = _ints([2, 0])
+    xd = x.cuda().view(batch, seq, -1)
+    out = torch.empty((batch, seq, geo["hidden"]), dtype=torch.bfloat16, device="cuda")
+    at = [0, 0]
+    for news in ([17, 40], [23, 1], [1, 1], [1, 1], [6, 5]):  # chunks and steps, uneven
+        starts = [0, news[0], sum(news)]
+        part = torch.cat([xd[b, at[b]:at[b] + n] for b, n in enumerate(news)])
+        pos = torch.cat([torch.arange(at[b], at[b] + n) for b, n in enumerate(news)]).int().cuda()
+        cache.extend(_ints(news), rows=rows)
+        got = blk.step(part, cache, plan, positions=pos, layer=1, rows=rows, starts=_ints(starts))
+        for b, n in enumerate(news):
+            out[b, at[b]:at[b] + n] = got[starts[b]:starts[b + 1]]
+            at[b] += n
+    assert at == [seq, seq]
+    torch.cuda.synchronize()
+    err = (out.view(batch * seq, -1).float().cpu() - ref).abs()
+    assert bool((err <= 0.08 + 2.0 ** -8 * ref.abs()).all()), float(err.max())
+    assert device_status() == 0
+
+    # a step captured in a graph, replayed on another token
+    one = xd[:, -1].contiguous()
+    pos = _ints([seq, seq])
+    cache.extend(_ints([1, 1]), rows=rows)
+    blk.step(one, cache, plan, positions=pos, layer=1, rows=rows)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = blk.step(one, cache, plan, positions=pos, layer=1, rows=rows)
+    one.copy_(xd[:, 3])
+    graph.replay()
+    want = blk.step(xd[:, 3].contiguous(), cache, plan, positions=pos, layer=1, rows=rows)
+    torch.cuda.synchronize()
+    assert torch.equal(y, want)
+
+
+def test_step_refusals():
+    from b200fp8 import blocks, kvcache, rotary
+    w = qwen_weights(seq=8, g=gen(1), interleaved=False, hidden=512, heads=4, kv_heads=1,
+                     head_dim=64, rotary_dim=64, theta=1e6)
+    blk = blocks.QwenBlock(w, batch=1, seq=8)
+    cache = kvcache.Fp4Cache(layers=1, pages=2, page_size=16, kv_heads=1, head_dim=64, max_seqs=1,
+                             max_pages=1)
+    pos, x = _ints([0]), torch.zeros((1, 512), device="cuda")
+    for plan in (rotary.RotaryPlan(128), rotary.RotaryPlan(64, rotary_dim=32),
+                 rotary.RotaryPlan(64, layout="interleaved")):
+        with pytest.raises(ValueError, match="plan"):
+            blk.step(x, cache, plan, positions=pos)
+    plan = rotary.RotaryPlan(64)
+    other = kvcache.Fp4Cache(layers=1, pages=2, page_size=16, kv_heads=2, head_dim=64, max_seqs=1,
+                             max_pages=1)
+    with pytest.raises(ValueError, match="cache"):
+        blk.step(x, other, plan, positions=pos)
+    with pytest.raises(ValueError, match="hidden"):
+        blk.step(x[:, :256], cache, plan, positions=pos)
+    with pytest.raises(ValueError, match="layer"):
+        blk.step(x, cache, plan, positions=pos, layer=1)
