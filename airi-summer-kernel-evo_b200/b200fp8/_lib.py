@@ -403,7 +403,7 @@ def _declare(lib: ctypes.CDLL) -> None:
         getattr(lib, f"b2f_{nm}").restype = ctypes.c_int
     lib.b2f_kv4_attn_args_init.argtypes = [ctypes.POINTER(Kv4AttnArgs)]
     lib.b2f_kv4_attn_args_init.restype = None
-    lib.b2f_kv4_attention_workspace_bytes.argtypes = [ctypes.c_int]
+    lib.b2f_kv4_attention_workspace_bytes.argtypes = [ctypes.POINTER(Kv4AttnArgs)]
     lib.b2f_kv4_attention_workspace_bytes.restype = ctypes.c_longlong
     lib.b2f_kv4_attention.argtypes = [ctypes.POINTER(Kv4AttnArgs), vp]
     lib.b2f_kv4_attention.restype = ctypes.c_int

@@ -87,8 +87,7 @@ class Fp4Cache:
         lib = _lib.lib()
         self._write, self._read, self._attention = (lib.b2f_kv4_write, lib.b2f_kv4_read,
                                                     lib.b2f_kv4_attention)
-        with torch.cuda.device(self._index):
-            self._work_ints = -(-int(lib.b2f_kv4_attention_workspace_bytes(head_dim)) // 4)
+        self._workspace = lib.b2f_kv4_attention_workspace_bytes
         c = _lib.Kv4Cache()
         c.storage, c.page_stride = storage.data_ptr(), storage.stride(1)
         c.pages, c.kv_heads = self.pages, self.kv_heads
@@ -252,8 +251,9 @@ class Fp4Cache:
         a.out, a.out_dtype, a.ctx_scale = out.data_ptr(), _DT[out.dtype], ctx_scale
         # A workspace of this call's own, from the caching allocator of the current stream: calls
         # on other streams, and in graphs, never share it.
-        work = self.lens.new_empty(self._work_ints)
-        a.workspace, a.workspace_bytes = work.data_ptr(), 4 * self._work_ints
+        ints = -(-self._workspace(a) // 4)
+        work = self.lens.new_empty(ints)
+        a.workspace, a.workspace_bytes = work.data_ptr(), 4 * ints
         self._run(self._attention, a)
         return (out, lse) if return_lse else out
 

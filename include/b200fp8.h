@@ -565,7 +565,8 @@ int b2f_kv4_read(const b2f_kv4_read_args* args, b2f_stream_t stream);
  *   [tokens, heads], the natural log of the sum of exp(score).  A token that sees no key gets
  *   zeros and -infinity.  A NaN or infinity in a key or value reaches no token that may not
  *   see it.  sm_scale <= 0 selects 1/sqrt(head_dim).
- *   workspace: b2f_kv4_attention_workspace_bytes(head_dim) bytes, 16-byte aligned, no zeroing;
+ *   workspace: b2f_kv4_attention_workspace_bytes(args) bytes (by cache, batch and heads; up to
+ *   40 MB for chunks of prompts), 16-byte aligned, no zeroing;
  *   calls that may run at the same time need one each.  Bitwise reproducible.
  * Next to b2f_attention_fp8, whose keys and values are the batch's own. */
 typedef struct b2f_kv4_attn_args {
@@ -591,7 +592,7 @@ typedef struct b2f_kv4_attn_args {
 } b2f_kv4_attn_args;
 
 void b2f_kv4_attn_args_init(b2f_kv4_attn_args* args);
-long long b2f_kv4_attention_workspace_bytes(int head_dim);
+long long b2f_kv4_attention_workspace_bytes(const b2f_kv4_attn_args* args); /* -1: no device */
 int b2f_kv4_attention(const b2f_kv4_attn_args* args, b2f_stream_t stream);
 
 /* The pages of all layers of a cache, and who uses them.  refs[p] counts the table rows that

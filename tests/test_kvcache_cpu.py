@@ -138,7 +138,7 @@ def test_cache_refusals(name):
     _refuses(f, a, "e4m3 output", ctx_scale=0.5)
     _refuses(f, a, "misaligned lse", lse=4097)
     if not torch.cuda.is_available():
-        assert lib.b2f_kv4_attention_workspace_bytes(128) == -1
+        assert lib.b2f_kv4_attention_workspace_bytes(ctypes.byref(a)) == -1
 
 
 def test_pool_refusals():

@@ -531,3 +531,101 @@ def test_a_served_sequence():
     step([1, 2, 3, 5], [1] * 4)
     assert int((c.refs > 0).nonzero().max()) < 64 - c.free_pages() + 4
     assert device_status() == 0
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("heads,kv,page", [(4, 1, 16), (8, 2, 64), (14, 2, 32)])
+def test_chunks_of_prompts(d, heads, kv, page):
+    """Chunks with enough rows for the tensor-core tiles: rows that end inside a tile, in one or
+    both tiles, sequences cut among CTAs, prefixes of all lengths, an empty sequence, a chunk that
+    is the whole sequence, every page size."""
+    g = gen(d + heads)
+    lens = [700, 130, 61, 0, 257, 1000, 128]
+    news = [90, 130, 61, 0, 33, 150, 1]
+    c, _, _, _ = _filled(lens, None, kv=kv, d=d, page=page, g=g, garbage=True)
+    starts = [0]
+    for n in news:
+        starts.append(starts[-1] + n)
+    q = randn((starts[-1], heads * d), g).to(BF16)
+    out, lse = c.attention(q.cuda(), heads=heads, starts=_ints(starts), return_lse=True)
+    again, _ = c.attention(q.cuda(), heads=heads, starts=_ints(starts), return_lse=True)
+    torch.cuda.synchronize()
+    assert torch.equal(out, again)
+    _check_attention(c, q, out, lens, starts, heads, lse=lse)
+
+
+@pytest.mark.parametrize("q_dtype,out_dtype", [(F16, BF16), (E4M3, E4M3)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_chunks_with_gate_types_and_uniform_lengths(q_dtype, out_dtype, causal):
+    g = gen(5 + causal)
+    lens, n, heads, d = [300, 50, 40], 48, 8, 128
+    c, _, _, _ = _filled(lens, None, kv=2, d=d, page=16, g=g, garbage=True)
+    qs = 1 / 64 if q_dtype == E4M3 else 1.0
+    q = (randn((3 * n, heads * d), g) / qs).clamp(-440, 440).to(q_dtype)
+    gate = (randn((3 * n, heads * d), g) * 64).clamp(-440, 440).to(E4M3)
+    outs = 1 / 256 if out_dtype == E4M3 else 1.0
+    out, lse = c.attention(q.cuda(), heads=heads, causal=causal, q_scale=qs, gate=gate.cuda(),
+                           gate_scale=1 / 64, out_dtype=out_dtype, ctx_scale=outs, return_lse=True)
+    torch.cuda.synchronize()
+    _check_attention(c, q, out, lens, [0, n, 2 * n, 3 * n], heads, causal=causal, q_scale=qs,
+                     gate=gate.float() / 64, out_scale=outs, lse=lse)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("which", ["k", "v"])
+def test_nan_in_a_chunk_reaches_only_those_who_see_it(d, which):
+    g = gen(d + 1)
+    lens = [200, 200]
+    c, k, v, starts = _filled(lens, None, kv=1, d=d, page=16, g=g)
+    k, v = k.clone(), v.clone()
+    (k if which == "k" else v)[150, 3] = float("nan")
+    c.write(k.cuda(), v.cuda(), starts=_ints(starts))
+    q = randn((200, 2 * d), g).to(BF16)
+    out = c.attention(q.cuda(), heads=2, starts=_ints([0, 100, 200]))
+    torch.cuda.synchronize()
+    clean = torch.isfinite(out).all(1).cpu().tolist()
+    assert clean == [True] * 50 + [False] * 50 + [True] * 100
+    assert bool(torch.isnan(out[50:100, :16]).all())
+    for b, lo, hi, seen in ((0, 0, 50, 150), (1, 100, 200, 200)):
+        kk, vv = _oracle_kv(c, b, 200)
+        want, _, mass, size = serving.attention(q[lo:hi].double().unflatten(-1, (2, d)),
+                                                kk[:seen], vv[:seen])
+        got = out[lo:hi].cpu().double().unflatten(-1, (2, d))
+        bound = mass * (2.0 ** -11 + 2.0 ** -16 + size * 2.0 ** -20) + want.abs() * 2.0 ** -8
+        assert bool(((got - want).abs() <= bound).all())
+
+
+def test_bad_pages_in_a_chunk_are_left_out():
+    from b200fp8 import device_status
+    g = gen(22)
+    c, _, _, _ = _filled([300], None, kv=1, d=128, page=16, g=g)
+    good = c.table.clone()
+    device_status(reset=True)
+    c.table[0, 3], c.table[0, 9] = c.pages, -1
+    q = randn((100, 128), g).to(BF16)
+    out = c.attention(q.cuda(), heads=1)
+    torch.cuda.synchronize()
+    assert device_status(reset=True) == 5
+    k, v = serving.cached(c.storage[0].cpu(), good[0].cpu(), 300, 16, 128, 0.25, 0.25)
+    hidden = [i for i in range(300) if i // 16 in (3, 9)]
+    for i in (0, 57, 99):
+        keep = [j for j in range(201 + i) if j not in hidden]
+        want, _, mass, size = serving.attention(q[i:i + 1].double().unflatten(-1, (1, 128)),
+                                                k[keep], v[keep])
+        err = (out[i].cpu().double() - want.flatten()).abs()
+        bound = mass.flatten() * (2.0 ** -11 + 2.0 ** -16 + size * 2.0 ** -20) + want.flatten().abs() * 2.0 ** -8
+        assert bool((err <= bound).all())
+
+
+def test_late_large_scores_in_a_chunk_move_the_maximum():
+    g = gen(3)
+    n, d = 500, 128
+    c = _cache(layers=1, pages=40, page_size=16, kv_heads=1, head_dim=d, max_seqs=1, max_pages=40,
+               k_scale=1 / 16)
+    c.extend(_ints([n]))
+    k = randn((n, d), g) * 0.05 + torch.linspace(-4, 4, n)[:, None]
+    c.write(k.to(BF16).cuda(), randn((n, d), g).to(BF16).cuda())
+    q = torch.cat([torch.full((64, d), 0.5), torch.full((64, d), -0.5)]).to(BF16)
+    out, lse = c.attention(q.cuda(), heads=1, sm_scale=1.0, return_lse=True)
+    torch.cuda.synchronize()
+    _check_attention(c, q, out, [n], [0, 128], 1, sm_scale=1.0, lse=lse)
