@@ -24,12 +24,13 @@
 namespace b2f {
 namespace {
 
-constexpr int kStep = 128;  // keys of a step: also the unit in which items are cut
+constexpr int kStep = 128;        // keys of a step: also the unit in which items are cut
+constexpr int kDequantWarps = 7;
 
 template <int D, int TILES, int ST>
 struct Tiles {
   static constexpr int R = 128 * TILES;
-  static constexpr int kThreads = 128 + 128 * TILES;
+  static constexpr int kThreads = 256 + 128 * TILES;
   static constexpr int kQ = 128 * D * 2, kKV = kStep * D * 2;
   static constexpr int kBytes = TILES * kQ + 2 * ST * kKV + 1024;
   static constexpr int kSCol(int t) { return t * 128; }
@@ -89,8 +90,8 @@ __global__ void __launch_bounds__(Tiles<D, TILES, ST>::kThreads, 1) kv4_attentio
   if (threadIdx.x == 0) {
     mbar_init(&q_full, 4 * TILES);
     for (int s = 0; s < ST; ++s) {
-      mbar_init(&k_full[s], 3);
-      mbar_init(&v_full[s], 3);
+      mbar_init(&k_full[s], kDequantWarps);
+      mbar_init(&v_full[s], kDequantWarps);
       mbar_init(&k_empty[s], 1);
       mbar_init(&v_empty[s], 1);
     }
@@ -184,11 +185,12 @@ __global__ void __launch_bounds__(Tiles<D, TILES, ST>::kThreads, 1) kv4_attentio
       mma_commit(&drain);
       mbar_wait(&drain, 0, kDevTimeoutDrain, nullptr);
     }
-  } else if (warp < 4) {
+  } else if (warp <= kDequantWarps) {
     // ------------------------------------------------------------ dequantisation
     // Work is dealt in blocks of eight keys of K or V (q: 0 .. 15 K, 16 .. 31 V): lane = 4 * key + c,
     // c a quarter of the row.
-    constexpr int kWords = D / 32, kMine = 11;  // 32-bit words of codes of a lane; blocks of a warp
+    constexpr int kWords = D / 32;                // 32-bit words of codes of a lane
+    constexpr int kMine = (32 + kDequantWarps - 1) / kDequantWarps;  // blocks of a warp, all in flight
     constexpr int kScaleBytes = D / 64;
     const int key8 = lane >> 2, c = lane & 3, first_q = warp - 1;
     const int log2p = p.c.page_log2;
@@ -217,8 +219,7 @@ __global__ void __launch_bounds__(Tiles<D, TILES, ST>::kThreads, 1) kv4_attentio
       return page;
     };
     uint32_t codes[kMine][kWords], scales[kMine];
-    auto load = [&](const StepKeys& s, int page, int i) {
-      const int q = first_q + 3 * i;
+    auto load = [&](const StepKeys& s, int page, int q, int i) {
       if (q >= 32) return;
       const int b = q & 15, key = s.key0 + b * 8 + key8;
       const int pg = __shfl_sync(0xffffffffu, page, b);
@@ -248,7 +249,7 @@ __global__ void __launch_bounds__(Tiles<D, TILES, ST>::kThreads, 1) kv4_attentio
     StepKeys now, next;
     int page = look(now);
 #pragma unroll
-    for (int i = 0; i < kMine; ++i) load(now, page, i);
+    for (int i = 0; i < kMine; ++i) load(now, page, first_q + kDequantWarps * i, i);
     int now_page = page, next_page = look(next);
     bool ok = true;
     for (long long n = 0; ok && now.keys >= 0; ++n) {
@@ -260,7 +261,7 @@ __global__ void __launch_bounds__(Tiles<D, TILES, ST>::kThreads, 1) kv4_attentio
       bool v_free = false;
 #pragma unroll
       for (int i = 0; i < kMine; ++i) {
-        const int q = first_q + 3 * i;
+        const int q = first_q + kDequantWarps * i;
         if (!ok || q >= 32) break;
         if (q >= 16 && !v_free) {  // K is done
           fence_async_shared();
@@ -305,7 +306,7 @@ __global__ void __launch_bounds__(Tiles<D, TILES, ST>::kThreads, 1) kv4_attentio
           *reinterpret_cast<uint4*>(to + (ch >> 3) * (kStep * 128) + (((ch & 7) ^ key8) << 4)) =
               make_uint4(f[0], f[1], f[2], f[3]);
         }
-        if (next.keys >= 0) load(next, next_page, i);
+        if (next.keys >= 0) load(next, next_page, q, i);
       }
       if (ok) {
         fence_async_shared();
@@ -319,13 +320,13 @@ __global__ void __launch_bounds__(Tiles<D, TILES, ST>::kThreads, 1) kv4_attentio
     }
   } else {
     // ------------------------------------------------------------ softmax, queries and results
-    const int t = (warp - 4) >> 2;               // tile
+    const int t = (warp - 1 - kDequantWarps) >> 2;  // tile
     const int r = (warp & 3) * 32 + lane;        // row of the tile: its lane of tensor memory
     const uint32_t t_lane = tmem + (uint32_t((warp & 3) * 32) << 16);
     bool ok = true;
     uint32_t steps = 0;  // of this tile
     uint32_t pieces = 0, mine = 0;  // of the CTA, and those with rows in this tile
-    long long n = 0;                // steps of the CTA
+    uint32_t n = 0;                 // steps of the CTA
     while (ok) {
       const Item& it = cur.it;
       const bool active = t < tiles_of(it);
@@ -389,32 +390,49 @@ __global__ void __launch_bounds__(Tiles<D, TILES, ST>::kThreads, 1) kv4_attentio
         ok = __all_sync(0xffffffffu, mbar_wait(&s_full[t], steps & 1, kDevTimeoutEpilogue, &aborted));
         if (!ok) break;
         tc_fence_after();
-        float s[kStep];
-        {
-          uint32_t raw[4][32];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) tmem_ld32_async(t_lane + C::kSCol(t) + k * 32, raw[k]);
-          tmem_ld_wait_regs(raw[0]);
-          reg_fence32(raw[1]);
-          reg_fence32(raw[2]);
-          reg_fence32(raw[3]);
-#pragma unroll
-          for (int k = 0; k < kStep; ++k) s[k] = __uint_as_float(raw[k >> 5][k & 31]);
-        }
         // V of the step has come: its flags can be read
         ok = __all_sync(0xffffffffu, mbar_wait(&v_full[st], (n / ST) & 1, kDevTimeoutEpilogue, &aborted));
         if (!ok) break;
         const uint4 bad4 = *reinterpret_cast<const uint4*>(bad[st]), nan4 = *reinterpret_cast<const uint4*>(nan[st]);
         const bool flags = (bad4.x | bad4.y | bad4.z | bad4.w | nan4.x | nan4.y | nan4.z | nan4.w) != 0;
         if (__any_sync(0xffffffffu, key0 + kStep > limit) || flags) {
+          // Scores that the row may not see become -infinity, and NaN those that bring a NaN value
+          // (its scale was set to 0), in place: a loop of its own keeps the code below short.
+#pragma unroll 1
+          for (int k = 0; k < kStep; k += 16) {
+            uint32_t x[16];
+            tmem_ld16(t_lane + C::kSCol(t) + k, x);
+            const uint32_t b2 = *reinterpret_cast<const uint16_t*>(bad[st] + k / 8);
+            const uint32_t n2 = *reinterpret_cast<const uint16_t*>(nan[st] + k / 8);
 #pragma unroll
-          for (int k = 0; k < kStep; ++k)
-            if (key0 + k >= limit || bad[st][k >> 3]) s[k] = -INFINITY;
+            for (int u = 0; u < 16; ++u) {
+              if (n2 >> u & 1) x[u] = 0x7fffffffu;
+              if (key0 + k + u >= limit || (b2 >> (u & 8) & 1)) x[u] = 0xff800000u;
+            }
+            tmem_st16(t_lane + C::kSCol(t) + k, x);
+          }
+          tmem_st_wait();
         }
-        float top = -INFINITY;
+        // Two passes over the row of S, 32 columns at a time, the next ones on their way: the
+        // registers of a whole row would halve the warps of the CTA.
+        uint32_t a[32], b[32];
+        float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // four chains of maxima, of sums below
+        tmem_ld32_async(t_lane + C::kSCol(t), a);
 #pragma unroll
-        for (int k = 0; k < kStep; k += 2) top = fmax3(top, s[k], s[k + 1]);
-        top *= mul;
+        for (int k = 0; k < kStep; k += 64) {
+          tmem_ld_wait_regs(a);
+          tmem_ld32_async(t_lane + C::kSCol(t) + k + 32, b);
+#pragma unroll
+          for (int u = 0; u < 32; u += 2)
+            tops[u / 2 & 3] = fmax3(tops[u / 2 & 3], __uint_as_float(a[u]), __uint_as_float(a[u + 1]));
+          tmem_ld_wait_regs(b);
+          tmem_ld32_async(t_lane + C::kSCol(t) + (k == 0 ? 64 : 0), a);  // behind the last: the first again
+#pragma unroll
+          for (int u = 0; u < 32; u += 2)
+            tops[u / 2 & 3] = fmax3(tops[u / 2 & 3], __uint_as_float(b[u]), __uint_as_float(b[u + 1]));
+        }
+        tmem_ld_wait_regs(a);
+        const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * mul;
         // as in kv4_attention.cu: the base follows a new maximum only when it is 2^8 ahead
         float f = 1.f;
         const bool jump = top - base > kSlack + kLift;
@@ -431,29 +449,33 @@ __global__ void __launch_bounds__(Tiles<D, TILES, ST>::kThreads, 1) kv4_attentio
             for (int u = 0; u < 16; ++u) o[u] = __float_as_uint(__uint_as_float(o[u]) * f);
             tmem_st16(t_lane + C::kOCol(t) + k, o);
           }
-          tmem_st_wait();
         }
         const float ref = base == -INFINITY ? 0.f : base;
-        float2 part = make_float2(0.f, 0.f);
-        uint32_t pk[kStep / 2];
+        float2 part[4] = {};
+        const float2 mul2 = make_float2(mul, mul), ref2 = make_float2(-ref, -ref);
+        // P of 32 keys goes over columns of S that have been read
+        auto weights = [&](int k, uint32_t (&s)[32]) {
+          uint32_t pk[16];
 #pragma unroll
-        for (int k = 0; k < kStep; k += 2) {
-          const float2 x = ffma2(make_float2(s[k], s[k + 1]), make_float2(mul, mul), make_float2(-ref, -ref));
-          const float2 e = make_float2(ex2(x.x), ex2(x.y));
-          part = fadd2(part, e);
-          pk[k / 2] = pack_f16x2(e.x, e.y);
+          for (int u = 0; u < 32; u += 2) {
+            const float2 x = ffma2(make_float2(__uint_as_float(s[u]), __uint_as_float(s[u + 1])), mul2, ref2);
+            const float2 e = make_float2(ex2(x.x), ex2(x.y));
+            part[u / 2 & 3] = fadd2(part[u / 2 & 3], e);
+            pk[u / 2] = pack_f16x2(e.x, e.y);
+          }
+          tmem_st16(t_lane + C::kSCol(t) + k / 2, pk);
+        };
+#pragma unroll
+        for (int k = 0; k < kStep; k += 64) {
+          tmem_ld32_async(t_lane + C::kSCol(t) + k + 32, b);
+          weights(k, a);
+          tmem_ld_wait_regs(b);
+          if (k == 0) tmem_ld32_async(t_lane + C::kSCol(t) + 64, a);
+          weights(k + 32, b);
+          if (k == 0) tmem_ld_wait_regs(a);
         }
-        if (flags && (nan4.x | nan4.y | nan4.z | nan4.w) != 0) {
-#pragma unroll
-          for (int k = 0; k < kStep; ++k)
-            if ((nan[st][k >> 3] >> (k & 7) & 1) && key0 + k < limit && !bad[st][k >> 3]) {
-              pk[k / 2] |= k & 1 ? 0x7fff0000u : 0x7fffu;
-              part.x = NAN;
-            }
-        }
-        sum = sum * f + (part.x + part.y);
-#pragma unroll
-        for (int k = 0; k < kStep / 2; k += 16) tmem_st16p(t_lane + C::kSCol(t) + k, pk + k);
+        part[0] = fadd2(fadd2(part[0], part[1]), fadd2(part[2], part[3]));
+        sum = sum * f + (part[0].x + part[0].y);
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
@@ -466,7 +488,7 @@ __global__ void __launch_bounds__(Tiles<D, TILES, ST>::kThreads, 1) kv4_attentio
       tc_fence_after();
       const bool from_start = first == 0, to_end = cur.end == it.units, whole = from_start && to_end;
       const int slot = 2 * blockIdx.x + (from_start ? 1 : 0);
-      if (from_start && !to_end && threadIdx.x == 128) {
+      if (from_start && !to_end && threadIdx.x == 32 * (1 + kDequantWarps)) {
         const int last = runs.of(u1 - (cur.left + take) + it.units - 1);
         p.shared[blockIdx.x] = Shared{last - (int)blockIdx.x, it.s.start, it.s.n, it.h * p.group, it.rt * R};
       }
