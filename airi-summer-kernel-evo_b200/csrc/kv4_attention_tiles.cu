@@ -19,6 +19,8 @@
 // Bound: a step of two tiles is 4 * 2 * 128 * 128 * D operations: 2100 clocks of an SM at D =
 // 128, about what the softmax warps take for it; converting its codes is the third of the three
 // warpgroups' work beside them.
+#include <climits>
+
 #include "kv4_attention.cuh"
 
 namespace b2f {
@@ -82,7 +84,10 @@ __global__ void __launch_bounds__(Tiles<D, TILES, ST>::kThreads, 1) kv4_attentio
   __shared__ Scan sc;
   __shared__ __align__(8) uint64_t q_full, k_full[ST], k_empty[ST], v_full[ST], v_empty[ST], s_full[TILES],
       p_full[TILES], o_full[TILES], drain;
-  __shared__ __align__(16) uint8_t bad[ST][16], nan[ST][16];  // of eight keys: page is bad; NaN bits
+  // Of the eights of keys of a step: those on a bad page; the keys with a NaN value (bits; written
+  // in steps that not all rows see to the end).
+  __shared__ uint32_t bad[ST];
+  __shared__ __align__(16) uint8_t nan[ST][16];
   __shared__ uint32_t tmem_slot;
   __shared__ int aborted;
 
@@ -196,7 +201,7 @@ __global__ void __launch_bounds__(Tiles<D, TILES, ST>::kThreads, 1) kv4_attentio
     const int log2p = p.c.page_log2;
     bool over = false;  // no more steps to look ahead to
     auto look = [&](StepKeys& s) {  // the next step, and the page of lane's block of eight keys
-      int page = -1;
+      int page = INT_MIN;           // not needed
       if (cur.unit >= cur.end && !cur.next_piece(p)) over = true;
       if (over) {
         s.keys = -1;
@@ -209,13 +214,7 @@ __global__ void __launch_bounds__(Tiles<D, TILES, ST>::kThreads, 1) kv4_attentio
       s.lowest = p.causal ? min(cur.it.s.len - cur.it.s.n + by_group(cur.it.rt * R, p.group_inv) + 1, s.keys) : s.keys;
       ++cur.unit;
       const int key = s.key0 + lane * 8;
-      if (lane < 16 && key < s.keys) {
-        page = s.pages[key >> log2p];
-        if ((unsigned)page >= (unsigned)p.c.pages) {
-          record_error(kDevBadArgs);
-          page = -2;
-        }
-      }
+      if (lane < 16 && key < s.keys) page = s.pages[key >> log2p];
       return page;
     };
     uint32_t codes[kMine][kWords], scales[kMine];
@@ -226,7 +225,7 @@ __global__ void __launch_bounds__(Tiles<D, TILES, ST>::kThreads, 1) kv4_attentio
 #pragma unroll
       for (int w = 0; w < kWords; ++w) codes[i][w] = 0;
       scales[i] = 0;
-      if (pg < 0 || key >= s.keys) return;
+      if ((unsigned)pg >= (unsigned)p.c.pages || key >= s.keys) return;
       const int slot = key & (p.c.page_size - 1);
       const uint8_t* from = s.block + (long long)pg * p.c.page_stride + (q >= 16 ? p.c.codes_bytes + p.c.scales_bytes : 0);
       const uint8_t* row = from + slot * (D / 2) + c * (kWords * 4);
@@ -257,6 +256,7 @@ __global__ void __launch_bounds__(Tiles<D, TILES, ST>::kThreads, 1) kv4_attentio
       const uint32_t ph = ((n / ST) & 1) ^ 1;
       StepKeys after;
       const int after_page = look(after);
+      const bool some_hidden = now.key0 + kStep > now.lowest;
       ok = __all_sync(0xffffffffu, mbar_wait(&k_empty[st], ph, kDevTimeoutProducer, &aborted));
       bool v_free = false;
 #pragma unroll
@@ -270,13 +270,20 @@ __global__ void __launch_bounds__(Tiles<D, TILES, ST>::kThreads, 1) kv4_attentio
           ok = __all_sync(0xffffffffu, mbar_wait(&v_empty[st], ph, kDevTimeoutProducer, &aborted));
           if (!ok) break;
           v_free = true;
+          if (warp == 1) {
+            const unsigned wrong = __ballot_sync(0xffffffffu, now_page != INT_MIN && (unsigned)now_page >= (unsigned)p.c.pages);
+            if (lane == 0) {
+              bad[st] = wrong;
+              if (wrong) record_error(kDevBadArgs);
+            }
+          }
         }
-        const int b = q & 15, key = now.key0 + b * 8 + key8;
-        if (q >= 16) {
+        const int b = q & 15;
+        if (q >= 16 && some_hidden) {
           // A NaN in a value that some row may not see: 0 here, and flagged for the rows that do
           // see it (0 * NaN would reach the others).
           bool flag = false;
-          if (key >= now.lowest) {
+          if (now.key0 + b * 8 + key8 >= now.lowest) {
 #pragma unroll
             for (int k = 0; k < kScaleBytes; ++k)
               if ((scales[i] >> (8 * k) & 0x7f) == 0x7f) {
@@ -286,11 +293,7 @@ __global__ void __launch_bounds__(Tiles<D, TILES, ST>::kThreads, 1) kv4_attentio
           }
           const unsigned any = __ballot_sync(0xffffffffu, flag);
           const unsigned of8 = __ballot_sync(0xffffffffu, lane < 8 && (any >> (4 * (lane & 7)) & 15) != 0);
-          const int pg = __shfl_sync(0xffffffffu, now_page, b);
-          if (lane == 0) {
-            nan[st][b] = (uint8_t)of8;
-            bad[st][b] = pg == -2;
-          }
+          if (lane == 0) nan[st][b] = (uint8_t)of8;
         }
         uint8_t* const to = (q < 16 ? sk : sv) + st * C::kKV + (b * 8 + key8) * 128;
         uint32_t m[(kScaleBytes + 1) / 2];
@@ -335,6 +338,7 @@ __global__ void __launch_bounds__(Tiles<D, TILES, ST>::kThreads, 1) kv4_attentio
       const int token = row_token(p, row, it.h, it.s.start, it.s.n, head);
       float mul = 0.f;
       int limit = it.keys;
+      const int lowest = p.causal ? min(it.s.len - it.s.n + by_group(it.rt * R, p.group_inv) + 1, it.keys) : it.keys;
       if (active) {
         // the row of Q: the power of two, then the operand
         const long long at = (long long)token * p.q_ld + (long long)head * D;
@@ -393,21 +397,21 @@ __global__ void __launch_bounds__(Tiles<D, TILES, ST>::kThreads, 1) kv4_attentio
         // V of the step has come: its flags can be read
         ok = __all_sync(0xffffffffu, mbar_wait(&v_full[st], (n / ST) & 1, kDevTimeoutEpilogue, &aborted));
         if (!ok) break;
-        const uint4 bad4 = *reinterpret_cast<const uint4*>(bad[st]), nan4 = *reinterpret_cast<const uint4*>(nan[st]);
-        const bool flags = (bad4.x | bad4.y | bad4.z | bad4.w | nan4.x | nan4.y | nan4.z | nan4.w) != 0;
-        if (__any_sync(0xffffffffu, key0 + kStep > limit) || flags) {
+        const uint32_t wrong = bad[st];
+        const bool some_hidden = key0 + kStep > lowest;
+        if (some_hidden || wrong != 0) {
           // Scores that the row may not see become -infinity, and NaN those that bring a NaN value
           // (its scale was set to 0), in place: a loop of its own keeps the code below short.
 #pragma unroll 1
           for (int k = 0; k < kStep; k += 16) {
             uint32_t x[16];
             tmem_ld16(t_lane + C::kSCol(t) + k, x);
-            const uint32_t b2 = *reinterpret_cast<const uint16_t*>(bad[st] + k / 8);
-            const uint32_t n2 = *reinterpret_cast<const uint16_t*>(nan[st] + k / 8);
+            const uint32_t b2 = wrong >> (k / 8);
+            const uint32_t n2 = some_hidden ? *reinterpret_cast<const uint16_t*>(nan[st] + k / 8) : 0;
 #pragma unroll
             for (int u = 0; u < 16; ++u) {
               if (n2 >> u & 1) x[u] = 0x7fffffffu;
-              if (key0 + k + u >= limit || (b2 >> (u & 8) & 1)) x[u] = 0xff800000u;
+              if (key0 + k + u >= limit || (b2 >> (u / 8) & 1)) x[u] = 0xff800000u;
             }
             tmem_st16(t_lane + C::kSCol(t) + k, x);
           }
