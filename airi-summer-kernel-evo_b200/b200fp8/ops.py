@@ -39,6 +39,11 @@ def _raw_stream(index: int) -> int:
     return torch._C._cuda_getCurrentRawStream(index)
 
 
+def _sig(t: Optional[torch.Tensor]):
+    """What the checks of a call see of a tensor."""
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.get_device())
+
+
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
@@ -488,57 +493,72 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
     transposed map).  Outputs, [rows, heads * head_dim], have the inputs' type unless
     ``out_dtype`` says otherwise (e4m3: stored = value / out_scale); ``q_out`` / ``k_out`` may be
     the inputs themselves.  Returns (q_out, k_out)."""
-    index = q.get_device()
-    for t in (q, k, positions, q_weight, k_weight, q_out, k_out, plan.freqs):
-        if t is not None and t.get_device() != index or index < 0:
-            _check_cuda(q, t)
-            raise ValueError("all tensors, and the plan, must be on one device")
-    d = plan.head_dim
-    rows = q.shape[0]
-    if (k is None) != (kv_heads == 0):
-        raise ValueError("k and kv_heads go together")
-    if (positions.dtype not in (torch.int32, torch.int64) or positions.shape != (rows,)
-            or not positions.is_contiguous()):
-        raise TypeError("positions must be contiguous int32 or int64 [rows]")
+    d, rows = plan.head_dim, q.shape[0]
     if out_dtype is None:
         out_dtype = (q_out.dtype if q_out is not None else
                      k_out.dtype if k_out is not None else q.dtype)
-    a = _lib.RotaryArgs()
-    if q_weight is not None or k_weight is not None:
-        if k is not None and (q_weight is None or k_weight is None):
+    if q_out is None:
+        q_out = q.new_empty((rows, heads * d), dtype=out_dtype)
+    if k is not None and k_out is None:
+        k_out = q.new_empty((rows, kv_heads * d), dtype=out_dtype)
+    index = q.get_device()
+    key = (q.shape, q.stride(), q.dtype, index, _sig(k), _sig(positions), heads, kv_heads,
+           q_head_stride, k_head_stride, in_scale, _sig(q_weight), _sig(k_weight), weight_offset,
+           eps, inverse, q_out.shape, q_out.stride(), q_out.dtype, q_out.get_device(), _sig(k_out),
+           out_dtype, out_scale)
+    known = plan.known_calls.get(key)  # by shapes, types and options: argument blocks that passed
+    if known is None:
+        for t in (q, k, positions, q_weight, k_weight, q_out, k_out, plan.freqs):
+            if t is not None and t.get_device() != index or index < 0:
+                _check_cuda(q, t)
+                raise ValueError("all tensors, and the plan, must be on one device")
+        if (k is None) != (kv_heads == 0):
+            raise ValueError("k and kv_heads go together")
+        if (positions.dtype not in (torch.int32, torch.int64) or positions.shape != (rows,)
+                or not positions.is_contiguous()):
+            raise TypeError("positions must be contiguous int32 or int64 [rows]")
+        if k is not None and (q_weight is None) != (k_weight is None):
             raise ValueError("q_weight and k_weight go together")
         for w in (q_weight, k_weight):
             if w is not None and (w.dtype != torch.float32 or not w.is_contiguous()
                                   or w.numel() != d):
                 raise TypeError("weights must be contiguous float32 [head_dim]")
-        a.q_weight, a.k_weight = _ptr(q_weight), _ptr(k_weight)
-    if q_out is None:
-        q_out = q.new_empty((rows, heads * d), dtype=out_dtype)
-    a.q_head_stride = d if q_head_stride is None else q_head_stride
-    a.q_ld, a.q_out_ld = _rotary_side("q", q, q_out, q.dtype, out_dtype, rows, heads, d,
-                                      a.q_head_stride)
-    a.q, a.q_out = q.data_ptr(), q_out.data_ptr()
+        a = _lib.RotaryArgs()
+        a.q_head_stride = d if q_head_stride is None else q_head_stride
+        a.q_ld, a.q_out_ld = _rotary_side("q", q, q_out, q.dtype, out_dtype, rows, heads, d,
+                                          a.q_head_stride)
+        if k is not None:
+            a.k_head_stride = d if k_head_stride is None else k_head_stride
+            a.k_ld, a.k_out_ld = _rotary_side("k", k, k_out, q.dtype, out_dtype, rows, kv_heads, d,
+                                              a.k_head_stride)
+        if rows == 0:
+            return q_out, k_out
+        a.rows, a.q_heads, a.k_heads, a.head_dim, a.rotary_dim = (rows, heads, kv_heads, d,
+                                                                  plan.rotary_dim)
+        a.interleaved, a.inverse = plan.interleaved, inverse
+        a.in_dtype, a.in_scale = _DT[q.dtype], in_scale
+        a.out_dtype, a.out_scale = _DT[out_dtype], out_scale
+        a.weight_offset, a.eps = weight_offset, eps
+        a.position_bits, a.magnitude = 8 * positions.element_size(), plan.magnitude
+        if len(plan.known_calls) >= 1024:
+            plan.known_calls.clear()
+        known = plan.known_calls[key] = bytes(a)
+    a = _lib.RotaryArgs.from_buffer_copy(known)
+    a.q, a.q_out, a.positions = q.data_ptr(), q_out.data_ptr(), positions.data_ptr()
+    a.freqs = plan.freqs.data_ptr()
     if k is not None:
-        if k_out is None:
-            k_out = q.new_empty((rows, kv_heads * d), dtype=out_dtype)
-        a.k_head_stride = d if k_head_stride is None else k_head_stride
-        a.k_ld, a.k_out_ld = _rotary_side("k", k, k_out, q.dtype, out_dtype, rows, kv_heads, d,
-                                          a.k_head_stride)
         a.k, a.k_out = k.data_ptr(), k_out.data_ptr()
-    if rows == 0:
-        return q_out, k_out
-    a.rows, a.q_heads, a.k_heads, a.head_dim, a.rotary_dim = rows, heads, kv_heads, d, plan.rotary_dim
-    a.interleaved, a.inverse = plan.interleaved, inverse
-    a.in_dtype, a.in_scale, a.out_dtype, a.out_scale = _DT[q.dtype], in_scale, _DT[out_dtype], out_scale
-    a.weight_offset, a.eps = weight_offset, eps
-    a.positions, a.position_bits = positions.data_ptr(), 8 * positions.element_size()
-    a.freqs, a.magnitude = plan.freqs.data_ptr(), plan.magnitude
+    if q_weight is not None:
+        a.q_weight = q_weight.data_ptr()
+    if k_weight is not None:
+        a.k_weight = k_weight.data_ptr()
     if torch.cuda.current_device() == index:
         code = _lib.lib().b2f_rotary(a, _raw_stream(index))
     else:
         with torch.cuda.device(index):
             code = _lib.lib().b2f_rotary(a, _raw_stream(index))
-    check(code)
+    if code:
+        check(code)
     return q_out, k_out
 
 

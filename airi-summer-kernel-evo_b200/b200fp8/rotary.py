@@ -80,3 +80,4 @@ class RotaryPlan:
         fixed = [round(w / (2 * math.pi) * 2.0 ** 64) % (1 << 64) for w in self.radians]
         self.freqs = torch.tensor([f - (1 << 64) if f >= 1 << 63 else f for f in fixed],
                                   dtype=torch.int64, device=device)
+        self.known_calls = {}  # of ops.rotary
