@@ -34,6 +34,8 @@
 //    every CTA takes an equal run of consecutive units, whatever the lengths: at most its
 //    first and its last item are shared with other CTAs.  Their partial (O, max, sum) go to a
 //    workspace and a second kernel joins them in order of the keys: same bits in every run.
+#include <cfloat>
+
 #include "kv4_attention.cuh"
 
 namespace b2f {
@@ -329,7 +331,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) kv4_attention_kernel(const Kv4
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        base[nt][j] = -INFINITY;
+        base[nt][j] = -FLT_MAX;  // no score yet: any is far above it, and -infinity stays -infinity
         sum[nt][j] = 0.f;
       }
 #pragma unroll
@@ -393,19 +395,35 @@ __global__ void __launch_bounds__(kThreads, CTAS) kv4_attention_kernel(const Kv4
         }
         // ---- scores to P
         float x[G][NT][4];
-        unsigned hidden = 0;  // bit (g * NT + nt) * 4 + j: the row does not see the key
-        if (edge) {
+        if (__builtin_expect(edge, 0)) {
+          // Keys that a row may not see: score -infinity.  Their values must not reach it either:
+          // 0 * NaN would.  NaN scales of values that not all rows see are set to 0 in the ring,
+          // and a row that does see one gets it through its score.  A lane looks at one key.
+          const uint32_t gone = (okay >> page0 & 1 ? 0u : 0xffffu) | (okay >> page1 & 1 ? 0u : 0xffff0000u);
+          bool nan = false;
+          if (lane < kChunk) {
+            uint32_t* row = reinterpret_cast<uint32_t*>(const_cast<uint8_t*>(
+                ks + v_part + (lane >= 16 ? scales_2nd : 0) + (lane & 15) * (D / 16)));
+#pragma unroll
+            for (int i = 0; i < D / 64; ++i) {
+              const uint32_t v = row[i], is = ((v & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;  // bytes 0x7f, 0xff
+              if (is != 0 && (key0 + lane >= lowest || (gone >> lane & 1))) {
+                row[i] = v & ~((is >> 7) * 0xffu);
+                nan = true;
+              }
+            }
+          }
+          fence_async_shared();  // the next copy into the stage comes after these stores
+          const uint32_t nans = __ballot_sync(0xffffffffu, nan);
 #pragma unroll
           for (int g = 0; g < G; ++g)
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
-                const int key = key0 + g * 16 + kr + (j >> 1) * 8;
-                if (key >= limit[nt][j & 1] || !(okay >> (g ? page1 : page0) & 1)) {
-                  hidden |= 1u << ((g * NT + nt) * 4 + j);
-                  s[g][nt][j] = -INFINITY;
-                }
+                const int key = g * 16 + kr + (j >> 1) * 8;
+                if (nans >> key & 1) s[g][nt][j] = NAN;
+                if (key0 + key >= limit[nt][j & 1] || (gone >> key & 1)) s[g][nt][j] = -INFINITY;
               }
         }
         float top = -INFINITY;
@@ -419,7 +437,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) kv4_attention_kernel(const Kv4
               x[g][nt][j + 1] = fmaf(s[g][nt][j + 1], mul[nt][1], -base[nt][1]);
               top = fmax3(top, x[g][nt][j], x[g][nt][j + 1]);  // a first score is infinitely far above the base
             }
-        if (__any_sync(0xffffffffu, top > kSlack + kLift)) {
+        if (__builtin_expect(__any_sync(0xffffffffu, top > kSlack + kLift), 0)) {
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -446,15 +464,6 @@ __global__ void __launch_bounds__(kThreads, CTAS) kv4_attention_kernel(const Kv4
               }
             }
         }
-        if (edge) {
-#pragma unroll
-          for (int g = 0; g < G; ++g)
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-              for (int j = 0; j < 4; ++j)
-                if (hidden >> ((g * NT + nt) * 4 + j) & 1) x[g][nt][j] = -INFINITY;
-        }
 #pragma unroll
         for (int g = 0; g < G; ++g)
 #pragma unroll
@@ -464,25 +473,6 @@ __global__ void __launch_bounds__(kThreads, CTAS) kv4_attention_kernel(const Kv4
               x[g][nt][j] = ex2(x[g][nt][j]);
               sum[nt][j & 1] += x[g][nt][j];
             }
-        if (edge) {
-          // What a row may not see must not reach it: 0 * NaN would.  NaN scales (of keys behind
-          // the last, or of tokens that only later rows see) count as 0 below, and a row that
-          // does see a NaN gets it through P.
-#pragma unroll
-          for (int g = 0; g < G; ++g)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              const uint8_t* row = ks + v_part + (g ? scales_2nd : 0) + (kr + j * 8) * (D / 16);
-              bool nan = false;
-#pragma unroll
-              for (int i = 0; i < D / 16; ++i) nan |= e4m3_is_nan(row[i]);
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int k = 0; k < 2; ++k)
-                  if (nan && !(hidden >> ((g * NT + nt) * 4 + 2 * j + k) & 1)) x[g][nt][2 * j + k] = NAN;
-            }
-        }
         // ---- O^T += V^T P^T
 #pragma unroll
         for (int g = 0; g < G; ++g) {
@@ -513,13 +503,6 @@ __global__ void __launch_bounds__(kThreads, CTAS) kv4_attention_kernel(const Kv4
               v[i][kWordsV / 2] = a.z;
               v[i][kWordsV - 1] = a.w;
               vm[i] = *reinterpret_cast<const uint16_t*>(vsk + i * 4 * (D / 16));
-            }
-          }
-          if (edge) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              if (e4m3_is_nan(vm[i])) vm[i] &= 0xff00;
-              if (D == 256 && e4m3_is_nan(vm[i] >> 8)) vm[i] &= 0xff;
             }
           }
           uint32_t vm01[D == 256 ? 2 : 1], vm23[D == 256 ? 2 : 1];  // scales of two keys as f16 pairs

@@ -257,8 +257,6 @@ __device__ __forceinline__ float ex2(float x) {
   return r;
 }
 
-__device__ __forceinline__ bool e4m3_is_nan(uint32_t v) { return (v & 0x7f) == 0x7f; }
-
 __device__ __forceinline__ float load1(const char* base, int dt, long long off) {
   switch (dt) {
     case kF32: return reinterpret_cast<const float*>(base)[off];
