@@ -663,7 +663,7 @@ static long long rows_of_a_sequence(const b2f_kv4_attn_args* a) {
 static long long attention_workspace(const b2f_kv4_attn_args* a, int sms) {
   if (sms <= 0) return -1;
   const int d = a->cache.head_dim;
-  if (b2f::kv4_tiles_fit(d, rows_of_a_sequence(a))) return b2f::kv4_tiles_workspace(d, sms);
+  if (b2f::kv4_tiles_fit(rows_of_a_sequence(a))) return b2f::kv4_tiles_workspace(d, sms);
   const long long rows = d == 256 ? 8 : 16, ctas = (long long)sms * b2f::kMaxPerSm;
   return ctas * (2ll * rows * (d + 2) * 4 + (long long)sizeof(b2f::Shared));
 }
@@ -724,7 +724,7 @@ int b2f_kv4_attention(const b2f_kv4_attn_args* a, b2f_stream_t stream) {
   p.ctx_scale = a->ctx_scale; p.lse = a->lse;
   p.partial = reinterpret_cast<float*>(a->workspace);
   cudaStream_t s = (cudaStream_t)stream;
-  if (kv4_tiles_fit(d, rows_of_a_sequence(a))) return kv4_tiles_launch(p, sms, s);
+  if (kv4_tiles_fit(rows_of_a_sequence(a))) return kv4_tiles_launch(p, sms, s);
   // 16 rows a tile read every key half as often as 8 do, once there are more than 8.
   const long long most = a->batch.starts != nullptr ? a->batch.tokens : a->batch.tokens / a->batch.seqs;
   const int rows = tile_rows(d, most * p.group);

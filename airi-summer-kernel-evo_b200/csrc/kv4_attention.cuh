@@ -447,7 +447,7 @@ struct FuncAttrOnce {
 
 // The kernel for many rows of queries (kv4_attention_tiles.cu): whether it is for these rows, its
 // workspace, and its launch.
-bool kv4_tiles_fit(int head_dim, long long rows_of_a_sequence);
+bool kv4_tiles_fit(long long rows_of_a_sequence);
 long long kv4_tiles_workspace(int head_dim, int sms);
 int kv4_tiles_launch(Kv4AttnParams& p, int sms, cudaStream_t s);
 

@@ -3,22 +3,28 @@
 //
 // A CTA works on TILES tiles of 128 query rows (query heads of one kv head x new tokens) and
 // walks over the keys 128 at a time:
-//   dequantisation (3 warps)  K and V codes of the step from the pages to f16 operands in shared
+//   products (1 warp)         S = Q K^T into tensor memory; O += P V with P read from there, then S
+//                             of the next step over it
+//   dequantisation (7 warps)  K and V codes of the step from the pages to f16 operands in shared
 //                             memory, 128-byte-swizzled rows of 64 elements: K-major for Q.K^T,
 //                             MN-major for P.V, the same bytes.  e2m1 x e4m3 is exact in f16.
 //                             The codes of the next step are in registers while these are
-//                             converted, and the page numbers of the one after that.
-//   products (1 thread)       S = Q K^T into tensor memory; O += P V with P read from there
-//   softmax (4 warps a tile)  a thread a row: the row of S into registers, P = 2^(s - base) as f16
-//                             over S, the sum in f32; O is rescaled only when a score passes the
-//                             running maximum by 2^8
-// With two tiles the tensor cores work on one while the other is exponentiated.  Queries are
-// brought to [2^14, 2^15) by a power of two of their row, as in kv4_attention.cu; P is at most
-// 2^15, its largest at least 2^7.
+//                             converted, and the page numbers of the one after that.  K and V share
+//                             a ring of NS operands.
+//   softmax (4 warps a tile)  a thread a row: the row of S from tensor memory, twice (its maximum,
+//                             then P = 2^(s - base) as f16 over S), the sum in f32; O is rescaled
+//                             only when a score passes the running maximum by 2^8
+// Queries are brought to [2^14, 2^15) by a power of two of their row, as in kv4_attention.cu; P is
+// at most 2^15, its largest at least 2^7.
 //
-// Bound: a step of two tiles is 4 * 2 * 128 * 128 * D operations: 2100 clocks of an SM at D =
-// 128, about what the softmax warps take for it; converting its codes is the third of the three
-// warpgroups' work beside them.
+// The runs of CTAs are as there (equal numbers of units, pieces joined by a second kernel); a unit
+// is a step.
+//
+// Bound: at D = 128 a step of two tiles is 2048 clocks of the tensor pipe.  Two sequences' chunks
+// (see the figures at the end) take some 5400 a step: the chain of a tile, S to P (128 exponentials
+// a thread, two such threads a scheduler's lane: 2048 clocks of the exponential unit) to P V to S, is
+// longer than the other tile's share can hide.  Tried and no faster: S in halves of 64 keys (199 us
+// against 193), two warps for the products (219; with halves 199), two rings of two for K and V.
 #include <climits>
 
 #include "kv4_attention.cuh"
@@ -29,12 +35,12 @@ namespace {
 constexpr int kStep = 128;        // keys of a step: also the unit in which items are cut
 constexpr int kDequantWarps = 7;
 
-template <int D, int TILES, int ST>
+template <int D, int TILES, int NS>
 struct Tiles {
   static constexpr int R = 128 * TILES;
   static constexpr int kThreads = 256 + 128 * TILES;
   static constexpr int kQ = 128 * D * 2, kKV = kStep * D * 2;
-  static constexpr int kBytes = TILES * kQ + 2 * ST * kKV + 1024;
+  static constexpr int kBytes = TILES * kQ + NS * kKV + 1024;
   static constexpr int kSCol(int t) { return t * 128; }
   static constexpr int kOCol(int t) { return TILES * 128 + t * D; }
   static_assert(TILES * (128 + D) <= 512, "tensor memory");
@@ -43,6 +49,57 @@ struct Tiles {
 __device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
   return make_sdesc_sw128(addr, sbo, lbo);
 }
+
+// The products are issued by one lane from code that the whole warp runs: the operands of a converged
+// warp are in uniform registers, those of a single lane's branch are moved there one by one (a
+// chunk of prompts: 242 us so, 212 us this way, with a first version of the loop below).
+__device__ __forceinline__ void mma_ss(bool mine, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
+      "r"((uint32_t)add), "r"((uint32_t)mine)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(bool mine, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc),
+      "r"((uint32_t)add), "r"((uint32_t)mine)
+      : "memory");
+}
+__device__ __forceinline__ void commit(bool mine, uint64_t* bar) {
+  if (mine) mma_commit(bar);
+  __syncwarp();
+}
+
+// A wait of the products' warp that is not over at once: out of line, for its loop has to stay in
+// the first instruction cache beside those of the other roles.
+__device__ __noinline__ bool products_wait(uint64_t* bar, uint32_t parity, int* aborted) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, kDevTimeoutMma, aborted));
+}
+
+// A place in the ring and how often it has been gone round.
+template <int NS>
+struct RingAt {
+  uint32_t slot = 0, round = 0;
+  __device__ __forceinline__ void next() {
+    if (++slot == NS) {
+      slot = 0;
+      round ^= 1;
+    }
+  }
+};
+
+// The power of two that brings a row of queries, by its largest magnitude, to [2^14, 2^15); and 2^n.
+__device__ __forceinline__ int lift_of(float top) {
+  const int ex = (__float_as_int(top) >> 23) & 0xff;
+  return ex == 0 || ex == 255 ? 0 : min(max(127 + 14 - ex, -120), 120);
+}
+__device__ __forceinline__ float exp2_of(int n) { return __int_as_float((127 + n) << 23); }
 
 // What the dequantising warps need of a step.
 struct StepKeys {
@@ -72,33 +129,30 @@ struct Cursor {
   }
 };
 
-template <int D, int TILES, int ST>
-__global__ void __launch_bounds__(Tiles<D, TILES, ST>::kThreads, 1) kv4_attention_tiles_kernel(const Kv4AttnParams p) {
-  using C = Tiles<D, TILES, ST>;
+template <int D, int TILES, int NS>
+__global__ void __launch_bounds__(Tiles<D, TILES, NS>::kThreads, 1) kv4_attention_tiles_kernel(const Kv4AttnParams p) {
+  using C = Tiles<D, TILES, NS>;
   constexpr int R = C::R;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* const sq = smem;
-  uint8_t* const sk = sq + TILES * C::kQ;
-  uint8_t* const sv = sk + ST * C::kKV;
+  uint8_t* const ring = sq + TILES * C::kQ;  // K of a step, then its V, then the next K, ...
   __shared__ Scan sc;
-  __shared__ __align__(8) uint64_t q_full, k_full[ST], k_empty[ST], v_full[ST], v_empty[ST], s_full[TILES],
-      p_full[TILES], o_full[TILES], drain;
-  // Of the eights of keys of a step: those on a bad page; the keys with a NaN value (bits; written
-  // in steps that not all rows see to the end).
-  __shared__ uint32_t bad[ST];
-  __shared__ __align__(16) uint8_t nan[ST][16];
+  __shared__ __align__(8) uint64_t q_full, kv_full[NS], kv_empty[NS],
+      s_full[TILES], p_full[TILES], o_full[TILES], drain;
+  // Of the eights of keys of a step: those on a bad page (with K); the keys with a NaN value (with
+  // V: bits; written in steps that not all rows see to the end).
+  __shared__ uint32_t bad[NS];
+  __shared__ __align__(16) uint8_t nan[NS][16];
   __shared__ uint32_t tmem_slot;
   __shared__ int aborted;
 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (threadIdx.x == 0) {
     mbar_init(&q_full, 4 * TILES);
-    for (int s = 0; s < ST; ++s) {
-      mbar_init(&k_full[s], kDequantWarps);
-      mbar_init(&v_full[s], kDequantWarps);
-      mbar_init(&k_empty[s], 1);
-      mbar_init(&v_empty[s], 1);
+    for (int s = 0; s < NS; ++s) {
+      mbar_init(&kv_full[s], kDequantWarps);
+      mbar_init(&kv_empty[s], 1);
     }
     for (int t = 0; t < TILES; ++t) {
       mbar_init(&s_full[t], 1);
@@ -132,64 +186,71 @@ __global__ void __launch_bounds__(Tiles<D, TILES, ST>::kThreads, 1) kv4_attentio
   if (u0 >= u1) {
     // nothing to do but to free the tensor memory
   } else if (warp == 0) {
-    if (lane == 0) {
-      // ------------------------------------------------------------ products
-      constexpr uint32_t idesc_s = make_idesc_f16(128, kStep, 0), idesc_o = make_idesc_f16(128, D, 1);
-      bool ok = true;
-      uint32_t piece = 0;
-      long long n = 0;         // steps
-      uint32_t done[2] = {0, 0};  // steps of each tile
-      auto scores = [&](int t, int stage) {
-        const uint32_t qa = smem_u32(sq + t * C::kQ), ka = smem_u32(sk + stage * C::kKV);
-        const uint64_t ad = smem_desc(qa, 16, 1024), bd = smem_desc(ka, 16, 1024);
+    // -------------------------------------------------------------- products
+    constexpr uint32_t idesc_s = make_idesc_f16(128, kStep, 0), idesc_o = make_idesc_f16(128, D, 1);
+    const bool mine = elect_one();
+    bool ok = true;
+    uint32_t piece = 0;
+    RingAt<NS> at;
+    uint32_t done[2] = {0, 0};  // steps of each tile
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+      return __all_sync(0xffffffffu, mbar_test(bar, parity & 1)) || products_wait(bar, parity & 1, &aborted);
+    };
+    auto scores = [&](int t, uint32_t stage) {
+      const uint64_t ad = smem_desc(smem_u32(sq + t * C::kQ), 16, 1024);
+      const uint64_t bd = smem_desc(smem_u32(ring + stage * C::kKV), 16, 1024);
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const uint32_t at = (k >> 2) * 128 * 128 + (k & 3) * 32;  // 64 elements a block of rows
-          mma_bf16(tmem + C::kSCol(t), ad + (at >> 4), bd + (at >> 4), idesc_s, k != 0);
-        }
-        mma_commit(&s_full[t]);
-      };
-      while (ok) {
-        const int tiles = tiles_of(cur.it), take = cur.end - cur.unit;
-        ok = mbar_wait(&q_full, piece & 1, kDevTimeoutMma, &aborted) &&
-             mbar_wait(&k_full[n % ST], (n / ST) & 1, kDevTimeoutMma, &aborted);
-        if (!ok) break;
-        tc_fence_after();
-        for (int t = 0; t < tiles; ++t) scores(t, n % ST);
-        mma_commit(&k_empty[n % ST]);
-        for (int j = 0; j < take && ok; ++j, ++n) {
-          const bool more = j + 1 < take;
-          const int st = n % ST, nst = (n + 1) % ST;
-          ok = mbar_wait(&v_full[st], (n / ST) & 1, kDevTimeoutMma, &aborted);
-          if (!ok) break;
-          const uint64_t vd = smem_desc(smem_u32(sv + st * C::kKV), kStep * 128, 1024);
-          for (int t = 0; t < tiles && ok; ++t) {
-            ok = mbar_wait(&p_full[t], done[t] & 1, kDevTimeoutMma, &aborted);
-            if (!ok) break;
-            ++done[t];
-            tc_fence_after();
-#pragma unroll
-            for (int k = 0; k < kStep / 16; ++k)
-              mma_bf16_ts(tmem + C::kOCol(t), tmem + C::kSCol(t) + k * 8, vd + ((k * 2048) >> 4), idesc_o,
-                          (j | k) != 0);
-            if (!more) {
-              mma_commit(&o_full[t]);
-            } else {
-              if (t == 0) ok = mbar_wait(&k_full[nst], ((n + 1) / ST) & 1, kDevTimeoutMma, &aborted);
-              if (!ok) break;
-              tc_fence_after();
-              scores(t, nst);
-            }
-          }
-          mma_commit(&v_empty[st]);
-          if (more) mma_commit(&k_empty[nst]);
-        }
-        ++piece;
-        if (!ok || !cur.next_piece(p)) break;
+      for (int k = 0; k < D / 16; ++k) {
+        const uint32_t off = (k >> 2) * 128 * 128 + (k & 3) * 32;  // 64 elements a block of rows
+        mma_ss(mine, tmem + C::kSCol(t), ad + (off >> 4), bd + (off >> 4), idesc_s, k != 0);
       }
-      mma_commit(&drain);
-      mbar_wait(&drain, 0, kDevTimeoutDrain, nullptr);
+      commit(mine, &s_full[t]);
+    };
+    while (ok) {
+      const int tiles = __reduce_max_sync(0xffffffffu, tiles_of(cur.it));
+      const int take = __reduce_max_sync(0xffffffffu, cur.end - cur.unit);
+      ok = wait(&q_full, piece) && wait(&kv_full[at.slot], at.round);
+      if (!ok) break;
+      tc_fence_after();
+#pragma unroll 1
+      for (int t = 0; t < tiles; ++t) scores(t, at.slot);
+      commit(mine, &kv_empty[at.slot]);
+      at.next();
+      for (int j = 0; j < take && ok; ++j) {
+        const bool more = j + 1 < take;
+        const uint32_t vs = at.slot;
+        ok = wait(&kv_full[vs], at.round);
+        at.next();  // K of the next step
+        if (!ok) break;
+        const uint64_t vd = smem_desc(smem_u32(ring + vs * C::kKV), kStep * 128, 1024);
+#pragma unroll 1
+        for (int t = 0; t < tiles && ok; ++t) {
+          ok = wait(&p_full[t], done[t]++);
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int k = 0; k < kStep / 16; ++k)
+            mma_ts(mine, tmem + C::kOCol(t), tmem + C::kSCol(t) + k * 8, vd + ((k * 2048) >> 4), idesc_o, (j | k) != 0);
+          if (more) {  // S of the next step, over the P that has just been used
+            if (t == 0) ok = wait(&kv_full[at.slot], at.round);
+            if (!ok) break;
+            tc_fence_after();
+            scores(t, at.slot);
+          } else {
+            commit(mine, &o_full[t]);
+          }
+        }
+        commit(mine, &kv_empty[vs]);
+        if (more) {
+          commit(mine, &kv_empty[at.slot]);
+          at.next();
+        }
+      }
+      ++piece;
+      if (!ok || !cur.next_piece(p)) break;
     }
+    commit(mine, &drain);
+    mbar_wait(&drain, 0, kDevTimeoutDrain, nullptr);
   } else if (warp <= kDequantWarps) {
     // ------------------------------------------------------------ dequantisation
     // Work is dealt in blocks of eight keys of K or V (q: 0 .. 15 K, 16 .. 31 V): lane = 4 * key + c,
@@ -251,13 +312,21 @@ __global__ void __launch_bounds__(Tiles<D, TILES, ST>::kThreads, 1) kv4_attentio
     for (int i = 0; i < kMine; ++i) load(now, page, first_q + kDequantWarps * i, i);
     int now_page = page, next_page = look(next);
     bool ok = true;
-    for (long long n = 0; ok && now.keys >= 0; ++n) {
-      const int st = n % ST;
-      const uint32_t ph = ((n / ST) & 1) ^ 1;
+    RingAt<NS> at;
+    while (ok && now.keys >= 0) {
+      RingAt<NS> ka = at;  // of K, and of V behind it
+      at.next();
       StepKeys after;
       const int after_page = look(after);
       const bool some_hidden = now.key0 + kStep > now.lowest;
-      ok = __all_sync(0xffffffffu, mbar_wait(&k_empty[st], ph, kDevTimeoutProducer, &aborted));
+      ok = __all_sync(0xffffffffu, mbar_wait(&kv_empty[ka.slot], ka.round ^ 1, kDevTimeoutProducer, &aborted));
+      if (ok && warp == 1) {
+        const unsigned wrong = __ballot_sync(0xffffffffu, now_page != INT_MIN && (unsigned)now_page >= (unsigned)p.c.pages);
+        if (lane == 0) {
+          bad[ka.slot] = wrong;
+          if (wrong) record_error(kDevBadArgs);
+        }
+      }
       bool v_free = false;
 #pragma unroll
       for (int i = 0; i < kMine; ++i) {
@@ -266,17 +335,10 @@ __global__ void __launch_bounds__(Tiles<D, TILES, ST>::kThreads, 1) kv4_attentio
         if (q >= 16 && !v_free) {  // K is done
           fence_async_shared();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&k_full[st]);
-          ok = __all_sync(0xffffffffu, mbar_wait(&v_empty[st], ph, kDevTimeoutProducer, &aborted));
+          if (lane == 0) mbar_arrive(&kv_full[ka.slot]);
+          ok = __all_sync(0xffffffffu, mbar_wait(&kv_empty[at.slot], at.round ^ 1, kDevTimeoutProducer, &aborted));
           if (!ok) break;
           v_free = true;
-          if (warp == 1) {
-            const unsigned wrong = __ballot_sync(0xffffffffu, now_page != INT_MIN && (unsigned)now_page >= (unsigned)p.c.pages);
-            if (lane == 0) {
-              bad[st] = wrong;
-              if (wrong) record_error(kDevBadArgs);
-            }
-          }
         }
         const int b = q & 15;
         if (q >= 16 && some_hidden) {
@@ -293,9 +355,9 @@ __global__ void __launch_bounds__(Tiles<D, TILES, ST>::kThreads, 1) kv4_attentio
           }
           const unsigned any = __ballot_sync(0xffffffffu, flag);
           const unsigned of8 = __ballot_sync(0xffffffffu, lane < 8 && (any >> (4 * (lane & 7)) & 15) != 0);
-          if (lane == 0) nan[st][b] = (uint8_t)of8;
+          if (lane == 0) nan[at.slot][b] = (uint8_t)of8;
         }
-        uint8_t* const to = (q < 16 ? sk : sv) + st * C::kKV + (b * 8 + key8) * 128;
+        uint8_t* const to = ring + (q < 16 ? ka.slot : at.slot) * C::kKV + (b * 8 + key8) * 128;
         uint32_t m[(kScaleBytes + 1) / 2];
 #pragma unroll
         for (int k = 0; k < (kScaleBytes + 1) / 2; ++k) m[k] = e4m3x2_to_f16x2(scales[i] >> (16 * k));
@@ -314,8 +376,9 @@ __global__ void __launch_bounds__(Tiles<D, TILES, ST>::kThreads, 1) kv4_attentio
       if (ok) {
         fence_async_shared();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&v_full[st]);
+        if (lane == 0) mbar_arrive(&kv_full[at.slot]);
       }
+      at.next();
       now = next;
       now_page = next_page;
       next = after;
@@ -329,7 +392,7 @@ __global__ void __launch_bounds__(Tiles<D, TILES, ST>::kThreads, 1) kv4_attentio
     bool ok = true;
     uint32_t steps = 0;  // of this tile
     uint32_t pieces = 0, mine = 0;  // of the CTA, and those with rows in this tile
-    uint32_t n = 0;                 // steps of the CTA
+    RingAt<NS> place;               // of the step's K
     while (ok) {
       const Item& it = cur.it;
       const bool active = t < tiles_of(it);
@@ -340,39 +403,36 @@ __global__ void __launch_bounds__(Tiles<D, TILES, ST>::kThreads, 1) kv4_attentio
       int limit = it.keys;
       const int lowest = p.causal ? min(it.s.len - it.s.n + by_group(it.rt * R, p.group_inv) + 1, it.keys) : it.keys;
       if (active) {
-        // the row of Q: the power of two, then the operand
-        const long long at = (long long)token * p.q_ld + (long long)head * D;
-        float top = 0.f;
-        auto q4 = [&](int e, float* y) {
-          if (p.q_dtype == kBF16) load4<kBF16>(p.q, at + e, y);
-          else if (p.q_dtype == kF16) load4<kF16>(p.q, at + e, y);
-          else load4<kE4M3>(p.q, at + e, y);
-        };
-        if (token >= 0) {
+        // Q of the warp's 32 rows, eight elements a lane, and each row's power of two
+        constexpr int kLanes = D / 8, kRows = 32 / kLanes;  // lanes of a row, rows at once
+        const int e = (lane % kLanes) * 8;
+        const long long mine_at = (long long)token * p.q_ld + (long long)head * D;
+        uint8_t* const to = sq + t * C::kQ + (e >> 6) * (128 * 128);
+        float own = 0.f;  // the largest of this lane's row
 #pragma unroll 4
-          for (int e = 0; e < D; e += 4) {
-            float y[4];
-            q4(e, y);
-            top = fmax3(top, fabsf(y[0]), fabsf(y[1]));
-            top = fmax3(top, fabsf(y[2]), fabsf(y[3]));
-          }
-        }
-        const int ex = (__float_as_int(top) >> 23) & 0xff;
-        const int up = ex == 0 || ex == 255 ? 0 : min(max(127 + 14 - ex, -120), 120);
-        const float lift = __int_as_float((127 + up) << 23);
-        mul = __int_as_float((127 - up) << 23) * p.scale_log2;
-        uint8_t* const to = sq + t * C::kQ + r * 128;
-#pragma unroll 4
-        for (int e = 0; e < D; e += 8) {
+        for (int i = 0; i < kLanes; ++i) {
+          const int x = i * kRows + lane / kLanes, rr = (warp & 3) * 32 + x;
+          const int there = __shfl_sync(0xffffffffu, token, x);
+          const long long at = __shfl_sync(0xffffffffu, mine_at, x) + e;
           float y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-          if (token >= 0) {
-            q4(e, y);
-            q4(e + 4, y + 4);
+          if (there >= 0) {
+            if (p.q_dtype == kBF16) { load4<kBF16>(p.q, at, y); load4<kBF16>(p.q, at + 4, y + 4); }
+            else if (p.q_dtype == kF16) { load4<kF16>(p.q, at, y); load4<kF16>(p.q, at + 4, y + 4); }
+            else { load4<kE4M3>(p.q, at, y); load4<kE4M3>(p.q, at + 4, y + 4); }
           }
-          *reinterpret_cast<uint4*>(to + (e >> 6) * (128 * 128) + ((((e >> 3) & 7) ^ (r & 7)) << 4)) =
+          float top = 0.f;
+#pragma unroll
+          for (int k = 0; k < 8; k += 2) top = fmax3(top, fabsf(y[k]), fabsf(y[k + 1]));
+#pragma unroll
+          for (int k = 1; k < kLanes; k *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
+          const float lift = exp2_of(lift_of(top));
+          *reinterpret_cast<uint4*>(to + rr * 128 + ((((e >> 3) & 7) ^ (rr & 7)) << 4)) =
               make_uint4(pack_f16x2(y[0] * lift, y[1] * lift), pack_f16x2(y[2] * lift, y[3] * lift),
                          pack_f16x2(y[4] * lift, y[5] * lift), pack_f16x2(y[6] * lift, y[7] * lift));
+          const float theirs = __shfl_sync(0xffffffffu, top, lane % kRows * kLanes);
+          if (lane / kRows == i) own = theirs;
         }
+        mul = exp2_of(-lift_of(own)) * p.scale_log2;
         if (p.causal && token >= 0) limit = min(it.s.len - it.s.n + (token - it.s.start) + 1, it.keys);
       }
       fence_async_shared();
@@ -381,7 +441,7 @@ __global__ void __launch_bounds__(Tiles<D, TILES, ST>::kThreads, 1) kv4_attentio
       if (lane == 0) mbar_arrive(&q_full);
       ++pieces;
       if (!active) {  // the next queries wait until the piece is done: q_full counts all eight warps once
-        n += take;
+        for (int j = 0; j < 2 * take; ++j) place.next();
         ok = __all_sync(0xffffffffu, mbar_wait(&o_full[0], (pieces - 1) & 1, kDevTimeoutEpilogue, &aborted));
         if (!ok || !cur.next_piece(p)) break;
         continue;
@@ -389,53 +449,53 @@ __global__ void __launch_bounds__(Tiles<D, TILES, ST>::kThreads, 1) kv4_attentio
       ++mine;
 
       float base = -INFINITY, sum = 0.f;
-      for (int j = 0; j < take && ok; ++j, ++steps, ++n) {
-        const int st = n % ST, key0 = (first + j) * kStep;
+      for (int j = 0; j < take && ok; ++j, ++steps) {
+        const int key0 = (first + j) * kStep;
+        const uint32_t ks = place.slot;
+        place.next();
+        const bool some_hidden = key0 + kStep > lowest;
+        const uint32_t col = t_lane + C::kSCol(t);
         ok = __all_sync(0xffffffffu, mbar_wait(&s_full[t], steps & 1, kDevTimeoutEpilogue, &aborted));
         if (!ok) break;
         tc_fence_after();
-        // V of the step has come: its flags can be read
-        ok = __all_sync(0xffffffffu, mbar_wait(&v_full[st], (n / ST) & 1, kDevTimeoutEpilogue, &aborted));
-        if (!ok) break;
-        const uint32_t wrong = bad[st];
-        const bool some_hidden = key0 + kStep > lowest;
+        const uint32_t wrong = bad[ks];
+        if (some_hidden) {  // V of the step has come: its flags can be read
+          ok = __all_sync(0xffffffffu, mbar_wait(&kv_full[place.slot], place.round, kDevTimeoutEpilogue, &aborted));
+          if (!ok) break;
+        }
         if (some_hidden || wrong != 0) {
           // Scores that the row may not see become -infinity, and NaN those that bring a NaN value
           // (its scale was set to 0), in place: a loop of its own keeps the code below short.
 #pragma unroll 1
           for (int k = 0; k < kStep; k += 16) {
             uint32_t x[16];
-            tmem_ld16(t_lane + C::kSCol(t) + k, x);
+            tmem_ld16(col + k, x);
             const uint32_t b2 = wrong >> (k / 8);
-            const uint32_t n2 = some_hidden ? *reinterpret_cast<const uint16_t*>(nan[st] + k / 8) : 0;
+            const uint32_t n2 = some_hidden ? *reinterpret_cast<const uint16_t*>(nan[place.slot] + k / 8) : 0;
 #pragma unroll
             for (int u = 0; u < 16; ++u) {
               if (n2 >> u & 1) x[u] = 0x7fffffffu;
               if (key0 + k + u >= limit || (b2 >> (u / 8) & 1)) x[u] = 0xff800000u;
             }
-            tmem_st16(t_lane + C::kSCol(t) + k, x);
+            tmem_st16(col + k, x);
           }
           tmem_st_wait();
         }
-        // Two passes over the row of S, 32 columns at a time, the next ones on their way: the
-        // registers of a whole row would halve the warps of the CTA.
-        uint32_t a[32], b[32];
         float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // four chains of maxima, of sums below
-        tmem_ld32_async(t_lane + C::kSCol(t), a);
-#pragma unroll
+        uint32_t a[32], b[32];
+#pragma unroll 1
         for (int k = 0; k < kStep; k += 64) {
+          tmem_ld32_async(col + k, a);
+          tmem_ld32_async(col + k + 32, b);
           tmem_ld_wait_regs(a);
-          tmem_ld32_async(t_lane + C::kSCol(t) + k + 32, b);
+          reg_fence32(b);
 #pragma unroll
-          for (int u = 0; u < 32; u += 2)
-            tops[u / 2 & 3] = fmax3(tops[u / 2 & 3], __uint_as_float(a[u]), __uint_as_float(a[u + 1]));
-          tmem_ld_wait_regs(b);
-          tmem_ld32_async(t_lane + C::kSCol(t) + (k == 0 ? 64 : 0), a);  // behind the last: the first again
-#pragma unroll
-          for (int u = 0; u < 32; u += 2)
-            tops[u / 2 & 3] = fmax3(tops[u / 2 & 3], __uint_as_float(b[u]), __uint_as_float(b[u + 1]));
+          for (int u = 0; u < 32; u += 2) {
+            tops[u / 2 & 1] = fmax3(tops[u / 2 & 1], __uint_as_float(a[u]), __uint_as_float(a[u + 1]));
+            tops[2 + (u / 2 & 1)] = fmax3(tops[2 + (u / 2 & 1)], __uint_as_float(b[u]), __uint_as_float(b[u + 1]));
+          }
         }
-        tmem_ld_wait_regs(a);
+        tmem_ld32_async(col, a);  // again, for the weights: on its way while the maxima are joined
         const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * mul;
         // as in kv4_attention.cu: the base follows a new maximum only when it is 2^8 ahead
         float f = 1.f;
@@ -444,7 +504,7 @@ __global__ void __launch_bounds__(Tiles<D, TILES, ST>::kThreads, 1) kv4_attentio
           f = ex2(base - (top - kLift));
           base = top - kLift;
         }
-        if (__any_sync(0xffffffffu, jump) && j > 0) {
+        if (__any_sync(0xffffffffu, jump) && j > 0) {  // O is complete up to the step before: S came after it
 #pragma unroll 1
           for (int k = 0; k < D; k += 16) {
             uint32_t o[16];
@@ -457,8 +517,7 @@ __global__ void __launch_bounds__(Tiles<D, TILES, ST>::kThreads, 1) kv4_attentio
         const float ref = base == -INFINITY ? 0.f : base;
         float2 part[4] = {};
         const float2 mul2 = make_float2(mul, mul), ref2 = make_float2(-ref, -ref);
-        // P of 32 keys goes over columns of S that have been read
-        auto weights = [&](int k, uint32_t (&s)[32]) {
+        auto weights = [&](int k, uint32_t (&s)[32]) {  // P of 32 keys, over the columns of S
           uint32_t pk[16];
 #pragma unroll
           for (int u = 0; u < 32; u += 2) {
@@ -467,16 +526,16 @@ __global__ void __launch_bounds__(Tiles<D, TILES, ST>::kThreads, 1) kv4_attentio
             part[u / 2 & 3] = fadd2(part[u / 2 & 3], e);
             pk[u / 2] = pack_f16x2(e.x, e.y);
           }
-          tmem_st16(t_lane + C::kSCol(t) + k / 2, pk);
+          tmem_st16(col + k / 2, pk);
         };
-#pragma unroll
+#pragma unroll 1
         for (int k = 0; k < kStep; k += 64) {
-          tmem_ld32_async(t_lane + C::kSCol(t) + k + 32, b);
+          tmem_ld_wait_regs(a);
+          tmem_ld32_async(col + k + 32, b);
           weights(k, a);
           tmem_ld_wait_regs(b);
-          if (k == 0) tmem_ld32_async(t_lane + C::kSCol(t) + 64, a);
+          if (k + 64 < kStep) tmem_ld32_async(col + k + 64, a);
           weights(k + 32, b);
-          if (k == 0) tmem_ld_wait_regs(a);
         }
         part[0] = fadd2(fadd2(part[0], part[1]), fadd2(part[2], part[3]));
         sum = sum * f + (part[0].x + part[0].y);
@@ -484,6 +543,7 @@ __global__ void __launch_bounds__(Tiles<D, TILES, ST>::kThreads, 1) kv4_attentio
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[t]);
+        place.next();
       }
       if (!ok) break;
       // ---- the piece is done
@@ -496,23 +556,36 @@ __global__ void __launch_bounds__(Tiles<D, TILES, ST>::kThreads, 1) kv4_attentio
         const int last = runs.of(u1 - (cur.left + take) + it.units - 1);
         p.shared[blockIdx.x] = Shared{last - (int)blockIdx.x, it.s.start, it.s.n, it.h * p.group, it.rt * R};
       }
-      float* const part_o = p.partial + ((long long)slot * R + t * 128 + r) * D;
+      float* const part_o = p.partial + ((long long)slot * R + t * 128) * D;
       float* const part_ms = p.partial + 2ll * p.ctas * R * D + ((long long)slot * R + t * 128 + r) * 2;
+      // O of the warp's rows through shared memory (where their queries were), sixteen columns at a
+      // time: a lane then stores four elements, and four lanes the 64 bytes of a row.
+      constexpr int kLd = 20;  // floats of a row there: sixteen and a pad
+      float* const turn = reinterpret_cast<float*>(sq + t * C::kQ + (warp & 3) * 32 * 128);
 #pragma unroll 1
       for (int d = 0; d < D; d += 16) {
         uint32_t o[16];
         tmem_ld16(t_lane + C::kOCol(t) + d, o);
-        float x[16];
+        __syncwarp();
 #pragma unroll
-        for (int u = 0; u < 16; ++u) x[u] = __uint_as_float(o[u]);
-        if (whole) {
-          if (token >= 0) finish_row<16>(p, token, head, d, x, sum);
-        } else {
+        for (int u = 0; u < 16; u += 4)
+          *reinterpret_cast<uint4*>(turn + lane * kLd + u) = make_uint4(o[u], o[u + 1], o[u + 2], o[u + 3]);
+        __syncwarp();
 #pragma unroll
-          for (int u = 0; u < 16; u += 4)
-            *reinterpret_cast<float4*>(part_o + d + u) = make_float4(x[u], x[u + 1], x[u + 2], x[u + 3]);
+        for (int i = 0; i < 4; ++i) {
+          const int x = i * 8 + (lane >> 2), c = (lane & 3) * 4;
+          const float4 v = *reinterpret_cast<const float4*>(turn + x * kLd + c);
+          if (whole) {
+            const float y[4] = {v.x, v.y, v.z, v.w};
+            const int t2 = __shfl_sync(0xffffffffu, token, x), h2 = __shfl_sync(0xffffffffu, head, x);
+            const float sum2 = __shfl_sync(0xffffffffu, sum, x);
+            if (t2 >= 0) finish_row<4>(p, t2, h2, d + c, y, sum2);
+          } else {
+            *reinterpret_cast<float4*>(part_o + ((warp & 3) * 32 + x) * D + d + c) = v;
+          }
         }
       }
+      __syncwarp();
       if (whole) {
         if (token >= 0) finish_lse(p, token, head, base, sum);
       } else {
@@ -571,23 +644,31 @@ __global__ void __launch_bounds__(kJoinThreads) kv4_tiles_join_kernel(const Kv4A
   }
 }
 
-template <int D, int TILES, int ST>
+template <int D, int TILES, int NS>
 int launch_tiles(Kv4AttnParams& p, int sms, cudaStream_t s) {
-  using C = Tiles<D, TILES, ST>;
+  using C = Tiles<D, TILES, NS>;
   static_assert(C::kBytes + 2048 <= 227 * 1024, "a CTA fits on an SM");
   static FuncAttrOnce once;
   p.ctas = sms;
   p.split = 1;
   p.shared = reinterpret_cast<Shared*>(p.partial + 2ll * p.ctas * C::R * (D + 2));
-  B2F_CUDA_TRY(once.max_smem(kv4_attention_tiles_kernel<D, TILES, ST>, C::kBytes));
-  B2F_CUDA_TRY(launch_pdl(kv4_attention_tiles_kernel<D, TILES, ST>, dim3((unsigned)p.ctas), dim3(C::kThreads), C::kBytes, s, p));
+  B2F_CUDA_TRY(once.max_smem(kv4_attention_tiles_kernel<D, TILES, NS>, C::kBytes));
+  B2F_CUDA_TRY(launch_pdl(kv4_attention_tiles_kernel<D, TILES, NS>, dim3((unsigned)p.ctas), dim3(C::kThreads), C::kBytes, s, p));
   B2F_CUDA_TRY(launch_pdl(kv4_tiles_join_kernel<D, C::R>, dim3((unsigned)p.ctas, 16), dim3(kJoinThreads), 0, s, p));
   return B2F_OK;
 }
 
 }  // namespace
 
-bool kv4_tiles_fit(int head_dim, long long rows) { return rows >= 64; }
+// Rows a sequence (new tokens x query heads of a kv head), on average, from which this form is the
+// faster one.  Microseconds, this form / the one of kv4_attention.cu, full sequences:
+//   rows                            64         128        512
+//   D  64, 4 sequences of 4096    27 / 21    30 / 28    45 / 72
+//   D 128, 4 sequences of 4096    47 / 39    49 / 61    78 / 194
+//   D 128, 16 sequences of 1024   24 / 22    26 / 30    46 / 75
+//   D 128, 1 sequence of 1024     21 / 16    23 / 18    31 / 31
+//   D 256, 4 sequences of 2048    38 / 34    43 / 52    79 / 150
+bool kv4_tiles_fit(long long rows) { return rows >= 96; }
 
 long long kv4_tiles_workspace(int head_dim, int sms) {
   const int rows = head_dim == 256 ? 128 : 256;
@@ -595,9 +676,9 @@ long long kv4_tiles_workspace(int head_dim, int sms) {
 }
 
 int kv4_tiles_launch(Kv4AttnParams& p, int sms, cudaStream_t s) {
-  if (p.c.head_dim == 64) return launch_tiles<64, 2, 2>(p, sms, s);
-  if (p.c.head_dim == 128) return launch_tiles<128, 2, 2>(p, sms, s);
-  return launch_tiles<256, 1, 1>(p, sms, s);
+  if (p.c.head_dim == 64) return launch_tiles<64, 2, 8>(p, sms, s);
+  if (p.c.head_dim == 128) return launch_tiles<128, 2, 5>(p, sms, s);
+  return launch_tiles<256, 1, 2>(p, sms, s);
 }
 
 }  // namespace b2f
