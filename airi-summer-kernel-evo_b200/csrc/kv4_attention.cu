@@ -6,10 +6,19 @@
 //
 // Bound: a step of one token per sequence reads 9/8 D bytes per key and kv head and does
 // 4 D * (heads / kv_heads) operations on them: HBM, if the codes become matrix operands cheaply
-// enough.  At the copy rate an SM receives one key (D = 128, 144 B) in 6.2 clocks; in
-// these it converts 256 codes (3.5 clocks: cvt.rn.f16x2.e2m1x2, measured 3.5 clocks a
-// warp instruction on a scheduler), scales them (2 clocks) and feeds 2 clocks of matrix
-// instructions, on three different pipes.
+// enough.  At the copy rate (6.5 TB/s) an SM receives one key (D = 128, 144 B) in 6.2 clocks; in
+// these a scheduler issues about 4.5 instructions of it (575 a warp for 32 keys), of which the
+// conversions (cvt.rn.f16x2.e2m1x2) and the scalings (multiplications of f16 pairs) take 2 clocks
+// each and the matrix instructions another 2, on three different pipes.
+//
+// Measured (device time, bytes of the cache over it), head_dim 128, 8 kv heads of 4 query heads:
+//   2 sequences of 131072 keys             64 us   4.7 TB/s   issue slots 55 % busy
+//   64 sequences of up to 8191, 273K keys  74 us   4.2 TB/s
+//   1 sequence of 197                       9.2 us (launch, one unit's latency, no join)
+//   head_dim 256, 4 kv heads, gate, e4m3; 16 sequences of up to 4000, 40K keys
+//                                          26.5 us  1.7 TB/s
+// About 10 us of each are ends: finding the run of units, the first pages' latency, cold
+// instructions, and the join (5 us); between them pages arrive at 5.6 TB/s.
 //
 // How the work is laid out
 //  - Keys on the rows of the matrix instruction (m16n8k16, f16 in, f32 out): S^T = K Q^T and
@@ -26,10 +35,16 @@
 //    bf16 and f16 queries lose nothing that is above 2^-39 of the row's largest.  P is held
 //    in f16, at most 2^15 and scaled so that the row's largest is at least 2^7: a rounding of
 //    2^-11, and of 2^-31 of the largest for the smallest.  Sums, maxima and O are f32.
-//  - Each warp walks over 32 keys at a time with a maximum, a sum and an O of its own (the
-//    maximum moves only when a score passes it by 2^8, so most steps need no exchange), and
-//    has its own ring of pages in shared memory, filled by bulk copies that it starts itself.
-//    No two warps wait for each other until a piece of work ends.
+//  - Each of four warps walks over 32 keys at a time (16 at D = 256, for its registers) with a
+//    maximum, a sum and an O of its own (the maximum moves only when a score passes it by 2^8,
+//    so most steps need no exchange); the four are joined when a piece of work ends.
+//  - A fifth warp keeps a ring of units filled: one bulk copy a page, for the block of a kv head
+//    is one piece of memory (with four copies a page, of K, V and their scales, the copies were
+//    the bound), and lays the queries of the next item out as matrix operands.
+//  - What a row may not see (keys behind the end or its position, pages that are not there, NaN in
+//    such places) is taken out of the ring by a lane a key, in a loop of its own, before it is
+//    used: the loop over all other units has no test for it (batch 76 -> 74 us, long 67 -> 64; its
+//    instructions stay in the first cache).
 //  - The keys of all (sequence, kv head, row tile) items are cut into units of 128 keys, and
 //    every CTA takes an equal run of consecutive units, whatever the lengths: at most its
 //    first and its last item are shared with other CTAs.  Their partial (O, max, sum) go to a

@@ -3,13 +3,27 @@
 //
 //   s8   = e4m3(amax(|x_0..15|) / (6 * scale))        (6 = the largest e2m1 value; saturating)
 //   code = e2m1(x / (s8 * scale))                     (ties to even, saturating; 0 when s8 is 0)
-// with IEEE f32 divisions.  A quotient of a 16-bit x lies on a border between two codes or is
-// at least 2^-13 of itself away from it, so the codes are those of exact arithmetic.  A NaN
-// makes the scale of its group NaN, an infinity saturates.
+// The code is that of the quotient as f32 rounds it; with a scale that is a power of two the divisor
+// has 4 significant bits, a quotient of a 16-bit x that is not on a border between two codes is far
+// from it, and the codes are those of exact arithmetic.  A NaN makes the scale of its group NaN, an
+// infinity saturates.
+//
+// Quotients.  With r the rounded reciprocal of s, two corrections q <- q + (x - q s) r of q = x r
+// end in the rounded quotient (P. Markstein, "Computation of elementary functions on the IBM RISC
+// System/6000 processor", 1990: the first brings q within a unit of the last place, of such a q the
+// second makes the rounded quotient; x - q s is exact in one fused multiply-add).  s lies within
+// 2^-73 and 2^73, quotients that matter within 1/8 and 16: nothing leaves the range of f32; below 1/8
+// only the sign of q matters, which is taken from x.  Groups whose scale saturates, where quotients
+// have no bound, are divided one by one.
 //
 // Bound: memory.  One lane owns one group: 32 bytes of 16-bit input in, 8 bytes of codes and
 // a scale byte out; a warp owns a token (its place is found once, all lanes alike) and runs
 // over its groups, K heads then V heads, neighbouring lanes on neighbouring groups.
+//
+// Measured: 4251 tokens of four prompts, bf16, 8 kv heads of head_dim 128 (22 MB): written and read
+// back 17.0 us, 21.0 with 16 IEEE divisions a group in place of the corrections (issue slots were
+// half busy, most of them with divisions).  24 single tokens, both calls: 4.3 us, of launches and
+// two dependent loads (a token's sequence, its page).
 #include <algorithm>
 #include <cmath>
 #include <string>
@@ -84,6 +98,21 @@ __device__ __forceinline__ uint32_t e2m1x8(const float* y) {
   return r;
 }
 
+// x / s as f32 rounds it, for |x| < 16 s and 2^-73 <= s <= 2^73 (see above; |q| < 1/8: about).
+__device__ __forceinline__ void divide16(float (&x)[16], float s) {
+  const float r = __frcp_rn(s);
+  const float2 r2 = make_float2(r, r), minus_s = make_float2(-s, -s);
+#pragma unroll
+  for (int i = 0; i < 16; i += 2) {
+    const float2 v = make_float2(x[i], x[i + 1]);
+    float2 q = fmul2(v, r2);
+    q = ffma2(ffma2(q, minus_s, v), r2, q);
+    q = ffma2(ffma2(q, minus_s, v), r2, q);
+    x[i] = copysignf(q.x, v.x);
+    x[i + 1] = copysignf(q.y, v.y);
+  }
+}
+
 // Where group g of a token lies: K (0) or V (1), the kv head, the group within the head.
 struct Kv4Group {
   int part, head, in_head;
@@ -148,9 +177,13 @@ __global__ void __launch_bounds__(32 * kMoveWarps) kv4_write_kernel(const Kv4Mov
       if (nan) top = __int_as_float(0x7fc00000);
       const uint16_t s8 = f32x2_to_e4m3x2(__fdiv_rn(top, 6.0f * scale), 0.f) & 0xff;
       const float s = e4m3_to_f32(uint8_t(s8)) * scale;
-      const bool some = s > 0.f;  // false for NaN too
+      if (s > 0.f && s8 < 0x7e) {
+        divide16(x, s);
+      } else {  // 0, NaN, or the largest scale, which may have been saturated
+        const bool some = s > 0.f;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) x[i] = some ? __fdiv_rn(x[i], s) : 0.f;
+        for (int i = 0; i < 16; ++i) x[i] = some ? __fdiv_rn(x[i], s) : 0.f;
+      }
       uint8_t* block = kv4_block(c, page, at);
       *reinterpret_cast<uint2*>(block + slot * (c.head_dim >> 1) + at.in_head * 8) =
           make_uint2(e2m1x8(x), e2m1x8(x + 8));

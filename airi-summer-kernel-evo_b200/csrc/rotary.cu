@@ -16,6 +16,11 @@
 // heads with the four sines and cosines of the lane in registers (their cost is shared by
 // all heads of q and k), the next head loaded ahead.  With few tokens the heads of a
 // token are dealt to several warps (see the launch).
+//
+// Measured (bytes in and out over device time): 8192 tokens x 40 heads of 128, f32, interleaved
+// 56 us, 6.0 TB/s; 4099 x 20 heads of 256, bf16, 64 elements rotated 21.9 us, 3.8 TB/s (84 MB: an
+// elementwise copy of 42 MB, which moves as much, takes 29 us); 8 tokens, e4m3 and RMS weights
+// 2.3 us, a launch.
 #include <algorithm>
 #include <cmath>
 #include <string>

@@ -554,6 +554,50 @@ def test_chunks_of_prompts(d, heads, kv, page):
     _check_attention(c, q, out, lens, starts, heads, lse=lse)
 
 
+@pytest.mark.parametrize("scale", [0.3, 1.0, 2.0 ** -64, 2.0 ** 64, 0.9999999, 1.0000001])
+def test_codes_are_those_of_the_f32_quotient(scale):
+    """Values within a few units of the last place of every border between two codes, and on it, for
+    groups of all scales (subnormal and saturated ones among them), zeros of both signs, values so
+    small that their quotients underflow.  The rule is the f32 quotient's, in numpy's division."""
+    import numpy as np
+    rng = np.random.default_rng(7)
+    n, d, f = 512, 128, np.float32
+    scale = float(f(scale))
+    s8 = torch.arange(1, 0x7f, dtype=torch.uint8).view(torch.float8_e4m3fn).float().numpy()
+    want_s = s8[rng.integers(0, len(s8), (n, d // 16, 1))].astype(f)
+    s = (want_s * f(scale)).astype(f)
+    border = np.array([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0], f)[rng.integers(0, 7, (n, d // 16, 16))]
+    x = (border * s).astype(f)
+    x = (x.view(np.int32) + rng.integers(-3, 4, x.shape, dtype=np.int32)).view(f)
+    tiny = rng.random(x.shape) < 0.1
+    x = np.where(tiny, rng.choice(np.array([0.0, 1e-45, 1e-30, 1e-38], f), x.shape), x).astype(f)
+    x[..., 0:1] = 6 * want_s * f(scale)  # fixes the scale of the group
+    x[: n // 8, :, 1:2] = 1e4 * want_s[: n // 8] * f(scale)  # another one, saturated for many
+    x = (x * np.where(rng.random(x.shape) < 0.5, f(-1), f(1))).astype(f)
+    top = np.abs(x).max(-1, keepdims=True)
+    got_s8 = torch.from_numpy((top / f(f(6) * f(scale))).astype(f)).clamp(max=448).to(torch.float8_e4m3fn)
+    div = (got_s8.float().numpy() * f(scale)).astype(f)
+    with np.errstate(divide="ignore", invalid="ignore", under="ignore"):
+        q = np.where(div > 0, (x / div).astype(f), f(0))
+    steps = (np.abs(q)[..., None] > np.array([0.25, 1.25, 2.5, 5.0], f)).sum(-1) + \
+        (np.abs(q)[..., None] >= np.array([0.75, 1.75, 3.5], f)).sum(-1)
+    codes = steps + 8 * np.signbit(q)
+    c = _cache(layers=1, pages=n // 16, page_size=16, kv_heads=1, head_dim=d, max_seqs=1,
+               max_pages=n // 16, k_scale=scale, v_scale=scale)
+    c.extend(_ints([n]))
+    flat = torch.from_numpy(x).flatten(1).cuda()
+    c.write(flat, flat)
+    torch.cuda.synchronize()
+    pages = c.table[0].long().cpu()
+    block = c.storage[0].cpu()[pages, 0]
+    for at in (0, 16 * d * 9 // 16):
+        packed = block[:, at:at + 16 * d // 2].reshape(n, d // 2)
+        got = torch.stack([packed & 15, packed >> 4], -1).flatten(1).numpy()
+        scales = block[:, at + 16 * d // 2:at + 16 * d * 9 // 16].reshape(n, d // 16)
+        assert torch.equal(scales, got_s8.view(torch.uint8)[..., 0])
+        assert (got == codes.reshape(n, d)).all()
+
+
 @pytest.mark.parametrize("q_dtype,out_dtype", [(F16, BF16), (E4M3, E4M3)])
 @pytest.mark.parametrize("causal", [True, False])
 def test_chunks_with_gate_types_and_uniform_lengths(q_dtype, out_dtype, causal):
