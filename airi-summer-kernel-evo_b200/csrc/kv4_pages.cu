@@ -15,9 +15,10 @@
 // The pages themselves are moved by a second kernel, a warp for 2 KB, bound by memory.
 //
 // Measured (device time, 8 kv heads of head_dim 128, pages of 16 tokens, 4 layers): compact of a
-// pool of 6000 pages 45.7 us: 9 for the plan, 28.5 for moving 100 MB (7.0 TB/s read and written: some
-// of it stays in the L2 cache), the rest the rewriting of tables and two launches; fork of 8 sequences of up to 1500
-// tokens eight times 12 us, 8.5 of them the plan: a chain of a few dependent loads and barriers.
+// pool of 6000 pages 45.7 us: 9 for the plan, 28.5 for moving 100 MB (7.0 TB/s read and written:
+// some of it stays in the L2 cache), the rest the rewriting of tables and two launches; fork of 8
+// sequences of up to 1500 tokens eight times 12 us, 8.5 of them the plan: a chain of a few
+// dependent loads and barriers.
 #include <algorithm>
 #include <new>
 #include <string>
