@@ -180,7 +180,8 @@ class Fp4Cache:
         bf16, f16 or e4m3; value = stored * in_scale) into their places: token i of the n of a
         sequence at position length - n + i.  ``starts`` int32 [seqs + 1] cuts the packed
         tokens into sequences (None: equal parts), ``rows`` int32 [seqs] names their table
-        rows (None: in order; distinct)."""
+        rows (None: in order; distinct).  A page that rows share is written for all of them: after
+        a fork only tokens that were added since are a row's own."""
         key = (0, k.shape, k.stride(), k.dtype, k.get_device(), v.shape, v.stride(), v.dtype,
                v.get_device(), layer, _sig(rows), _sig(starts), k_in_scale, v_in_scale)
         known = self._known.get(key)

@@ -142,9 +142,12 @@ __global__ void __launch_bounds__(Tiles<D, TILES, NS>::kThreads, 1) kv4_attentio
   __shared__ Scan sc;
   __shared__ __align__(8) uint64_t q_full, kv_full[NS], kv_empty[NS],
       s_full[TILES], p_full[TILES], o_full[TILES], drain;
-  // Of the eights of keys of a step: those on a bad page (with K); the keys with a NaN value (with
-  // V: bits; written in steps that not all rows see to the end).
-  __shared__ uint32_t bad[NS];
+  // Of the eights of keys of a step: those on a bad page; the keys with a NaN value (bits; written
+  // with V, in steps that not all rows see to the end).  The pages' flags come with K, whose place is
+  // free as soon as S is made, while the softmax warps may still have to read them: K of step m is
+  // made when they are at step m - NS / 2 or later, so there are NS / 2 + 1 of them.
+  constexpr int kFlags = NS / 2 + 1;
+  __shared__ uint32_t bad[kFlags];
   __shared__ __align__(16) uint8_t nan[NS][16];
   __shared__ uint32_t tmem_slot;
   __shared__ int aborted;
@@ -277,7 +280,7 @@ __global__ void __launch_bounds__(Tiles<D, TILES, NS>::kThreads, 1) kv4_attentio
       s.lowest = p.causal ? min(cur.it.s.len - cur.it.s.n + by_group(cur.it.rt * R, p.group_inv) + 1, s.keys) : s.keys;
       ++cur.unit;
       const int key = s.key0 + lane * 8;
-      if (lane < 16 && key < s.keys) page = s.pages[key >> log2p];
+      if (lane < 16 && key < s.keys) page = max(s.pages[key >> log2p], -1);
       return page;
     };
     uint32_t codes[kMine][kWords], scales[kMine];
@@ -315,6 +318,7 @@ __global__ void __launch_bounds__(Tiles<D, TILES, NS>::kThreads, 1) kv4_attentio
     int now_page = page, next_page = look(next);
     bool ok = true;
     RingAt<NS> at;
+    RingAt<kFlags> flags;
     while (ok && now.keys >= 0) {
       RingAt<NS> ka = at;  // of K, and of V behind it
       at.next();
@@ -325,7 +329,7 @@ __global__ void __launch_bounds__(Tiles<D, TILES, NS>::kThreads, 1) kv4_attentio
       if (ok && warp == 1) {
         const unsigned wrong = __ballot_sync(0xffffffffu, now_page != INT_MIN && (unsigned)now_page >= (unsigned)p.c.pages);
         if (lane == 0) {
-          bad[ka.slot] = wrong;
+          bad[flags.slot] = wrong;
           if (wrong) record_error(kDevBadArgs);
         }
       }
@@ -381,6 +385,7 @@ __global__ void __launch_bounds__(Tiles<D, TILES, NS>::kThreads, 1) kv4_attentio
         if (lane == 0) mbar_arrive(&kv_full[at.slot]);
       }
       at.next();
+      flags.next();
       now = next;
       now_page = next_page;
       next = after;
@@ -395,6 +400,7 @@ __global__ void __launch_bounds__(Tiles<D, TILES, NS>::kThreads, 1) kv4_attentio
     uint32_t steps = 0;  // of this tile
     uint32_t pieces = 0, mine = 0;  // of the CTA, and those with rows in this tile
     RingAt<NS> place;               // of the step's K
+    RingAt<kFlags> flags;           // and of its pages' flags
     while (ok) {
       const Item& it = cur.it;
       const bool active = t < tiles_of(it);
@@ -443,7 +449,11 @@ __global__ void __launch_bounds__(Tiles<D, TILES, NS>::kThreads, 1) kv4_attentio
       if (lane == 0) mbar_arrive(&q_full);
       ++pieces;
       if (!active) {  // the next queries wait until the piece is done: q_full counts all eight warps once
-        for (int j = 0; j < 2 * take; ++j) place.next();
+        for (int j = 0; j < take; ++j) {
+          place.next();
+          place.next();
+          flags.next();
+        }
         ok = __all_sync(0xffffffffu, mbar_wait(&o_full[0], (pieces - 1) & 1, kDevTimeoutEpilogue, &aborted));
         if (!ok || !cur.next_piece(p)) break;
         continue;
@@ -453,14 +463,13 @@ __global__ void __launch_bounds__(Tiles<D, TILES, NS>::kThreads, 1) kv4_attentio
       float base = -INFINITY, sum = 0.f;
       for (int j = 0; j < take && ok; ++j, ++steps) {
         const int key0 = (first + j) * kStep;
-        const uint32_t ks = place.slot;
         place.next();
         const bool some_hidden = key0 + kStep > lowest;
         const uint32_t col = t_lane + C::kSCol(t);
         ok = __all_sync(0xffffffffu, mbar_wait(&s_full[t], steps & 1, kDevTimeoutEpilogue, &aborted));
         if (!ok) break;
         tc_fence_after();
-        const uint32_t wrong = bad[ks];
+        const uint32_t wrong = bad[flags.slot];
         if (some_hidden) {  // V of the step has come: its flags can be read
           ok = __all_sync(0xffffffffu, mbar_wait(&kv_full[place.slot], place.round, kDevTimeoutEpilogue, &aborted));
           if (!ok) break;
@@ -546,6 +555,7 @@ __global__ void __launch_bounds__(Tiles<D, TILES, NS>::kThreads, 1) kv4_attentio
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[t]);
         place.next();
+        flags.next();
       }
       if (!ok) break;
       // ---- the piece is done

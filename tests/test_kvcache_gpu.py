@@ -673,3 +673,32 @@ def test_late_large_scores_in_a_chunk_move_the_maximum():
     out, lse = c.attention(q.cuda(), heads=1, sm_scale=1.0, return_lse=True)
     torch.cuda.synchronize()
     _check_attention(c, q, out, [n], [0, 128], 1, sm_scale=1.0, lse=lse)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("n", [1, 100])
+def test_bad_pages_of_all_kinds_in_a_long_sequence(d, n):
+    """Pages that are not there, of every number that says so, in one in four of the steps: their keys
+    are left out by every row, those of the steps next to them are not."""
+    from b200fp8 import device_status
+    g = gen(d + n)
+    length = 2500
+    c, _, _, _ = _filled([length], None, kv=1, d=d, page=16, g=g)
+    good = c.table.clone()
+    device_status(reset=True)
+    hidden = set()
+    for i, bad in zip(range(3, length // 16, 32), (c.pages, -1, -2 ** 31, 2 ** 31 - 1, -7)):
+        c.table[0, i] = bad
+        hidden.update(range(16 * i, 16 * i + 16))
+    q = randn((n, 2 * d), g).to(BF16)
+    out = c.attention(q.cuda(), heads=2)
+    torch.cuda.synchronize()
+    assert device_status(reset=True) == 5
+    k, v = serving.cached(c.storage[0].cpu(), good[0].cpu(), length, 16, d, 0.25, 0.25)
+    for i in {0, n // 2, n - 1}:
+        keep = [j for j in range(length - n + 1 + i) if j not in hidden]
+        want, _, mass, size = serving.attention(q[i:i + 1].double().unflatten(-1, (2, d)),
+                                                k[keep], v[keep])
+        err = (out[i].cpu().double() - want.flatten()).abs()
+        bound = (mass * (2.0 ** -11 + 2.0 ** -16 + size * 2.0 ** -20) + want.abs() * 2.0 ** -8).flatten()
+        assert bool((err <= bound).all())
