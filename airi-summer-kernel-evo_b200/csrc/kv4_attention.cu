@@ -296,14 +296,14 @@ __global__ void __launch_bounds__(kThreads, CTAS) kv4_attention_kernel(const Kv4
         pieces[buf].take = 0;
         mbar_arrive(&q_full[buf]);
       }
-    } else {  // no copy is left in flight when the CTA ends
-      for (int s = 0; s < min(fetched, STAGES); ++s) {
-        if (--stage < 0) {
-          stage = STAGES - 1;
-          phase ^= 1;
-        }
-        mbar_wait(&full[stage], phase, kDevTimeoutDrain, nullptr);
+    }
+    // no copy is left in flight when the CTA ends, whoever has given up
+    for (int s = 0; s < min(fetched, STAGES); ++s) {
+      if (--stage < 0) {
+        stage = STAGES - 1;
+        phase ^= 1;
       }
+      mbar_wait(&full[stage], phase, kDevTimeoutDrain, nullptr);
     }
     return;
   }
@@ -333,7 +333,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) kv4_attention_kernel(const Kv4
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        mul[nt][j] = q_drop[buf][nt * 8 + 2 * c + j] * p.scale_log2;
+        mul[nt][j] = fmaxf(q_drop[buf][nt * 8 + 2 * c + j] * p.scale_log2, FLT_MIN);  // -infinity * 0 is none
         const int i = by_group(it.row0 + nt * 8 + 2 * c + j, p.group_inv);
         limit[nt][j] = p.causal ? min(it.seen + i + 1, it.keys) : it.keys;
         if (i < it.n) lowest = min(lowest, limit[nt][j]);
@@ -430,6 +430,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) kv4_attention_kernel(const Kv4
           }
           fence_async_shared();  // the next copy into the stage comes after these stores
           const uint32_t nans = __ballot_sync(0xffffffffu, nan);
+          __syncwarp();  // the scales are read by other lanes below
 #pragma unroll
           for (int g = 0; g < G; ++g)
 #pragma unroll

@@ -27,6 +27,7 @@
 // exponentials each: 2048 clocks of the exponential unit) to P V to S, is longer than the other
 // tile's share can hide.  Tried and no faster: S in halves of 64 keys (199 us against 193), two
 // warps for the products (219; with halves 199), rings of two for K and for V apart (the same).
+#include <cfloat>
 #include <climits>
 
 #include "kv4_attention.cuh"
@@ -440,7 +441,7 @@ __global__ void __launch_bounds__(Tiles<D, TILES, NS>::kThreads, 1) kv4_attentio
           const float theirs = __shfl_sync(0xffffffffu, top, lane % kRows * kLanes);
           if (lane / kRows == i) own = theirs;
         }
-        mul = exp2_of(-lift_of(own)) * p.scale_log2;
+        mul = fmaxf(exp2_of(-lift_of(own)) * p.scale_log2, FLT_MIN);  // -infinity * 0 is none
         if (p.causal && token >= 0) limit = min(it.s.len - it.s.n + (token - it.s.start) + 1, it.keys);
       }
       fence_async_shared();

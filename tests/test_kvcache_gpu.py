@@ -702,3 +702,30 @@ def test_bad_pages_of_all_kinds_in_a_long_sequence(d, n):
         err = (out[i].cpu().double() - want.flatten()).abs()
         bound = (mass * (2.0 ** -11 + 2.0 ** -16 + size * 2.0 ** -20) + want.abs() * 2.0 ** -8).flatten()
         assert bool((err <= bound).all())
+
+
+@pytest.mark.parametrize("n", [3, 100])
+def test_queries_and_scales_too_small_for_a_product(n):
+    """Queries and a key scale whose product underflows: all scores are 0, and rows average the
+    values that they see, no others."""
+    g = gen(n)
+    d, length = 128, 170
+    c = _cache(layers=1, pages=16, page_size=16, kv_heads=1, head_dim=d, max_seqs=1, max_pages=16,
+               k_scale=2.0 ** -64, v_scale=0.25)
+    c.extend(_ints([length]))
+    k = (randn((length, d), g) * 2.0 ** -64).to(BF16)
+    c.write(k.cuda(), randn((length, d), g).to(BF16).cuda())
+    q = (randn((n, 2 * d), g) * 2.0 ** -124).to(BF16)
+    out, lse = c.attention(q.cuda(), heads=2, return_lse=True)
+    torch.cuda.synchronize()
+    _, v = serving.cached(c.storage[0].cpu(), c.table[0].cpu(), length, 16, d, 2.0 ** -64, 0.25)
+    v = v.reshape(length, d)
+    for i in range(n):
+        seen = v[:length - n + 1 + i]
+        # P is one value for all keys, exact in f16: the roundings are those of the sums and of the output
+        bound = seen.abs().mean(0) * 2.0 ** -15 + seen.mean(0).abs() * 2.0 ** -8
+        for h in range(2):
+            err = (out[i, h * d:(h + 1) * d].cpu().double() - seen.mean(0)).abs()
+            assert bool((err <= bound).all())
+        want = torch.log(torch.tensor(float(len(seen)), dtype=torch.float64))
+        assert bool(((lse[i].cpu().double() - want).abs() < 2.0 ** -18).all())
