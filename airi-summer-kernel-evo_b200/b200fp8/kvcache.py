@@ -251,13 +251,13 @@ class Fp4Cache:
         them (see b2f_kv4_attention).  ``out`` bf16, f16 or e4m3 (stored = value / ctx_scale).
         With ``return_lse`` returns (out, lse f32 [tokens, heads])."""
         tokens, cols = q.shape[0], heads * self.head_dim
+        key = (2, q.shape, q.stride(), q.dtype, q.get_device(), heads, layer, _sig(rows),
+               _sig(starts), causal, q_scale, sm_scale, _sig(gate), gate_scale, gate_head_stride,
+               _sig(out), out_dtype, ctx_scale, _sig(lse), return_lse)
         if out is None:
             out = q.new_empty((tokens, cols), dtype=out_dtype)
         if return_lse and lse is None:
             lse = q.new_empty((tokens, heads), dtype=torch.float32)
-        key = (2, q.shape, q.stride(), q.dtype, q.get_device(), heads, layer, _sig(rows),
-               _sig(starts), causal, q_scale, sm_scale, _sig(gate), gate_scale, gate_head_stride,
-               out.shape, out.stride(), out.dtype, out.get_device(), ctx_scale, _sig(lse))
         known = self._known.get(key)
         if known is None:
             a = _lib.Kv4AttnArgs()

@@ -497,15 +497,14 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
     if out_dtype is None:
         out_dtype = (q_out.dtype if q_out is not None else
                      k_out.dtype if k_out is not None else q.dtype)
+    index = q.get_device()
+    key = (q.shape, q.stride(), q.dtype, index, _sig(k), _sig(positions), heads, kv_heads,
+           q_head_stride, k_head_stride, in_scale, _sig(q_weight), _sig(k_weight), weight_offset,
+           eps, inverse, _sig(q_out), _sig(k_out), out_dtype, out_scale)
     if q_out is None:
         q_out = q.new_empty((rows, heads * d), dtype=out_dtype)
     if k is not None and k_out is None:
         k_out = q.new_empty((rows, kv_heads * d), dtype=out_dtype)
-    index = q.get_device()
-    key = (q.shape, q.stride(), q.dtype, index, _sig(k), _sig(positions), heads, kv_heads,
-           q_head_stride, k_head_stride, in_scale, _sig(q_weight), _sig(k_weight), weight_offset,
-           eps, inverse, q_out.shape, q_out.stride(), q_out.dtype, q_out.get_device(), _sig(k_out),
-           out_dtype, out_scale)
     known = plan.known_calls.get(key)  # by shapes, types and options: argument blocks that passed
     if known is None:
         for t in (q, k, positions, q_weight, k_weight, q_out, k_out, plan.freqs):
