@@ -21,8 +21,8 @@
 // over its groups, K heads then V heads, neighbouring lanes on neighbouring groups.
 //
 // Measured: 4251 tokens of four prompts, bf16, 8 kv heads of head_dim 128 (22 MB): written and read
-// back 17.0 us, 21.0 with 16 IEEE divisions a group in place of the corrections (issue slots were
-// half busy, most of them with divisions).  24 single tokens, both calls: 4.3 us, of launches and
+// back 16.0 us; 16 IEEE divisions a group in place of the corrections cost 4 more (issue slots were
+// half busy, most of them with divisions).  24 single tokens, both calls: 4.2 us, of launches and
 // two dependent loads (a token's sequence, its page).
 #include <algorithm>
 #include <cmath>
@@ -98,6 +98,13 @@ __device__ __forceinline__ uint32_t e2m1x8(const float* y) {
   return r;
 }
 
+// The largest magnitude of three; NaN when one of them is.
+__device__ __forceinline__ float max3_abs_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 // x / s as f32 rounds it, for |x| < 16 s and 2^-73 <= s <= 2^73 (see above; |q| < 1/8: about).
 __device__ __forceinline__ void divide16(float (&x)[16], float s) {
   const float r = __frcp_rn(s);
@@ -135,8 +142,10 @@ __device__ __forceinline__ uint8_t* kv4_block(const Kv4Cache& c, int page, const
 }
 
 template <int DT>
-__global__ void __launch_bounds__(32 * kMoveWarps) kv4_write_kernel(const Kv4MoveParams p) {
-  constexpr int N = DT == kF32 ? 2 : 4;  // groups of a lane in flight
+__global__ void __launch_bounds__(32 * kMoveWarps, 8) kv4_write_kernel(const Kv4MoveParams p) {
+  // Groups of a lane in flight.  Four, with the registers that they take (109), leave room for half the
+  // warps: 16.5 us for the prompts above against 16.0.
+  constexpr int N = DT == kF32 ? 1 : 2;
   pdl_wait();
   pdl_trigger();
   const long long w = (long long)blockIdx.x * kMoveWarps + (threadIdx.x >> 5);
@@ -166,15 +175,15 @@ __global__ void __launch_bounds__(32 * kMoveWarps) kv4_write_kernel(const Kv4Mov
       float x[16];
       unpack16<DT>(raw[u], x);
       const float in = at.part ? p.v_in : p.k_in, scale = at.part ? c.v_scale : c.k_scale;
+      const float2 in2 = make_float2(in, in);
       float top = 0.f;
-      bool nan = false;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        x[i] *= in;
-        nan |= x[i] != x[i];
-        top = fmaxf(top, fabsf(x[i]));
+      for (int i = 0; i < 16; i += 2) {
+        const float2 y = fmul2(make_float2(x[i], x[i + 1]), in2);
+        x[i] = y.x;
+        x[i + 1] = y.y;
+        top = max3_abs_nan(top, y.x, y.y);
       }
-      if (nan) top = __int_as_float(0x7fc00000);
       const uint16_t s8 = f32x2_to_e4m3x2(__fdiv_rn(top, 6.0f * scale), 0.f) & 0xff;
       const float s = e4m3_to_f32(uint8_t(s8)) * scale;
       if (s > 0.f && s8 < 0x7e) {
