@@ -729,3 +729,55 @@ def test_queries_and_scales_too_small_for_a_product(n):
             assert bool((err <= bound).all())
         want = torch.log(torch.tensor(float(len(seen)), dtype=torch.float64))
         assert bool(((lse[i].cpu().double() - want).abs() < 2.0 ** -18).all())
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_pages_layers_and_lists_with_strides_of_their_own(d):
+    """Pages 2 GB apart (byte offsets that pass 32 bits), layers between them, a table inside a wider
+    one, length and count lists inside longer ones; every call on it, both forms of the attention."""
+    from b200fp8 import device_status
+    from b200fp8.kvcache import Fp4Cache
+    g = gen(d)
+    kv, page, heads = 2, 16, 8
+    block = page * d * 9 // 8
+    far, mid = 2 ** 31 + 4096, 2 ** 20
+    base = torch.empty(5 * far, dtype=torch.uint8, device="cuda")
+    storage = base.as_strided((2, 5, kv, block), (mid, far, block, 1))
+    storage.fill_(0xff)
+    table = torch.full((4, 9), 77, dtype=torch.int32, device="cuda")
+    lens = torch.full((6,), 99, dtype=torch.int32, device="cuda")
+    refs = torch.full((8,), 55, dtype=torch.int32, device="cuda")
+    table[1:4, 2:5], lens[2:5], refs[1:6] = -1, 0, 0
+    device_status(reset=True)
+    c = Fp4Cache.from_buffers(storage, table[1:4, 2:5], lens[2:5], refs[1:6], page_size=page,
+                              head_dim=d, k_scale=0.25, v_scale=0.25)
+    c.extend(_ints([10, 40]))          # page 0; pages 1, 2, 3
+    k, v = (randn((50, kv * d), g).to(BF16) for _ in range(2))
+    for layer in range(2):
+        c.write(k.cuda(), v.cuda(), starts=_ints([0, 10, 50]), layer=layer)
+    c.free(_ints([0]))                 # page 0
+    c.fork(_ints([1]), _ints([2]))     # its last page into page 0
+    q = randn((40, heads * d), g).to(BF16)
+    for row in (1, 2):
+        for n in (1, 40):
+            out, lse = c.attention(q[:n].cuda(), heads=heads, rows=_ints([row]), layer=1,
+                                   return_lse=True)
+            torch.cuda.synchronize()
+            _check_attention(c, q[:n], out, [0, 40, 40], [0, n], heads, layer=1, lse=lse, rows=[row])
+    c.free(_ints([1]))                 # page 3; its other pages are row 2's too
+    assert c.table[2].tolist() == [1, 2, 0] and refs[1:6].tolist() == [1, 1, 1, 0, 0]
+    kept = [t.clone() for t in c.read(40, rows=_ints([2]), layer=1)]
+    c.extend(_ints([16]), rows=_ints([0]))   # page 3
+    c.free(_ints([2]))
+    c.compact()                        # page 3 to page 0
+    assert c.table[0, 0].item() == 0 and refs[1:6].tolist() == [1, 0, 0, 0, 0]
+    c.copy_pages([0], [4])
+    torch.cuda.synchronize()
+    assert torch.equal(storage[:, 0], storage[:, 4])
+    rk, rv = serving.cached(storage[1].cpu(), torch.tensor([1, 2]), 32, page, d, 0.25, 0.25)
+    assert torch.equal(kept[0][:32].cpu().double(), rk.flatten(1).to(BF16).double())
+    assert torch.equal(kept[1][:32].cpu().double(), rv.flatten(1).to(BF16).double())
+    assert device_status(reset=True) == 0
+    assert (table[0] == 77).all() and (table[:, :2] == 77).all() and (table[:, 5:] == 77).all()
+    assert lens[:2].tolist() == [99, 99] and lens[5].item() == 99
+    assert refs[0].item() == 55 and refs[6:].tolist() == [55, 55]
