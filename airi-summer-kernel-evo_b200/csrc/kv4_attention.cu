@@ -159,8 +159,10 @@ __global__ void __launch_bounds__(kThreads, CTAS) kv4_attention_kernel(const Kv4
   long long u0, u1;
   bool blank;
   const Runs runs = find_run<R, U, kThreads>(p, sc, u0, u1, blank);
+  // No item yet; stored by the lane that stores the descriptor of one (below), for nothing else
+  // orders the two.
+  if (p.split && threadIdx.x == kWork) p.shared[blockIdx.x].more = 0;
   if (blank) blank_rows<D, R, kThreads>(p);
-  if (p.split && threadIdx.x == 0) p.shared[blockIdx.x].more = 0;
   if (u0 >= u1) return;
 
   int stage = 0, buf = 0;

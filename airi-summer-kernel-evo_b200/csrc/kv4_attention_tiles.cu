@@ -180,8 +180,9 @@ __global__ void __launch_bounds__(Tiles<D, TILES, NS>::kThreads, 1) kv4_attentio
   long long u0, u1;
   bool blank;
   const Runs runs = find_run<R, kStep, C::kThreads>(p, sc, u0, u1, blank);
+  // No item yet; stored by the thread that stores the descriptor of one (below).
+  if (threadIdx.x == 32 * (1 + kDequantWarps)) p.shared[blockIdx.x].more = 0;
   if (blank) blank_rows<D, R, C::kThreads>(p);
-  if (threadIdx.x == 0) p.shared[blockIdx.x].more = 0;
   Cursor<R> cur;
   if (u0 < u1) {
     const int first = find_item<R, kStep>(p, sc.b[0], u0 - sc.at[0], cur.it);

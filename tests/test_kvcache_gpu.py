@@ -781,3 +781,31 @@ def test_pages_layers_and_lists_with_strides_of_their_own(d):
     assert (table[0] == 77).all() and (table[:, :2] == 77).all() and (table[:, 5:] == 77).all()
     assert lens[:2].tolist() == [99, 99] and lens[5].item() == 99
     assert refs[0].item() == 55 and refs[6:].tolist() == [55, 55]
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("blank,long", [(53, 1), (160, 30)])
+def test_rows_that_see_nothing_beside_sequences_that_are_cut(d, blank, long):
+    """Sequences with many new tokens and no cached ones in front of long ones, which are cut among
+    the CTAs that fill the first ones' rows with zeros: every row is written, the same every time,
+    in both forms of the attention."""
+    g = gen(d + blank)
+    heads, page = 4, 16
+    lens = [0] * 8 + [1900, 700, 2301] * 4
+    news = [blank] * 8 + [long] * 12
+    c, _, _, _ = _filled(lens, None, kv=1, d=d, page=page, g=g)
+    starts = [0]
+    for n in news:
+        starts.append(starts[-1] + n)
+    q = randn((starts[-1], heads * d), g).to(BF16)
+    first = None
+    for _ in range(8):
+        out = torch.full((starts[-1], heads * d), float("nan"), dtype=BF16, device="cuda")
+        lse = torch.full((starts[-1], heads), float("nan"), device="cuda")
+        c.attention(q.cuda(), heads=heads, starts=_ints(starts), out=out, lse=lse)
+        torch.cuda.synchronize()
+        if first is None:
+            first = out, lse
+        assert torch.equal(out, first[0]) and torch.equal(lse, first[1])
+    assert bool((out[:8 * blank] == 0).all()) and bool((lse[:8 * blank] == -float("inf")).all())
+    _check_attention(c, q, out, lens, starts, heads, lse=lse)
