@@ -7,8 +7,9 @@ per position.  For contexts longer than a model was trained on the frequencies a
   {"kind": "ntk", "factor": s}      theta * s ** (rotary_dim / (rotary_dim - 2)) as theta
   {"kind": "yarn", "factor": s, "original_length": n, "fast": 32, "slow": 1, "magnitude": None}
       pairs that turn more than ``fast`` times in ``n`` positions keep w_i, those that turn less
-      than ``slow`` times get w_i / s, with a linear ramp between; rotated elements are multiplied
-      by ``magnitude`` (None: 0.1 ln s + 1)            [Peng et al., "YaRN", 2023]
+      than ``slow`` times get w_i / s, with a ramp linear in i between (its ends rounded outwards to
+      whole i, and cut off at 0 and rotary_dim - 1: it may end behind the last pair); rotated
+      elements are multiplied by ``magnitude`` (None: 0.1 ln s + 1)  [Peng et al., "YaRN", 2023]
 """
 from __future__ import annotations
 
@@ -47,7 +48,7 @@ def frequencies(rotary_dim: int, theta: float, scaling: Optional[dict] = None):
     def at(turns):  # the pair that turns so often in the original length
         return half * math.log(length / (turns * 2 * math.pi)) / math.log(theta)
 
-    lo, hi = max(math.floor(at(fast)), 0), min(math.ceil(at(slow)), half - 1)
+    lo, hi = max(math.floor(at(fast)), 0), min(math.ceil(at(slow)), rotary_dim - 1)
     ramp = [min(max((i - lo) / max(hi - lo, 0.001), 0.0), 1.0) for i in range(half)]
     magnitude = opts.get("magnitude")
     if magnitude is None:

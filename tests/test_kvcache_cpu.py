@@ -230,6 +230,23 @@ def test_frequencies():
     assert all(abs(t - x / (2 * math.pi)) < 1e-16 for t, x in zip(turns, w))
 
 
+@pytest.mark.parametrize("length,factor,lo,hi,last", [
+    (131072, 4.0, 45, 70, 0.46), (1048576, 8.0, 59, 84, 0.86)])
+def test_a_ramp_of_frequencies_may_end_behind_the_last_pair(length, factor, lo, hi, last):
+    """Trained lengths in which every pair turns more than once: none is stretched fully.  Pair i
+    of 64 at base 1e4 turns length * 1e4^(-i / 64) / (2 pi) times; the ramp runs from the last
+    whole i with 32 turns or more (lo) to the first with one or fewer (hi), which is no pair here."""
+    from b200fp8.rotary import frequencies
+    turns = lambda i: length * 1e4 ** (-i / 64) / (2 * math.pi)  # noqa: E731
+    assert turns(lo) >= 32 > turns(lo + 1) and turns(hi - 1) > 1 >= turns(hi) and turns(63) > 1
+    y, _ = frequencies(128, 1e4, {"kind": "yarn", "factor": factor, "original_length": length})
+    for i in range(64):
+        part = max(0, i - lo) / (hi - lo)  # of the way from w to w / factor
+        want = 1e4 ** (-i / 64) * (1 - part + part / factor)
+        assert abs(y[i] - want) <= 1e-14 * want, i
+    assert abs(y[63] * 1e4 ** (63 / 64) - last) < 0.005
+
+
 def test_oracle_pack_round_trip():
     """Values on the grid survive; a tie goes to the even code; the page layout is the header's."""
     x = torch.tensor([0.0, 0.5, -0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0, 0.25, 0.75, 1.25, 1.75, 2.5,
