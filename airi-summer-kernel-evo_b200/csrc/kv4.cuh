@@ -107,8 +107,10 @@ __device__ __forceinline__ int kv4_place(const Kv4Cache& c, const Kv4Batch& bt, 
     const unsigned below = __ballot_sync(0xffffffffu, start <= t);
     const int b = below == 0 ? -1 : 31 - __clz(below);
     if (b < 0 || b >= bt.seqs) return -2;
+    const int end = __shfl_sync(0xffffffffu, start, b + 1);
     s.start = __shfl_sync(0xffffffffu, start, b);
-    s.n = __shfl_sync(0xffffffffu, start, b + 1) - s.start;
+    s.n = end - s.start;
+    if (s.start < 0 || end > bt.tokens) s.start = s.n = 0;  // not a part of the batch: as kv4_seq has it
     s.row = __shfl_sync(0xffffffffu, row, b);
     s.len = __shfl_sync(0xffffffffu, len, b);
   } else {

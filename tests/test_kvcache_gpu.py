@@ -809,3 +809,69 @@ def test_rows_that_see_nothing_beside_sequences_that_are_cut(d, blank, long):
         assert torch.equal(out, first[0]) and torch.equal(lse, first[1])
     assert bool((out[:8 * blank] == 0).all()) and bool((lse[:8 * blank] == -float("inf")).all())
     _check_attention(c, q, out, lens, starts, heads, lse=lse)
+
+
+def _cut_wrongly(seqs, which):
+    """starts that leave the batch at one end, the tokens of the batch, and those of the sequence
+    that is cut wrongly; the others have two tokens each."""
+    tokens = 2 * seqs + 3
+    starts = [2 * i for i in range(seqs + 1)]
+    if which == "end":
+        starts[-1] = tokens + 10
+        return starts, tokens, range(2 * seqs - 2, tokens)
+    starts[0] = -4
+    return starts, tokens, range(0, 2)
+
+
+@pytest.mark.parametrize("seqs", [1, 2, 31, 32, 33])
+@pytest.mark.parametrize("which", ["start", "end"])
+def test_sequences_cut_outside_of_the_batch_are_not_written(seqs, which):
+    """However many sequences a call has, one whose tokens are not all in the batch is left out of
+    it and recorded; the others are written and read."""
+    from b200fp8 import device_status
+    from b200fp8.kvcache import Fp4Cache
+    g = gen(seqs)
+    c, _, _, _ = _filled([40] * seqs, None, kv=1, d=64, page=16, g=g)
+    starts, tokens, bad = _cut_wrongly(seqs, which)
+    k, v = randn((tokens, 64), g).to(BF16), randn((tokens, 64), g).to(BF16)
+    ref = Fp4Cache.from_buffers(c.storage.clone(), c.table, c.lens, c.refs, page_size=16,
+                                head_dim=64, k_scale=0.25, v_scale=0.25)
+    good = [b for b in range(seqs) if starts[b] >= 0 and starts[b + 1] <= tokens]
+    if good:
+        ref.write(k[2 * good[0]:2 * good[-1] + 2].cuda(), v[2 * good[0]:2 * good[-1] + 2].cuda(),
+                  rows=_ints(good))
+    assert device_status(reset=True) == 0
+    c.write(k.cuda(), v.cuda(), starts=_ints(starts))
+    assert device_status(reset=True) == 5
+    assert torch.equal(c.storage, ref.storage)
+    rk, rv = (torch.full((tokens, 64), 7.0, dtype=BF16, device="cuda") for _ in range(2))
+    c.read(tokens, starts=_ints(starts), k=rk, v=rv)
+    assert device_status(reset=True) == 5
+    for x, r in ((k, rk), (v, rv)):
+        r = r.cpu()
+        for t in range(tokens):
+            if t in bad:
+                assert bool((r[t] == 0).all())
+            elif t >= 2 * seqs:
+                assert bool((r[t] == 7).all())
+            else:
+                assert torch.equal(r[t].double(), serving.pack(x[t], 0.25)[2])
+
+
+@pytest.mark.parametrize("seqs", [2, 33])
+@pytest.mark.parametrize("which", ["start", "end"])
+def test_sequences_cut_outside_of_the_batch_are_not_attended(seqs, which):
+    from b200fp8 import device_status
+    g = gen(seqs + 1)
+    lens = [40] * seqs
+    c, _, _, _ = _filled(lens, None, kv=1, d=64, page=16, g=g)
+    starts, tokens, bad = _cut_wrongly(seqs, which)
+    q = randn((tokens, 128), g).to(BF16)
+    out = torch.full((tokens, 128), 5.0, dtype=BF16, device="cuda")
+    assert device_status(reset=True) == 0
+    c.attention(q.cuda(), heads=2, starts=_ints(starts), out=out)
+    assert device_status(reset=True) == 5
+    for t in [*bad, *range(2 * seqs, tokens)]:
+        assert bool((out[t] == 5).all())
+    good = [b for b in range(seqs) if starts[b] >= 0 and starts[b + 1] <= tokens]
+    _check_attention(c, q, out, lens, [2 * b for b in good] + [2 * good[-1] + 2], 2, rows=good)
