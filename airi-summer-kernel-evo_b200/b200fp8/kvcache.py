@@ -8,7 +8,7 @@ pages that it was given then).
 
 A step of a serving loop:
 
-    cache.extend(rows, counts)                  # pages for the new tokens
+    cache.extend(counts, rows=rows)             # pages for the new tokens
     q, k = ops.rotary(q, k, positions, plan, ...)
     cache.write(k, v, layer=l, rows=rows)
     ctx = cache.attention(q, heads=h, layer=l, rows=rows)

@@ -260,3 +260,26 @@ def test_oracle_pack_round_trip():
     block[1], block[512] = 0x72, 0x40  # element 2 of token 0: code 2, element 3: code 7; scale 2
     k, v = serving.unpack_block(block, 16, 64, 0.5, 1.0)
     assert k[0, :4].tolist() == [0.0, 0.0, 1.0, 6.0] and float(v.abs().sum()) == 0.0
+
+
+def test_calls_in_the_documents_name_the_arguments_as_the_methods_do():
+    """A positional argument of a method that an example or sentence calls stands where the method
+    has the parameter of that name."""
+    import ast
+    import inspect
+    import pathlib
+    import re
+    from b200fp8 import kvcache
+    root = pathlib.Path(__file__).resolve().parents[1]
+    texts = [kvcache.__doc__, (root / "INTEGRATION.md").read_text()]
+    seen = set()
+    for call in re.findall(r"cache\.(?:extend|write|read|fork|free|attention)\([^`\n]*?\)",
+                           "\n".join(texts)):
+        node = ast.parse(call, mode="eval").body
+        method = getattr(kvcache.Fp4Cache, node.func.attr)
+        names = list(inspect.signature(method).parameters)[1:]
+        for arg, name in zip(node.args, names):
+            assert isinstance(arg, ast.Name) and arg.id == name, call
+        assert {k.arg for k in node.keywords} <= set(names), call
+        seen.add(node.func.attr)
+    assert {"extend", "write", "attention"} <= seen
