@@ -14,13 +14,19 @@ per position.  For contexts longer than a model was trained on the frequencies a
 from __future__ import annotations
 
 import math
-from typing import Optional
+from decimal import Context, Decimal, localcontext
+from typing import List, Optional, Tuple
 
 import torch
 
 
-def frequencies(rotary_dim: int, theta: float, scaling: Optional[dict] = None):
-    """(w_i in radians per position as a list of floats, magnitude of the rotated elements)."""
+# 2 pi, and the digits that frequencies are computed with: a fixed-point word of 64 bits takes 20
+# digits behind the point, the rest is room for small factors.
+_TWO_PI = Decimal("6.28318530717958647692528676655900576839433879875021164194989")
+_DIGITS = 55
+
+
+def _exact(rotary_dim: int, theta: float, scaling: Optional[dict]) -> Tuple[List[Decimal], float]:
     half = rotary_dim // 2
     opts = dict(scaling or {"kind": "none"})
     kind = opts.pop("kind", None)
@@ -33,11 +39,14 @@ def frequencies(rotary_dim: int, theta: float, scaling: Optional[dict] = None):
     factor = float(opts.get("factor", 1.0))
     if kind != "none" and "factor" not in opts or not factor > 0 or not math.isfinite(factor):
         raise ValueError("scaling needs a factor > 0")
+    log_theta, stretch = Decimal(float(theta)).ln(), Decimal(factor)
     if kind == "ntk":
-        theta = theta * factor ** (half / (half - 1))
-    w = [theta ** (-i / half) for i in range(half)]
+        log_theta += stretch.ln() * half / (half - 1)
+    step, w = (-log_theta / half).exp(), [Decimal(1)]
+    while len(w) < half:  # half <= 128 products lose 3 of the digits
+        w.append(w[-1] * step)
     if kind == "linear":
-        return [x / factor for x in w], 1.0
+        return [x / stretch for x in w], 1.0
     if kind != "yarn":
         return w, 1.0
     length = opts.get("original_length")
@@ -49,11 +58,19 @@ def frequencies(rotary_dim: int, theta: float, scaling: Optional[dict] = None):
         return half * math.log(length / (turns * 2 * math.pi)) / math.log(theta)
 
     lo, hi = max(math.floor(at(fast)), 0), min(math.ceil(at(slow)), rotary_dim - 1)
-    ramp = [min(max((i - lo) / max(hi - lo, 0.001), 0.0), 1.0) for i in range(half)]
+    ramp = [min(max(Decimal(i - lo) / max(hi - lo, 1), Decimal(0)), Decimal(1))
+            for i in range(half)]
     magnitude = opts.get("magnitude")
     if magnitude is None:
         magnitude = 0.1 * math.log(factor) + 1.0
-    return [x * (1 - r) + x / factor * r for x, r in zip(w, ramp)], float(magnitude)
+    return [x * (1 - r) + x / stretch * r for x, r in zip(w, ramp)], float(magnitude)
+
+
+def frequencies(rotary_dim: int, theta: float, scaling: Optional[dict] = None):
+    """(w_i in radians per position as a list of floats, magnitude of the rotated elements)."""
+    with localcontext(Context(prec=_DIGITS)):
+        w, magnitude = _exact(rotary_dim, theta, scaling)
+    return [float(x) for x in w], magnitude
 
 
 class RotaryPlan:
@@ -61,8 +78,9 @@ class RotaryPlan:
 
     ``layout`` "half" pairs elements (i, i + rotary_dim / 2), "interleaved" (2 i, 2 i + 1);
     ``rotary_dim`` (None: head_dim) elements of a head turn, the rest passes through.  The
-    frequencies are held in 64-bit fixed point as turns per position (2^64 = one turn), so
-    that angles stay exact at positions in the millions."""
+    frequencies are held in 64-bit fixed point as turns per position (2^64 = one turn), rounded
+    once from their exact values: an angle is off by 2^-65 of a turn a position, 2^-34 of a turn
+    at position 2^31."""
 
     def __init__(self, head_dim: int, *, rotary_dim: Optional[int] = None, theta: float = 1e4,
                  layout: str = "half", scaling: Optional[dict] = None, device="cuda"):
@@ -77,8 +95,10 @@ class RotaryPlan:
             raise ValueError("theta must be > 1")
         self.head_dim, self.rotary_dim, self.theta = head_dim, rotary_dim, float(theta)
         self.interleaved = layout == "interleaved"
-        self.radians, self.magnitude = frequencies(rotary_dim, float(theta), scaling)
-        fixed = [round(w / (2 * math.pi) * 2.0 ** 64) % (1 << 64) for w in self.radians]
+        with localcontext(Context(prec=_DIGITS)):
+            w, self.magnitude = _exact(rotary_dim, float(theta), scaling)
+            fixed = [int((x / _TWO_PI * (1 << 64)).to_integral_value()) % (1 << 64) for x in w]
+        self.radians = [float(x) for x in w]
         self.freqs = torch.tensor([f - (1 << 64) if f >= 1 << 63 else f for f in fixed],
                                   dtype=torch.int64, device=device)
         self.known_calls = {}  # of ops.rotary

@@ -8,8 +8,8 @@
 // Angles of far positions: w_i is handed over as the fraction of a turn per position in
 // 64-bit fixed point (2^64 = one turn), so position * w_i modulo 2^64 IS the fraction of a
 // turn, exact but for the rounding of w_i (2^-65 of a turn per position: 2^-34 of a turn at
-// position 2^31).  Two integer multiply-adds give its top 32 bits; the f32 sincospi of those
-// is off by about 2^-24 of a half turn at any position.
+// position 2^31, 2^-25 at 2^40).  Two integer multiply-adds give its top 32 bits; the f32 sincospi
+// of those adds about 2^-24 of a half turn at any position.
 //
 // Bound: memory (each element is read and written once).  A lane owns four pairs of a head
 // (8 elements), so a rotation needs no shuffle; a warp owns one token and walks over its

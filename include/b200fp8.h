@@ -456,7 +456,8 @@ int b2f_swiglu_fp8(const void* gate, long long gate_ld, const void* up, long lon
  *   both); outputs of any of these types, head h at column h * head_dim; in place where type,
  *   pitch and head places agree.  q_heads or k_heads may be 0.
  *   positions: int32 or int64 [rows], any value.  freqs: [rotary_dim / 2] turns per position in
- *   64-bit fixed point, round(w_i / (2 pi) * 2^64): angles of far positions stay exact.
+ *   64-bit fixed point, round(w_i / (2 pi) * 2^64): an angle is off by 2^-65 of a turn a position
+ *   (2^-25 of a turn at position 2^40) and the f32 rounding of its fraction of a turn.
  * Next to b2f_head_norm_rope, which takes cos / sin tables at position row % seq and e4m3.
  * Requirements: head_dim, rotary_dim and head strides multiples of 8, head_dim <= 256; tensors and
  * rows aligned to four elements.

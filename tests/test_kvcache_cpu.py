@@ -247,6 +247,45 @@ def test_a_ramp_of_frequencies_may_end_behind_the_last_pair(length, factor, lo, 
     assert abs(y[63] * 1e4 ** (63 / 64) - last) < 0.005
 
 
+def _pi():
+    """pi as a fraction, good to 2^-300: Machin's formula."""
+    from fractions import Fraction
+    one = 1 << 320
+
+    def arctan_of_inverse(x):
+        total, term, k = 0, one // x, 0
+        while term:
+            total += (-1) ** k * (term // (2 * k + 1))
+            term //= x * x
+            k += 1
+        return total
+    return Fraction(4 * (4 * arctan_of_inverse(5) - arctan_of_inverse(239)), one)
+
+
+@pytest.mark.parametrize("rotary_dim,theta,scaling", [
+    (64, 1e4, None), (16, 1e7, None), (128, 1e6, None), (64, 1e4, {"kind": "linear", "factor": 8.0}),
+    (16, 1e4, {"kind": "ntk", "factor": 8.0})])
+def test_frequencies_are_rounded_once(rotary_dim, theta, scaling):
+    """The words of the plan are within half a unit of the exact frequencies, in turns: in whole
+    numbers, the power of a word that has no root in it lies between those of its neighbours."""
+    from fractions import Fraction
+    from b200fp8.rotary import RotaryPlan
+    half, pi = rotary_dim // 2, _pi()
+    kind, factor = (scaling or {}).get("kind"), int((scaling or {}).get("factor", 1))
+    plan = RotaryPlan(rotary_dim, theta=theta, scaling=scaling, device="cpu")
+    for i, word in enumerate(plan.freqs.tolist()):
+        # w = theta^(-i / half), / factor, or with theta * factor^(half / (half - 1)) as theta
+        n = half * (half - 1) if kind == "ntk" else half
+        power = Fraction(1, int(theta) ** (i * n // half))
+        if kind == "linear":
+            power /= factor ** n
+        if kind == "ntk":
+            power /= factor ** (i * half)
+        near = Fraction(10000001, 10000000)  # a little more than a half, for the digits of pi
+        low, high = (((word % (1 << 64)) * 2 + s) * pi / (1 << 64) for s in (-near, near))
+        assert low ** n <= power <= high ** n, i
+
+
 def test_oracle_pack_round_trip():
     """Values on the grid survive; a tie goes to the even code; the page layout is the header's."""
     x = torch.tensor([0.0, 0.5, -0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0, 0.25, 0.75, 1.25, 1.75, 2.5,

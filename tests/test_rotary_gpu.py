@@ -166,3 +166,24 @@ def test_nan_and_infinity_stay_in_their_pair():
     got, _ = ops.rotary(q.cuda(), None, torch.tensor([9], device="cuda"), plan, heads=1)
     bad = (~torch.isfinite(got[0])).nonzero().flatten().tolist()
     assert bad == [3, 10, 35, 42]
+
+
+@pytest.mark.parametrize("inter", [False, True])
+def test_positions_beyond_32_bits(inter):
+    """Angles of positions up to 2^40, by the exact frequencies: off by 2^-65 of a turn a position,
+    2^-25 of a turn at 2^40, as much as the rounding of the fraction that the tolerance counts."""
+    from decimal import Decimal, localcontext
+    ops, rotary = _mods()
+    g = gen(11)
+    plan = rotary.RotaryPlan(64, theta=1e4, device="cuda", layout="interleaved" if inter else "half")
+    pos = torch.tensor([1, 1 << 33, -(1 << 36) + 5, (1 << 40) - 1, 987654321987])
+    q = randn((5, 64), g)
+    got, _ = ops.rotary(q.cuda(), None, pos.cuda(), plan, heads=1)
+    with localcontext() as c:
+        c.prec = 60
+        two_pi = Decimal("6.2831853071795864769252867665590057683943387987502116419498892")
+        rest = [[float((p * Decimal(10000) ** (Decimal(-i) / 32)).remainder_near(two_pi))
+                 for i in range(32)] for p in pos.tolist()]
+    for row, angles in enumerate(rest):
+        want = serving.rotary(q[row:row + 1], torch.ones(1), angles, head_dim=64, interleaved=inter)
+        _check(got[row:row + 1], want, 64, inter, 64)
