@@ -875,3 +875,49 @@ def test_sequences_cut_outside_of_the_batch_are_not_attended(seqs, which):
         assert bool((out[t] == 5).all())
     good = [b for b in range(seqs) if starts[b] >= 0 and starts[b + 1] <= tokens]
     _check_attention(c, q, out, lens, [2 * b for b in good] + [2 * good[-1] + 2], 2, rows=good)
+
+
+@pytest.mark.parametrize("seqs", [31, 32, 33, 64, 1025])
+@pytest.mark.parametrize("each", [None, 1])
+def test_writing_and_reading_many_sequences(seqs, each):
+    """Packed tokens find their sequences, empty ones among them, however many there are."""
+    from b200fp8 import device_status
+    g = gen(seqs)
+    lens = [(i * 7) % 5 if each is None else each for i in range(seqs)]
+    device_status(reset=True)
+    c, k, v, starts = _filled(lens, None, kv=2, d=64, page=16, g=g)
+    rk, rv = c.read(starts[-1], starts=_ints(starts))
+    for x, r in ((k, rk), (v, rv)):
+        want = serving.pack(x.unflatten(-1, (2, 64)), 0.25)[2].flatten(1)
+        assert torch.equal(r.cpu().double(), want)
+    if each is not None:  # without starts, and a table row at a time from the other end
+        back = list(range(seqs - 1, -1, -1))
+        c.write(v.cuda(), k.cuda(), rows=_ints(back))
+        bk, bv = c.read(seqs)
+        assert torch.equal(bk.flip(0), rv) and torch.equal(bv.flip(0), rk)
+    assert device_status() == 0
+
+
+@pytest.mark.parametrize("d,seqs,new,starts", [
+    (64, 170, 1, False), (64, 170, 1, True), (128, 600, 1, False), (128, 600, 1, True),
+    (256, 600, 1, True), (64, 600, 14, True), (128, 170, 26, True), (256, 390, 13, False)])
+@pytest.mark.parametrize("empty", [False, True])
+def test_attention_of_many_sequences(d, seqs, new, starts, empty):
+    """More sequences than a CTA has threads, single tokens and chunks of 100 rows and more, with
+    and without sequences that hold nothing (more of them than there are CTAs, with `empty`)."""
+    g = gen(d + seqs + new)
+    heads, page = 8, 16
+    lens = [0 if (i % 8 != 5 if empty else i % 9 == 4) else 1 + (i * 29) % 70 for i in range(seqs)]
+    lens[seqs // 2] = 900
+    c, _, _, _ = _filled(lens, None, kv=1, d=d, page=page, g=g, garbage=True)
+    news = [new] * seqs
+    if starts and new > 1:
+        news = [0 if i % 11 == 3 else new for i in range(seqs)]
+    at = [0]
+    for n in news:
+        at.append(at[-1] + n)
+    q = randn((at[-1], heads * d), g).to(BF16)
+    out = torch.full((at[-1], heads * d), float("nan"), dtype=BF16, device="cuda")
+    lse = torch.full((at[-1], heads), float("nan"), device="cuda")
+    c.attention(q.cuda(), heads=heads, starts=_ints(at) if starts else None, out=out, lse=lse)
+    _check_attention(c, q, out, lens, at, heads, lse=lse)
