@@ -349,6 +349,8 @@ class Fp4Cache:
             raise ValueError("src and dst must have one length")
         if n:
             ints = ctypes.c_int * n
+            # a number that no C int holds names no page either; ctypes would cut it off to one
+            src, dst = ([p if 0 <= p < self.pages else -1 for p in x] for x in (src, dst))
             self._run(_lib.lib().b2f_kv4_copy_pages, self._pool, ints(*src), ints(*dst), n)
 
     def free_pages(self) -> int:

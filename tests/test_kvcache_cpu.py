@@ -322,3 +322,17 @@ def test_calls_in_the_documents_name_the_arguments_as_the_methods_do():
         assert {k.arg for k in node.keywords} <= set(names), call
         seen.add(node.func.attr)
     assert {"extend", "write", "attention"} <= seen
+
+
+def test_page_numbers_beyond_an_int_name_no_page(monkeypatch):
+    """copy_pages hands numbers of any size on as numbers out of range, not as their low 32 bits."""
+    from b200fp8.kvcache import Fp4Cache
+    c = Fp4Cache.__new__(Fp4Cache)
+    c.pages, c._pool = 8, _lib().Kv4Pool()
+    given = []
+    monkeypatch.setattr(Fp4Cache, "_run", lambda self, fn, pool, src, dst, n: given.append(
+        (list(src), list(dst))))
+    c.copy_pages([2 ** 32 + 1, 3, -2 ** 32, 8], [2 ** 64 + 2, 2 ** 31 + 4, 5, 7])
+    (src, dst), = given
+    assert src[1] == 3 and dst[2:] == [5, 7]
+    assert all(not 0 <= p < 8 for p in (src[0], src[2], src[3], dst[0], dst[1]))
