@@ -719,6 +719,10 @@ int b2f_kv4_attention(const b2f_kv4_attn_args* a, b2f_stream_t stream) {
       return fail(B2F_ERR_ARG, "kv4_attention: misaligned gate");
   }
   if (!(a->q_scale > 0.f) || !std::isfinite(a->q_scale)) return fail(B2F_ERR_ARG, "kv4_attention: q_scale must be > 0");
+  if (!std::isfinite(a->sm_scale)) return fail(B2F_ERR_ARG, "kv4_attention: sm_scale must be finite");
+  const float sm = a->sm_scale > 0.f ? a->sm_scale : 1.0f / std::sqrt((float)d);
+  p.scale_log2 = sm * a->q_scale * a->cache.k_scale * 1.4426950408889634f;
+  if (!std::isfinite(p.scale_log2)) return fail(B2F_ERR_ARG, "kv4_attention: sm_scale * q_scale * k_scale passes f32");
   if (!(a->ctx_scale > 0.f) || !std::isfinite(a->ctx_scale)) return fail(B2F_ERR_ARG, "kv4_attention: ctx_scale must be > 0");
   if (a->out_dtype != B2F_DTYPE_E4M3 && a->ctx_scale != 1.0f)
     return fail(B2F_ERR_ARG, "kv4_attention: ctx_scale belongs to an e4m3 output");
@@ -731,8 +735,6 @@ int b2f_kv4_attention(const b2f_kv4_attn_args* a, b2f_stream_t stream) {
   p.heads = a->heads; p.group = a->heads / hk; p.causal = a->causal != 0;
   p.group_inv = ((1ull << 40) + p.group - 1) / p.group;
   p.q = reinterpret_cast<const char*>(a->q); p.q_dtype = a->q_dtype; p.q_ld = a->q_ld;
-  const float sm = a->sm_scale > 0.f ? a->sm_scale : 1.0f / std::sqrt((float)d);
-  p.scale_log2 = sm * a->q_scale * a->cache.k_scale * 1.4426950408889634f;
   p.out_mul = a->cache.v_scale;
   p.gate = reinterpret_cast<const char*>(a->gate); p.gate_dtype = a->gate_dtype;
   const int four = a->gate_dtype == B2F_DTYPE_BF16 ? 8 : 4;

@@ -565,7 +565,8 @@ int b2f_kv4_read(const b2f_kv4_read_args* args, b2f_stream_t stream);
  *   gate optional, as in b2f_attention_fp8; out: bf16, f16 or e4m3.  lse: optional f32
  *   [tokens, heads], the natural log of the sum of exp(score).  A token that sees no key gets
  *   zeros and -infinity.  A NaN or infinity in a key or value reaches no token that may not
- *   see it.  sm_scale <= 0 selects 1/sqrt(head_dim).
+ *   see it.  sm_scale <= 0 selects 1/sqrt(head_dim); it must be finite, and so must its product with
+ *   q_scale and k_scale in f32.
  *   workspace: b2f_kv4_attention_workspace_bytes(args) bytes (by cache, batch and heads; up to
  *   40 MB for chunks of prompts), 16-byte aligned, no zeroing;
  *   calls that may run at the same time need one each.  Bitwise reproducible.

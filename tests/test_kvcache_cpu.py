@@ -336,3 +336,17 @@ def test_page_numbers_beyond_an_int_name_no_page(monkeypatch):
     (src, dst), = given
     assert src[1] == 3 and dst[2:] == [5, 7]
     assert all(not 0 <= p < 8 for p in (src[0], src[2], src[3], dst[0], dst[1]))
+
+
+def test_scales_of_scores_have_to_be_finite():
+    """A NaN as sm_scale is not "no sm_scale", and a product of scales beyond f32 is not a number."""
+    L = _lib()
+    a = L.Kv4AttnArgs()
+    L.lib().b2f_kv4_attn_args_init(ctypes.byref(a))
+    _cache(L, a)
+    a.heads, a.q, a.out, a.q_ld, a.out_ld = 8, 4096, 4096, 1024, 1024
+    f = L.lib().b2f_kv4_attention
+    for bad in (math.nan, math.inf, -math.inf):
+        _refuses(f, a, "sm_scale must be finite", sm_scale=bad)
+    _refuses(f, a, "passes f32", sm_scale=1e30, q_scale=1e30)
+    _refuses(f, a, "passes f32", q_scale=3e38, cache__k_scale=2.0 ** 64)
