@@ -253,7 +253,8 @@ int b2f_rotary(const b2f_rotary_args* a, b2f_stream_t stream) {
     return fail(B2F_ERR_ARG, "rotary: out_scale must be > 0");
   if (a->out_dtype != B2F_DTYPE_E4M3 && a->out_scale != 1.0f)
     return fail(B2F_ERR_ARG, "rotary: out_scale belongs to an e4m3 output");
-  if (a->q_heads && a->k_heads && (a->q_weight == nullptr) != (a->k_weight == nullptr))
+  // the weight of a side that is not there does not stand in for one that is
+  if ((a->q_heads && !a->q_weight && a->k_weight) || (a->k_heads && !a->k_weight && a->q_weight))
     return fail(B2F_ERR_ARG, "rotary: q_weight and k_weight go together");
   if ((reinterpret_cast<uintptr_t>(a->q_weight) | reinterpret_cast<uintptr_t>(a->k_weight)) & 15)
     return fail(B2F_ERR_ARG, "rotary: weights must be 16-byte aligned");

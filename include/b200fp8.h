@@ -471,7 +471,7 @@ typedef struct b2f_rotary_args {
   long long k_ld, k_head_stride;
   int in_dtype;
   float in_scale;
-  const float* q_weight; /* optional f32 [head_dim], 16-byte aligned; both or none */
+  const float* q_weight; /* optional f32 [head_dim], 16-byte aligned; for each side with heads, or none */
   const float* k_weight;
   float weight_offset, eps;
   const void* positions;

@@ -350,3 +350,20 @@ def test_scales_of_scores_have_to_be_finite():
         _refuses(f, a, "sm_scale must be finite", sm_scale=bad)
     _refuses(f, a, "passes f32", sm_scale=1e30, q_scale=1e30)
     _refuses(f, a, "passes f32", q_scale=3e38, cache__k_scale=2.0 ** 64)
+
+
+def test_a_weight_belongs_to_its_own_heads():
+    """A k_weight in a call without k does not normalise q, nor the other way round."""
+    L = _lib()
+    a = L.RotaryArgs()
+    L.lib().b2f_rotary_args_init(ctypes.byref(a))
+    a.rows, a.q_heads, a.head_dim, a.rotary_dim = 4, 2, 128, 128
+    a.q = a.k = a.q_out = a.k_out = a.positions = a.freqs = 4096
+    a.q_ld = a.k_ld = a.q_out_ld = a.k_out_ld = 256
+    a.q_head_stride = a.k_head_stride = 128
+    f = L.lib().b2f_rotary
+    # inverse: a call that takes the weight is refused for another reason, and nothing is launched
+    _refuses(f, a, "go together", k_weight=4096, inverse=1)
+    _refuses(f, a, "go together", q_heads=0, k_heads=2, q_weight=4096, inverse=1)
+    _refuses(f, a, "inverse", q_weight=4096, inverse=1)
+    _refuses(f, a, "inverse", q_weight=4096, k_weight=4096, inverse=1)
