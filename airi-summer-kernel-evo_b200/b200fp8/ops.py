@@ -507,6 +507,8 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
         k_out = q.new_empty((rows, kv_heads * d), dtype=out_dtype)
     known = plan.known_calls.get(key)  # by shapes, types and options: argument blocks that passed
     if known is None:
+        if rows >= 1 << 31:
+            raise ValueError("a call takes fewer than 2^31 rows")
         for t in (q, k, positions, q_weight, k_weight, q_out, k_out, plan.freqs):
             if t is not None and t.get_device() != index or index < 0:
                 _check_cuda(q, t)

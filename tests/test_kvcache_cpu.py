@@ -367,3 +367,14 @@ def test_a_weight_belongs_to_its_own_heads():
     _refuses(f, a, "go together", q_heads=0, k_heads=2, q_weight=4096, inverse=1)
     _refuses(f, a, "inverse", q_weight=4096, inverse=1)
     _refuses(f, a, "inverse", q_weight=4096, k_weight=4096, inverse=1)
+
+
+def test_rows_beyond_an_int_are_refused():
+    """2^32 + 1 rows of 8 elements fit on the GPU, but not in the C entry's int: one row there."""
+    from b200fp8 import ops, rotary
+    plan = rotary.RotaryPlan(8, device="cpu")
+    for rows in (1 << 31, (1 << 32) + 1):
+        q = torch.zeros((1, 8), dtype=torch.float8_e4m3fn).expand(rows, 8)
+        with pytest.raises(ValueError, match="rows"):
+            ops.rotary(q, None, torch.zeros(1, dtype=torch.int32).expand(rows), plan, heads=1,
+                       q_out=q)
