@@ -448,6 +448,13 @@ class QwenBlock(_Graphable):
             raise ValueError("the cache must have the block's kv_heads and head_dim")
         if hidden.dim() != 2 or hidden.shape[1] != self.hidden:
             raise ValueError(f"hidden must be [tokens, {self.hidden}]")
+        index = hidden.get_device()
+        if index != self.in_norm.get_device() or index != cache.device.index:
+            raise ValueError("hidden, the block and the cache must be on one device")
+        if index != torch.cuda.current_device():  # where the norms and products are launched
+            with torch.cuda.device(index):
+                return self.step(hidden, cache, plan, positions=positions, layer=layer, rows=rows,
+                                 starts=starts, hidden_scale=hidden_scale)
         n1, _ = ops.norm_quant(hidden, self.in_norm, kind="rms", weight_offset=1.0, eps=self.eps,
                                x_scale=hidden_scale, q_scale=self.ns)
         proj = _gemm(n1, self.w_cat, col_scale=self.cs_cat, out_dtype=_E4M3, out_scale=self.qs)

@@ -378,3 +378,46 @@ def test_rows_beyond_an_int_are_refused():
         with pytest.raises(ValueError, match="rows"):
             ops.rotary(q, None, torch.zeros(1, dtype=torch.int32).expand(rows), plan, heads=1,
                        q_out=q)
+
+
+def test_a_step_runs_on_the_device_of_its_tensors(monkeypatch):
+    """QwenBlock.step launches where its tensors are, whatever the current device, and refuses a
+    block, cache and input that are not on one device (devices by fakes: nothing is launched)."""
+    from types import SimpleNamespace
+    from b200fp8 import blocks
+    blk = blocks.QwenBlock.__new__(blocks.QwenBlock)
+    blk.h, blk.hk, blk.dh, blk.rot, blk.hidden, blk.eps, blk.ns = 2, 1, 64, 64, 128, 1e-6, 1.0
+    now = [0]
+
+    class On:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            self.old, now[0] = now[0], self.index
+
+        def __exit__(self, *_):
+            now[0] = self.old
+
+    class Launched(Exception):
+        pass
+
+    def launch(*_, **__):
+        raise Launched(now[0])
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: now[0])
+    monkeypatch.setattr(torch.cuda, "device", On)
+    monkeypatch.setattr(blocks.ops, "norm_quant", launch)
+    tensor = lambda i: SimpleNamespace(dim=lambda: 2, shape=(1, 128), get_device=lambda: i)  # noqa: E731
+    plan = SimpleNamespace(head_dim=64, rotary_dim=64, interleaved=False)
+    for hidden, block, cache in ((1, 1, 1), (0, 0, 0), (0, 1, 1), (1, 0, 1), (1, 1, 0)):
+        blk.in_norm = tensor(block)
+        kv = SimpleNamespace(kv_heads=1, head_dim=64, device=torch.device("cuda", cache), _index=cache)
+        call = lambda: blk.step(tensor(hidden), kv, plan, positions=None)  # noqa: E731
+        if hidden == block == cache:
+            with pytest.raises(Launched, match=str(hidden)):
+                call()
+        else:
+            with pytest.raises(ValueError, match="one device"):
+                call()
+    assert now == [0]
