@@ -20,13 +20,14 @@ from typing import List, Optional, Tuple
 import torch
 
 
-# 2 pi, and the digits that frequencies are computed with: a fixed-point word of 64 bits takes 20
-# digits behind the point, the rest is room for small factors.
-_TWO_PI = Decimal("6.28318530717958647692528676655900576839433879875021164194989")
-_DIGITS = 55
+# Frequencies are computed in whole multiples of 2^-192, which _DIGITS decimal digits hold.
+_BITS, _DIGITS = 192, 70
+_TWO_PI = Decimal("6.2831853071795864769252867665590057683943387987502116419498891846156328125724")
+with localcontext(Context(prec=_DIGITS)):
+    _TURNS = int((1 << _BITS) / _TWO_PI)  # of a radian
 
 
-def _exact(rotary_dim: int, theta: float, scaling: Optional[dict]) -> Tuple[List[Decimal], float]:
+def _exact(rotary_dim: int, theta: float, scaling: Optional[dict]) -> Tuple[List[int], float]:
     half = rotary_dim // 2
     opts = dict(scaling or {"kind": "none"})
     kind = opts.pop("kind", None)
@@ -39,14 +40,17 @@ def _exact(rotary_dim: int, theta: float, scaling: Optional[dict]) -> Tuple[List
     factor = float(opts.get("factor", 1.0))
     if kind != "none" and "factor" not in opts or not factor > 0 or not math.isfinite(factor):
         raise ValueError("scaling needs a factor > 0")
-    log_theta, stretch = Decimal(float(theta)).ln(), Decimal(factor)
-    if kind == "ntk":
-        log_theta += stretch.ln() * half / (half - 1)
-    step, w = (-log_theta / half).exp(), [Decimal(1)]
-    while len(w) < half:  # half <= 128 products lose 3 of the digits
-        w.append(w[-1] * step)
+    with localcontext(Context(prec=_DIGITS)):
+        log_theta = Decimal(float(theta)).ln()
+        if kind == "ntk":
+            log_theta += Decimal(factor).ln() * half / (half - 1)
+        step = int((-log_theta / half).exp() * (1 << _BITS))
+    w = [1 << _BITS]
+    while len(w) < half:  # half <= 128 products, each cut off by less than 2^-192
+        w.append(w[-1] * step >> _BITS)
+    num, den = factor.as_integer_ratio()
     if kind == "linear":
-        return [x / stretch for x in w], 1.0
+        return [x * den // num for x in w], 1.0
     if kind != "yarn":
         return w, 1.0
     length = opts.get("original_length")
@@ -58,19 +62,18 @@ def _exact(rotary_dim: int, theta: float, scaling: Optional[dict]) -> Tuple[List
         return half * math.log(length / (turns * 2 * math.pi)) / math.log(theta)
 
     lo, hi = max(math.floor(at(fast)), 0), min(math.ceil(at(slow)), rotary_dim - 1)
-    ramp = [min(max(Decimal(i - lo) / max(hi - lo, 1), Decimal(0)), Decimal(1))
-            for i in range(half)]
+    span = max(hi - lo, 1)
+    ramp = [min(max(i - lo, 0), span) for i in range(half)]  # of the span
     magnitude = opts.get("magnitude")
     if magnitude is None:
         magnitude = 0.1 * math.log(factor) + 1.0
-    return [x * (1 - r) + x / stretch * r for x, r in zip(w, ramp)], float(magnitude)
+    return [(x * (span - r) + x * den // num * r) // span for x, r in zip(w, ramp)], float(magnitude)
 
 
 def frequencies(rotary_dim: int, theta: float, scaling: Optional[dict] = None):
     """(w_i in radians per position as a list of floats, magnitude of the rotated elements)."""
-    with localcontext(Context(prec=_DIGITS)):
-        w, magnitude = _exact(rotary_dim, theta, scaling)
-    return [float(x) for x in w], magnitude
+    w, magnitude = _exact(rotary_dim, theta, scaling)
+    return [x / (1 << _BITS) for x in w], magnitude
 
 
 class RotaryPlan:
@@ -95,10 +98,11 @@ class RotaryPlan:
             raise ValueError("theta must be > 1")
         self.head_dim, self.rotary_dim, self.theta = head_dim, rotary_dim, float(theta)
         self.interleaved = layout == "interleaved"
-        with localcontext(Context(prec=_DIGITS)):
-            w, self.magnitude = _exact(rotary_dim, float(theta), scaling)
-            fixed = [int((x / _TWO_PI * (1 << 64)).to_integral_value()) % (1 << 64) for x in w]
-        self.radians = [float(x) for x in w]
+        w, self.magnitude = _exact(rotary_dim, float(theta), scaling)
+        self.radians = [x / (1 << _BITS) for x in w]
+        # w / (2 pi) at twice the bits, rounded to 64
+        cut = 2 * _BITS - 64
+        fixed = [(x * _TURNS + (1 << cut - 1) >> cut) % (1 << 64) for x in w]
         self.freqs = torch.tensor([f - (1 << 64) if f >= 1 << 63 else f for f in fixed],
                                   dtype=torch.int64, device=device)
         self.known_calls = {}  # of ops.rotary
