@@ -11,14 +11,17 @@
 // conversions (cvt.rn.f16x2.e2m1x2) and the scalings (multiplications of f16 pairs) take 2 clocks
 // each and the matrix instructions another 2, on three different pipes.
 //
-// Measured (device time, bytes of the cache over it), head_dim 128, 8 kv heads of 4 query heads:
-//   2 sequences of 131072 keys             64 us   4.7 TB/s   issue slots 55 % busy
+// Measured (device time in a replayed graph, bytes of the cache over it), head_dim 128, 8 kv heads of
+// 4 query heads, calls without starts:
+//   2 sequences of 131072 keys             64 us   4.7 TB/s   issue slots 55 %, DRAM 54 % busy
 //   64 sequences of up to 8191, 273K keys  74 us   4.2 TB/s
-//   1 sequence of 197                       9.2 us (launch, one unit's latency, no join)
+//   1 sequence of 197                       9.2 us (launch, one unit's latency; no join, for the table
+//                                          holds 208 tokens; 11.1 with a table of 8192)
 //   head_dim 256, 4 kv heads, gate, e4m3; 16 sequences of up to 4000, 40K keys
 //                                          26.5 us  1.7 TB/s
-// About 10 us of each are ends: finding the run of units, the first pages' latency, cold
-// instructions, and the join (5 us); between them pages arrive at 5.6 TB/s.
+// About 10 us of each are ends, by the call on 197 keys in a wide table: finding the run of units, the
+// first pages' latency, cold instructions, and the join.  Without these the long case has 5.6 TB/s
+// and the batch 4.9, and neither the issue slots nor DRAM are full.
 //
 // How the work is laid out
 //  - Keys on the rows of the matrix instruction (m16n8k16, f16 in, f32 out): S^T = K Q^T and
@@ -745,7 +748,9 @@ int b2f_kv4_attention(const b2f_kv4_attn_args* a, b2f_stream_t stream) {
   p.partial = reinterpret_cast<float*>(a->workspace);
   cudaStream_t s = (cudaStream_t)stream;
   if (kv4_tiles_fit(rows_of_a_sequence(a))) return kv4_tiles_launch(p, sms, s);
-  // 16 rows a tile read every key half as often as 8 do, once there are more than 8.
+  // 16 rows a tile read every key half as often as 8 do, once there are more than 8.  With starts the
+  // host knows no lengths, and takes all tokens for one sequence's: 64 single tokens of 4 query heads
+  // a kv head, 273K keys, 116 us with starts and 77 without (head_dim 64: 81 and 57).
   const long long most = a->batch.starts != nullptr ? a->batch.tokens : a->batch.tokens / a->batch.seqs;
   const int rows = tile_rows(d, most * p.group);
   if (d == 64) return rows == 8 ? launch_attention<64, 1, 4, 3>(p, sms, s) : launch_attention<64, 2, 4, 2>(p, sms, s);

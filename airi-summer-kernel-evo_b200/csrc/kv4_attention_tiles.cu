@@ -27,6 +27,10 @@
 // exponentials each: 2048 clocks of the exponential unit) to P V to S, is longer than the other
 // tile's share can hide.  Tried and no faster: S in halves of 64 keys (199 us against 193), two
 // warps for the products (219; with halves 199), rings of two for K and for V apart (the same).
+// The 128 registers of a thread do not hold all that the roles have: spilled are, stored and loaded, 8
+// and 20 bytes at D = 128, 40 and 80 at 64, 56 and 116 at 256.  At D = 256 a CTA has one tile and a ring
+// of two operands, so that the parts of a step follow one another: a chunk of 512 tokens, 16 heads on
+// 4, 8192 keys, 175 us; 32 heads of 64 on 8, 92 us.
 #include <cfloat>
 #include <climits>
 
@@ -682,6 +686,9 @@ int launch_tiles(Kv4AttnParams& p, int sms, cudaStream_t s) {
 //   D 128, 16 sequences of 1024   24 / 22    26 / 30    46 / 75
 //   D 128, 1 sequence of 1024     21 / 16    23 / 18    31 / 31
 //   D 256, 4 sequences of 2048    38 / 34    43 / 52    79 / 150
+// The average is all that the host knows of a call with starts, and misjudges mixed ones: D 128, 512
+// tokens over 8192 keys take 117 us in this form, 63 single tokens over 265K keys 116 in the other, and
+// both in one call 466 (36 rows on average, the other form; with 2048 tokens, 132 rows, this one: 740).
 bool kv4_tiles_fit(long long rows) { return rows >= 96; }
 
 long long kv4_tiles_workspace(int head_dim, int sms) {

@@ -19,7 +19,7 @@
 // pool of 6000 pages 43.9 us: 6 for the plan, 28.5 for moving 100 MB (7.0 TB/s read and written:
 // some of it stays in the L2 cache), the rest the rewriting of tables and two launches; fork of 8
 // sequences of up to 1500 tokens eight times 11.1 us, 7.5 of them the plan: a chain of a few
-// dependent loads and barriers.
+// dependent loads and barriers; extend of 64 rows by a token 3.3 us with 8192 pages, 3.8 with 65536.
 #include <algorithm>
 #include <new>
 #include <string>
