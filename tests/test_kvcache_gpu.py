@@ -921,3 +921,73 @@ def test_attention_of_many_sequences(d, seqs, new, starts, empty):
     lse = torch.full((at[-1], heads), float("nan"), device="cuda")
     c.attention(q.cuda(), heads=heads, starts=_ints(at) if starts else None, out=out, lse=lse)
     _check_attention(c, q, out, lens, at, heads, lse=lse)
+
+
+@pytest.mark.parametrize("d,seqs,kv,group,new", [
+    (64, 170, 1, 4, 1), (64, 1500, 1, 2, 1), (128, 600, 2, 4, 1), (128, 200, 1, 16, 5),
+    (256, 600, 1, 2, 1), (256, 170, 1, 8, 3), (64, 3, 2, 8, 11)])
+def test_many_sequences_in_a_short_table(d, seqs, kv, group, new):
+    """Tables so short that items are not cut: more items than CTAs, several row tiles a sequence,
+    sequences without keys, fewer keys than new tokens."""
+    g = gen(d + seqs)
+    most = 112 if d == 256 else 240
+    lens = [0 if i % 6 == 5 else 1 + (i * 53) % most for i in range(seqs)]
+    c, _, _, _ = _filled(lens, None, kv=kv, d=d, page=16, g=g, garbage=True)
+    heads = kv * group
+    for starts in (None, [i * new for i in range(seqs + 1)]):
+        q = randn((seqs * new, heads * d), g).to(BF16)
+        out = torch.full((seqs * new, heads * d), float("nan"), dtype=BF16, device="cuda")
+        lse = torch.full((seqs * new, heads), float("nan"), device="cuda")
+        c.attention(q.cuda(), heads=heads, starts=None if starts is None else _ints(starts), out=out,
+                    lse=lse)
+        _check_attention(c, q, out, lens, [i * new for i in range(seqs + 1)], heads, lse=lse)
+
+
+def test_first_calls_inside_a_capture():
+    """A graph may be captured before any call has run eagerly: the same as the eager calls."""
+    import subprocess
+    import sys
+    code = """
+import sys, torch
+sys.path[:0] = [%r, %r]
+from b200fp8 import device_status, kvcache, ops, rotary
+ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+torch.manual_seed(3)
+make = lambda: kvcache.Fp4Cache(layers=1, pages=400, page_size=16, kv_heads=1, head_dim=64,
+                                max_seqs=4, max_pages=90, k_scale=0.25, v_scale=0.25)
+plan = rotary.RotaryPlan(64, device="cuda")
+counts, src, dst, back = ints([1100, 700, 0, 0]), ints([0]), ints([2]), ints([1])
+k, v, q = (torch.randn(1800, h * 64, device="cuda").bfloat16() for h in (1, 1, 4))
+starts, pos = ints([0, 1100, 1800]), torch.arange(1800, device="cuda", dtype=torch.int32)
+
+def calls(c):
+    c.extend(counts)
+    qr, kr = ops.rotary(q, k, pos, plan, heads=4, kv_heads=1)
+    c.write(kr, v, rows=ints_01, starts=starts)
+    c.fork(src, dst)
+    c.free(back)
+    c.compact()
+    one = c.attention(qr[:1], heads=4, rows=dst)
+    many = c.attention(qr[:300], heads=4, rows=src)
+    return (one, many, *c.read(1100, rows=dst))
+
+ints_01 = ints([0, 1])
+a, b = make(), make()
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = calls(a)
+graph.replay()
+want = calls(b)
+torch.cuda.synchronize()
+assert all(torch.equal(x, y) for x, y in zip(got, want))
+assert torch.equal(a.table, b.table) and torch.equal(a.refs, b.refs) and torch.equal(a.lens, b.lens)
+assert device_status() == 0 and a.lens.tolist() == [1100, 0, 1100, 0]
+print("same")
+"""
+    import pathlib
+    root = pathlib.Path(__file__).resolve().parents[1]
+    run = subprocess.run([sys.executable, "-c", code % (str(root / "airi-summer-kernel-evo_b200"),
+                                                        str(root))],
+                         capture_output=True, text=True, timeout=300)
+    assert run.stdout.strip() == "same", run.stderr[-2000:]
